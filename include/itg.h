@@ -421,6 +421,52 @@ int itg_adam_ema_step(float* p, const float* g, float* m, float* v, float* ema, 
                       float beta1, float beta2, float eps, int step, const int32_t* step_dev, float ema_decay,
                       void* stream);
 
+/* ---- layer norm (type_norm_G = LN; the reference normalises with nn.BatchNorm2d / SSM only, models/layers.py:279-290) ----------
+ * Rows of c values at a stride of ld* elements (any stride >= c; any alignment the element type allows):
+ *   y = act(gamma (x - mean) / sqrt(var + eps) + beta)     mean, var: of the row's c values, fp32 for every type
+ * gamma / beta: c values or NULL (1 / 0).  `pad` channels of zeros are written behind the c of y (a patch-grid tensor: pad =
+ * ld - c, dtype ITG_F32).  dtype: ITG_F32 | ITG_BF16 | ITG_F16 of x, y, dy, dx; param_dtype: of gamma, beta and their gradients,
+ * ITG_F32 or dtype.  mean_rstd: [rows][2] floats for the backward pass, or NULL.  y may be x (dx may be dy or x).
+ * bwd: dx, dgamma, dbeta may each be NULL; accumulate: ITG_ACC_DW adds into dgamma / dbeta.  workspace:
+ * itg_layer_norm_bwd_workspace(rows, c) floats (shares of dgamma | dbeta, added in a fixed order), needed with dgamma / dbeta.  */
+enum { ITG_F32 = 0, ITG_BF16 = 1, ITG_F16 = 2 };
+#define ITG_LN_MAX_C (1 << 24)
+int itg_layer_norm_fwd(const void* x, int64_t ldx, const void* gamma, const void* beta, void* y, int64_t ldy, float* mean_rstd,
+                       int64_t rows, int c, int pad, int dtype, int param_dtype, float eps, int act, float slope, void* stream);
+int64_t itg_layer_norm_bwd_workspace(int64_t rows, int c);
+int itg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, const float* mean_rstd, const void* gamma,
+                       const void* beta, void* dx, int64_t lddx, void* dgamma, void* dbeta, int accumulate, int64_t rows, int c,
+                       int pad, int dtype, int param_dtype, int act, float slope, float* workspace, int64_t workspace_floats,
+                       void* stream);
+
+/* ---- orthogonalisation by Newton-Schulz products, and the Muon step (train.py --optimizer muon; the reference has Adam only,
+ * train.py:57-58) -----------------------------------------------------------------------------------------------------------
+ * For every matrix G (rows x cols, row-major with a row stride) of a call:  X = G / |G|_F  (zeros where |G|_F <= eps), then
+ * `steps` times  A = X X^T, X <- a X + (b A + c A A) X  (on the transpose where rows > cols), out = X in G's type.
+ * coefficients: HOST array of 3 * steps floats (a, b, c of each step); they must keep the singular values below 3.9 (checked).
+ * dtype: ITG_F32 / ITG_F16 = products as exact as fp32 ones, ITG_BF16 = as exact as the type.  out may be g (same layout).
+ * A job is `count` matrices of one shape at a stride; offsets and strides count elements from g / out.  Matrices of one call
+ * must not overlap in out.  A matrix that holds an infinity or a NaN comes out as NaN, the others of the call as they are.
+ * workspace: itg_newton_schulz_workspace() bytes, 16-byte aligned (-1 .. -4: the jobs are rejected).                            */
+#define ITG_NS_MAX_JOBS 32
+#define ITG_NS_MAX_DIM 65536
+#define ITG_NS_MAX_STEPS 16
+typedef struct {
+  int32_t rows, cols, count, reserved;      /* reserved: 0 */
+  int64_t in_offset, in_ld, in_stride, out_offset, out_ld, out_stride;
+} itg_ns_job;
+int64_t itg_newton_schulz_workspace(const itg_ns_job* jobs, int n, int dtype);
+int itg_newton_schulz(const itg_ns_job* jobs, int n, int dtype, const void* g, void* out, int steps, const float* coefficients,
+                      float eps, void* workspace, int64_t workspace_bytes, void* stream);
+/* One optimiser step over fp32 matrices that live in flat buffers (job: count 1, contiguous, in_offset == out_offset, the same
+ * offset in param, g, momentum and ema):
+ *   momentum <- mu momentum + g;  U = nesterov ? g + mu momentum : momentum;  O = Newton-Schulz(U);
+ *   param <- (1 - lr weight_decay) param - lr sqrt(max(1, rows / cols)) O;  ema <- ema_decay ema + (1 - ema_decay) param (ema may be NULL)
+ * workspace as itg_newton_schulz with ITG_F32.                                                                               */
+int itg_muon_step(const itg_ns_job* jobs, int n, float* param, const float* g, float* momentum, float* ema, float lr, float mu,
+                  int nesterov, float weight_decay, float ema_decay, int steps, const float* coefficients, float eps,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

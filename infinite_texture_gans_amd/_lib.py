@@ -60,6 +60,18 @@ class SnJob(C.Structure):
                 ("d_w_orig", C.c_void_p), ("rows", C.c_int32), ("cols", C.c_int32), ("accumulate", C.c_int32),
                 ("reserved", C.c_int32)]
 
+
+class NsJob(C.Structure):
+    """itg_ns_job: ``count`` matrices of one shape (itg.h)."""
+    _fields_ = [("rows", C.c_int32), ("cols", C.c_int32), ("count", C.c_int32), ("reserved", C.c_int32), ("in_offset", C.c_int64),
+                ("in_ld", C.c_int64), ("in_stride", C.c_int64), ("out_offset", C.c_int64), ("out_ld", C.c_int64),
+                ("out_stride", C.c_int64)]
+
+
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2      # itg.h ITG_F32 ...
+LN_MAX_C = 1 << 24
+NS_MAX_JOBS, NS_MAX_DIM, NS_MAX_STEPS = 32, 65536, 16
+
 _P = C.c_void_p
 _TP = C.POINTER(Tensor)
 _GP = C.POINTER(ConvGeom)
@@ -140,6 +152,12 @@ SIGNATURES = {
     "itg_spectral_norm_power_iter": (_i, [_P, _P, _P, _i, _i, _i, _f, _P, _P, _P, _P]),
     "itg_spectral_norm_power_iter_multi": (_i, [_i, _P, _P, _P, _P, _P, _i, _f, _P, _P, _P]),
     "itg_spectral_norm_bwd": (_i, [_P, _P, _P, _P, _P, _i, _i, _P, _i, _P, _P]),
+    "itg_layer_norm_fwd": (_i, [_P, _l, _P, _P, _P, _l, _P, _l, _i, _i, _i, _i, _f, _i, _f, _P]),
+    "itg_layer_norm_bwd_workspace": (_l, [_l, _i]),
+    "itg_layer_norm_bwd": (_i, [_P, _l, _P, _l, _P, _P, _P, _P, _l, _P, _P, _i, _l, _i, _i, _i, _i, _i, _f, _P, _l, _P]),
+    "itg_newton_schulz_workspace": (_l, [C.POINTER(NsJob), _i, _i]),
+    "itg_newton_schulz": (_i, [C.POINTER(NsJob), _i, _i, _P, _P, _i, C.POINTER(_f), _f, _P, _l, _P]),
+    "itg_muon_step": (_i, [C.POINTER(NsJob), _i, _P, _P, _P, _P, _f, _f, _i, _f, _f, _i, C.POINTER(_f), _f, _P, _l, _P]),
     "itg_adam_ema_step": (_i, [_P, _P, _P, _P, _P, _l, _f, _f, _f, _f, _i, _P, _f, _P]),
 }
 

@@ -1157,6 +1157,123 @@ def ssm_modulate(x, emb, rm, rv, nbt, training=True, eps=1e-5, momentum=0.1, act
     return GT(t, x.c)
 
 
+# ------------------------------------------------------------------------------- layer norm
+_DTYPES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+
+
+def _on(t):
+    """Launch on ``t``'s device: a device guard where it is not the current one."""
+    return _NullCtx() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _row_stride(t):
+    """Elements between two rows of ``t`` seen as (rows, t.shape[-1]), or None where it has no single row stride."""
+    if t.dim() == 1 or t.numel() == t.shape[-1]:
+        return t.shape[-1] if t.shape[-1] == 1 or t.stride(-1) == 1 else None
+    if t.shape[-1] != 1 and t.stride(-1) != 1:
+        return None
+    dims = [(s, st) for s, st in zip(t.shape[:-1], t.stride()[:-1]) if s != 1]
+    for (_, outer), (size, inner) in zip(dims, dims[1:]):
+        if outer != size * inner:
+            return None
+    return dims[-1][1] if dims[-1][1] >= t.shape[-1] else None
+
+
+def _rows(t):
+    """(tensor whose rows are at one stride, that stride): ``t`` itself, or a contiguous copy."""
+    ld = _row_stride(t)
+    return (t, ld) if ld is not None else (t.contiguous(), t.shape[-1])
+
+
+class _LayerNorm(torch.autograd.Function):
+    """y = act(gamma * xhat + beta), xhat = the row's values normalised with their own mean and variance; ``c`` of the
+    x.shape[-1] values of a row are channels, the rest (patch-grid padding) is written as zeros."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, c, eps, act, slope, sinks):
+        dt = _DTYPES[x.dtype]
+        pdt = _DTYPES[gamma.dtype if gamma is not None else beta.dtype] if gamma is not None or beta is not None else dt
+        x, ldx = _rows(x)
+        width = x.shape[-1]
+        rows = x.numel() // width
+        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        grads = any(ctx.needs_input_grad[:3])
+        stat = torch.empty(2 * rows, device=x.device, dtype=torch.float32) if grads else None
+        if rows:
+            with _on(x):
+                _lib.call("itg_layer_norm_fwd", _ptr(x), ldx, _ptr(gamma), _ptr(beta), _ptr(y), width, _ptr(stat), rows, c, width - c,
+                          dt, pdt, eps, act, slope, _stream())
+        if grads:
+            ctx.meta = (c, dt, pdt, act, slope)
+            ctx.sinks = sinks
+            ctx.save_for_backward(x, gamma, beta, stat)
+        if act == ACT_LRELU and dt == _lib.DT_F32:
+            _sink_act(y, c, act, "ln")
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, gamma, beta, stat = ctx.saved_tensors
+        c, dt, pdt, act, slope = ctx.meta
+        need = ctx.needs_input_grad
+        x, ldx = _rows(x)
+        dy, ldy = _rows(dy)
+        width = x.shape[-1]
+        rows = x.numel() // width
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
+        acc = 0
+        dg = db = None
+        if ctx.sinks is not None and (need[1] or need[2]):
+            (dg, db), acc = ctx.sinks, ACC_DW
+        else:
+            dg = torch.empty_like(gamma) if need[1] else None
+            db = torch.empty_like(beta) if need[2] else None
+        if rows:
+            n = _lib.fn("itg_layer_norm_bwd_workspace")(rows, c) if dg is not None or db is not None else 0
+            ws = torch.empty(n, device=x.device, dtype=torch.float32) if n else None
+            with _on(x):
+                _lib.call("itg_layer_norm_bwd", _ptr(x), ldx, _ptr(dy), ldy, _ptr(stat), _ptr(gamma), _ptr(beta), _ptr(dx), width,
+                          _ptr(dg), _ptr(db), acc, rows, c, width - c, dt, pdt, act, slope, _ptr(ws), n, _stream())
+        elif not acc:
+            dg, db = (t.zero_() if t is not None else None for t in (dg, db))
+        return (dx, None, None) + (None,) * 5 if acc else (dx, dg, db) + (None,) * 5
+
+
+def layer_norm(x, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, slope=0.0, sinks=None):
+    """act((x - mean) / sqrt(var + eps) * gamma + beta) over the channels of every pixel of a patch-grid activation (GT), or over
+    the last dimension of a float32 / bfloat16 / float16 tensor of any strides (one row stride: read in place; else copied).
+
+    ``gamma`` / ``beta``: one value per channel, contiguous, float32 or x's type, both alike; None = 1 / 0.  Statistics and sums are
+    fp32.  No running statistics: training and evaluation are the same function.  ``sinks`` = (gamma.grad, beta.grad) buffers
+    the backward accumulates into.  The activation's derivative at 0 is that of its negative side.  A NaN or an infinity in a
+    row makes that row NaN."""
+    grid = isinstance(x, GT)
+    t, c = (x.t, x.c) if grid else (x, x.shape[-1] if x.dim() else 0)
+    if grid:
+        _req_cuda(t, "layer_norm input")
+    elif not t.is_cuda or t.dtype not in _DTYPES:
+        raise _lib.ItgError("layer_norm: x must be a float32, bfloat16 or float16 tensor on the GPU, got %s on %s" % (t.dtype, t.device))
+    if c < 1 or c > _lib.LN_MAX_C:
+        raise _lib.ItgError("layer_norm: %d channels (1 .. %d are supported)" % (c, _lib.LN_MAX_C))
+    types = set()
+    for name, v in (("gamma", gamma), ("beta", beta)):
+        if v is None:
+            continue
+        if tuple(v.shape) != (c,) or v.device != t.device or not v.is_contiguous() or v.dtype not in (torch.float32, t.dtype):
+            raise _lib.ItgError("layer_norm: %s must be %d contiguous values on x's device, float32 or x's type, got %s %s"
+                                % (name, c, tuple(v.shape), v.dtype))
+        types.add(v.dtype)
+    if len(types) > 1:
+        raise _lib.ItgError("layer_norm: gamma and beta must be of one type")
+    if act not in (ACT_NONE, ACT_LRELU, ACT_TANH) or not eps >= 0.0:
+        raise _lib.ItgError("layer_norm: unknown activation %r or negative eps %r" % (act, eps))
+    if sinks is not None and (gamma is None or beta is None or any(s is None or s.dtype != gamma.dtype or tuple(s.shape) != (c,)
+                                                                   or not s.is_contiguous() or s.device != t.device for s in sinks)):
+        raise _lib.ItgError("layer_norm: sinks are two contiguous buffers like gamma and beta")
+    y = _LayerNorm.apply(t, gamma, beta, c, float(eps), int(act), float(slope), sinks)
+    return GT(y, c) if grid else y
+
+
 # ------------------------------------------------------------------------------- pointwise
 class _Act(torch.autograd.Function):
     @staticmethod
@@ -1605,3 +1722,132 @@ def adam_ema_step(p, g, m, v, ema, lr, beta1, beta2, eps, step, ema_decay=0.999,
     step count (graph-replay safe); else the host integer ``step``."""
     _lib.call("itg_adam_ema_step", _ptr(p), _ptr(g), _ptr(m), _ptr(v), _ptr(ema), p.numel(), float(lr), float(beta1),
               float(beta2), float(eps), int(step), _ptr(step_dev), float(ema_decay), _stream())
+
+
+# ------------------------------------------------------------------------------- orthogonalised updates
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _ns_coefficients(coefficients, steps):
+    """(ctypes array of 3 * steps floats, steps) of one (a, b, c) for every step or of one triple per step."""
+    co = list(coefficients)
+    if len(co) == 3 and not isinstance(co[0], (tuple, list)):
+        co = [tuple(co)] * int(steps)
+    if len(co) != steps or not 1 <= len(co) <= _lib.NS_MAX_STEPS or any(len(c) != 3 for c in co):
+        raise _lib.ItgError("Newton-Schulz: 1 .. %d steps with three coefficients each, got %r for %r steps"
+                            % (_lib.NS_MAX_STEPS, coefficients, steps))
+    return (C.c_float * (3 * len(co)))(*[float(v) for c in co for v in c]), len(co)
+
+
+def _ns_workspace(jobs, n, dtype, device):
+    need = _lib.fn("itg_newton_schulz_workspace")(jobs, n, dtype)
+    if need < 0:
+        raise _lib.ItgError("Newton-Schulz: matrices of 1 .. %d rows and columns expected" % _lib.NS_MAX_DIM)
+    return torch.empty(need, device=device, dtype=torch.uint8), need
+
+
+def orthogonalize(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-12, out=None):
+    """The matrices (..., rows, columns) of ``g`` with their singular values driven towards 1 by ``steps`` Newton-Schulz products
+    (the direction of a Muon update; no gradient flows through it).
+
+    float32 / float16: products as exact as fp32 ones; bfloat16: as exact as the type.  ``g`` may be strided (row- or column-major
+    matrices at one batch stride are read in place).  ``coefficients``: (a, b, c) of X <- a X + (b A + c A A) X, or one triple per
+    step.  A matrix with a norm of ``eps`` or less has no direction and gives zeros; one with a NaN or an infinity gives NaN.
+    ``out``: a contiguous tensor like ``g`` for the result; may be ``g`` itself where that is contiguous."""
+    if not g.is_cuda or g.dtype not in _DTYPES:
+        raise _lib.ItgError("orthogonalize: a float32, bfloat16 or float16 tensor on the GPU expected, got %s on %s" % (g.dtype, g.device))
+    if g.dim() < 2:
+        raise _lib.ItgError("orthogonalize: matrices (..., rows, columns) expected, got shape %s" % (tuple(g.shape),))
+    if not eps >= 0.0:
+        raise _lib.ItgError("orthogonalize: negative eps %r" % (eps,))
+    co, steps = _ns_coefficients(coefficients, steps)
+    rows, cols = g.shape[-2:]
+    if out is not None and (out.shape != g.shape or out.dtype != g.dtype or out.device != g.device or not out.is_contiguous()
+                            or (out.data_ptr() == g.data_ptr() and not g.is_contiguous())):
+        raise _lib.ItgError("orthogonalize: out must be a contiguous tensor of g's shape, type and device")
+    g = g.detach()
+    result = out if out is not None else torch.empty(g.shape, device=g.device, dtype=g.dtype)
+    if not g.numel():
+        return result
+    m, o = g.view(-1, rows, cols) if g.is_contiguous() else _matrices(g), result.view(-1, rows, cols)
+    flip = m.stride(-1) != 1 and cols > 1      # column-major: the transposes, whose orthogonalisation is the transpose
+    if flip:
+        m = m.mT
+        o = torch.empty(m.shape, device=g.device, dtype=g.dtype)
+    count, r, c = m.shape
+    job = _lib.NsJob(r, c, count, 0, 0, max(m.stride(1), c), m.stride(0) if count > 1 else r * c, 0, c, r * c)
+    dt = _DTYPES[g.dtype]
+    ws, need = _ns_workspace(C.byref(job), 1, dt, g.device)
+    with _on(g):
+        _lib.call("itg_newton_schulz", C.byref(job), 1, dt, _ptr(m), _ptr(o), steps, co, float(eps), _ptr(ws), need, _stream())
+    if flip:
+        result.view(-1, rows, cols).copy_(o.mT)
+    return result
+
+
+def _matrices(g):
+    """``g`` as (count, rows, columns) with unit stride along rows or columns and one batch stride: a view, or a copy."""
+    rows, cols = g.shape[-2:]
+    try:
+        m = g.view(-1, rows, cols)
+    except RuntimeError:
+        return g.reshape(-1, rows, cols).contiguous()
+    sr, sc = m.stride(1), m.stride(2)
+    if (sc == 1 or cols == 1) and (sr >= cols or rows == 1):
+        return m
+    if (sr == 1 or rows == 1) and (sc >= rows or cols == 1):
+        return m
+    return m.contiguous()
+
+
+class MuonPlan:
+    """The filter matrices of a flat fp32 parameter buffer: ``shapes`` = (rows, columns) of each, one behind the other from
+    element ``offset`` on.  Holds the job table and the workspace of :func:`muon_step`; steps of one plan have to be ordered
+    (they share parameters, momentum and workspace)."""
+
+    def __init__(self, shapes, device, offset=0):
+        self.shapes = [(int(r), int(c)) for r, c in shapes]
+        if not self.shapes or offset < 0:
+            raise _lib.ItgError("MuonPlan: at least one matrix and an offset of 0 or more expected")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise _lib.ItgError("MuonPlan: the parameters must live on the GPU: this build has no CPU path")
+        jobs, at = [], int(offset)
+        for r, c in self.shapes:
+            jobs.append(_lib.NsJob(r, c, 1, 0, at, c, 0, at, c, 0))
+            at += r * c
+        self.end = at          # the buffers hold at least this many values
+        self.calls, need = [], 0
+        for i in range(0, len(jobs), _lib.NS_MAX_JOBS):
+            part = jobs[i:i + _lib.NS_MAX_JOBS]
+            arr = (_lib.NsJob * len(part))(*part)
+            size = _lib.fn("itg_newton_schulz_workspace")(arr, len(part), _lib.DT_F32)
+            if size < 0:
+                raise _lib.ItgError("MuonPlan: matrices of 1 .. %d rows and columns expected, got %s" % (_lib.NS_MAX_DIM, self.shapes))
+            self.calls.append((arr, len(part)))
+            need = max(need, size)
+        self.workspace = torch.empty(need, device=self.device, dtype=torch.uint8)
+
+
+def muon_step(plan, p, g, momentum_buf, ema=None, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, ema_decay=0.999, steps=5,
+              coefficients=NS_COEFFICIENTS, eps=1e-12):
+    """One Muon step (+EMA) over the matrices of ``plan`` in flat fp32 buffers, in place:
+    m <- momentum m + g;  u = g + momentum m (nesterov) or m;  p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) NS(u);
+    ema <- ema_decay ema + (1 - ema_decay) p.  Values outside the plan's matrices are not touched."""
+    for name, t in (("p", p), ("g", g), ("momentum_buf", momentum_buf), ("ema", ema)):
+        if t is None and name == "ema":
+            continue
+        _req_cuda(t, "muon_step: " + name)
+        if not t.is_contiguous() or t.numel() < plan.end or t.device != p.device:
+            raise _lib.ItgError("muon_step: %s must be a contiguous buffer of at least %d values on one device" % (name, plan.end))
+    if p.device != plan.workspace.device:
+        raise _lib.ItgError("muon_step: the plan was made for %s, the parameters are on %s" % (plan.workspace.device, p.device))
+    if not eps >= 0.0:
+        raise _lib.ItgError("muon_step: negative eps %r" % (eps,))
+    co, steps = _ns_coefficients(coefficients, steps)
+    with _on(p):
+        st = _stream()
+        for jobs, n in plan.calls:
+            _lib.call("itg_muon_step", jobs, n, _ptr(p), _ptr(g), _ptr(momentum_buf), _ptr(ema), float(lr), float(momentum),
+                      int(bool(nesterov)), float(weight_decay), float(ema_decay), steps, co, float(eps), _ptr(plan.workspace),
+                      plan.workspace.numel(), st)

@@ -143,3 +143,63 @@ def test_bn_bwd_fuse_is_an_input_gradient_argument_only(lib):
     assert so.itg_conv2d_wgrad(ctypes.byref(ok), ctypes.byref(ok), panel, None, ctypes.byref(g), 0, None, 0, None) < 0
     assert so.itg_conv2d_dgrad(ctypes.byref(ok), panel, None, ctypes.byref(ok), None, 0, f0, ctypes.byref(g), None, 0, None) < 0
     assert g.bn_bwd.contents.taken == 0
+
+
+def test_training_operators_reject_bad_calls_on_the_host(lib):
+    """layer norm, Newton-Schulz and Muon entry points: every rejection happens before a launch (there is no GPU in this tier)"""
+    so = lib.load()
+    f, p = ctypes.c_float, ctypes.c_void_p
+    q = p(4096)
+
+    def fwd(x=q, ldx=8, y=q, ldy=8, stat=None, rows=4, c=8, pad=0, dt=0, pdt=0, eps=1e-5, act=0):
+        return so.itg_layer_norm_fwd(x, ldx, None, None, y, ldy, stat, rows, c, pad, dt, pdt, f(eps), act, f(0.0), None)
+
+    assert fwd(x=None) == -1 and fwd(y=None) == -1 and fwd(rows=0) == -1 and fwd(c=0) == -1 and fwd(c=(1 << 24) + 1) == -1
+    assert fwd(ldx=7) == -1 and fwd(ldy=8, pad=1) == -1 and fwd(pad=-1) == -1 and fwd(dt=3) == -1 and fwd(dt=0, pdt=1) == -1
+    assert fwd(dt=1, pdt=2) == -1 and fwd(eps=-1.0) == -1 and fwd(eps=float("nan")) == -1 and fwd(act=3) == -1
+    assert fwd(x=p(4098)) == -2 and fwd(dt=1, pdt=1, x=p(4097)) == -2 and fwd(stat=p(4097)) == -2
+    assert fwd(rows=1 << 41) == -1 and fwd(rows=1 << 30, ldx=1 << 40) == -1
+    assert so.itg_layer_norm_bwd_workspace(0, 4) == -1 and so.itg_layer_norm_bwd_workspace(1000, 10) > 0
+
+    def bwd(stat=q, dx=q, dg=q, ws=q, n=1 << 20, rows=4, c=8, lddx=8):
+        return so.itg_layer_norm_bwd(q, 8, q, 8, stat, None, None, dx, lddx, dg, None, 0, rows, c, 0, 0, 0, 0, f(0.0), ws, n, None)
+
+    assert bwd(stat=None) == -1 and bwd(ws=None) == -4 and bwd(n=7) == -4 and bwd(lddx=4) == -1 and bwd(ws=p(4097)) == -2
+    assert bwd(dx=None, dg=None) == 0                       # nothing asked for: nothing launched
+
+    def job(rows=4, cols=8, count=1, reserved=0, io=0, il=8, ist=32, oo=0, ol=8, ost=32):
+        return lib.NsJob(rows, cols, count, reserved, io, il, ist, oo, ol, ost)
+
+    def size(j, n=1, dt=0):
+        return so.itg_newton_schulz_workspace(ctypes.byref(j) if j is not None else None, n, dt)
+
+    assert size(job()) > 0 and size(job(), dt=1) > 0
+    for bad in (job(rows=0), job(cols=0), job(rows=65537), job(count=0), job(reserved=1), job(il=7), job(ol=7), job(io=-1), job(oo=-1),
+                job(count=2, ost=31), job(ist=-1), job(il=1 << 62), job(io=(1 << 62)), job(rows=65536, cols=65536, il=65536, ol=65536, count=1 << 30, ost=1 << 40)):
+        assert size(bad) == -1
+    assert size(None) == -1 and size(job(), n=0) == -1 and size(job(), n=33) == -1 and size(job(), dt=5) == -1
+    co = (f * 3)(3.4445, -4.7750, 2.0315)
+
+    def ns(j=job(), n=1, dt=0, g=q, out=q, steps=1, co=co, eps=0.0, ws=q, size=1 << 30):
+        return so.itg_newton_schulz(ctypes.byref(j), n, dt, g, out, steps, co, f(eps), ws, size, None)
+
+    assert ns(g=None) == -1 and ns(out=None) == -1 and ns(steps=0) == -1 and ns(steps=17) == -1 and ns(co=None) == -1 and ns(eps=-1.0) == -1
+    assert ns(co=(f * 3)(9.0, 0.0, 0.0)) == -1 and ns(co=(f * 3)(float("inf"), 0.0, 0.0)) == -1
+    assert ns(ws=None) == -4 and ns(size=16) == -4 and ns(ws=p(4100)) == -2 and ns(g=p(4098)) == -2
+
+    def muon(j=job(ist=0, ost=0), p_=q, g=q, m=q, e=None, ws=q, size=1 << 30):
+        return so.itg_muon_step(ctypes.byref(j), 1, p_, g, m, e, f(0.1), f(0.9), 1, f(0.0), f(0.9), 1, co, f(0.0), ws, size, None)
+
+    assert muon(p_=None) == -1 and muon(g=None) == -1 and muon(m=None) == -1 and muon(e=p(4098)) == -2 and muon(ws=None) == -4
+    assert muon(j=job(count=2)) == -1 and muon(j=job(il=9)) == -1 and muon(j=job(io=1, oo=0)) == -1
+
+
+def test_training_operators_have_no_cpu_path():
+    import torch
+    from infinite_texture_gans_amd import ops
+    from infinite_texture_gans_amd._lib import ItgError
+    x = torch.randn(4, 8)
+    for call in (lambda: ops.layer_norm(x), lambda: ops.orthogonalize(x), lambda: ops.MuonPlan([(4, 8)], "cpu"),
+                 lambda: ops.layer_norm(ops.GT(x.view(1, 1, 1, 1, 4, 8), 8))):
+        with pytest.raises(ItgError):
+            call()

@@ -1,0 +1,307 @@
+"""Layer norm on the GPU against its definition in 64 bits.
+
+Tolerances.  e = 2^-24 is half a step of fp32.  A sum of n terms over `d` sequential additions per thread and a tree is off by at
+most (d + 16) e times the sum of the magnitudes; that gives the mean, the variance, the two row means of the backward pass and the
+column sums.  They enter the results through the formulas as below; the result itself is rounded once to its type (half a step,
+finfo.eps / 2, of the value; below the type's smallest normal number the steps stay eps * smallest_normal apart whatever the
+value, so that half of that, 2^-25 in fp16, is added: a value of 1e-5 may be off by 3e-8, which is 6 times eps / 2 of it)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from infinite_texture_gans_amd import ops as o
+    return o
+
+
+def act_of(u, act, slope):
+    if act == 1:
+        return torch.where(u > 0, u, slope * u), torch.where(u > 0, torch.ones_like(u), torch.full_like(u, slope))
+    if act == 2:
+        return torch.tanh(u), 1 - torch.tanh(u) ** 2
+    return u, torch.ones_like(u)
+
+
+def oracle(x, w, b, dy, eps, act, slope, t, tw):
+    """values and tolerances (y, dx, dw, db) in fp64 for rows x (R, C)"""
+    R, C = x.shape
+    half = 0 if t == torch.float32 else torch.finfo(t).eps / 2
+    halfw = 0 if tw == torch.float32 else torch.finfo(tw).eps / 2
+    least, leastw = (torch.finfo(v).eps * torch.finfo(v).smallest_normal / 2 + 1e-30 for v in (t, tw))
+    d = C / 64 + 16                                   # sequential additions of a row sum (at least 64 threads share it) + tree
+    mean = x.mean(1, keepdim=True)
+    var = ((x - mean) ** 2).mean(1, keepdim=True)
+    r = 1 / torch.sqrt(var + eps)
+    xh = (x - mean) * r
+    dmean = (d + 1) * E * x.abs().mean(1, keepdim=True)
+    # r: the variance is off by (d + 4) e of itself (+ the square of the mean's error); 1 / sqrt halves that, plus its own rounding
+    drel = (d + 8) * E + (dmean * r) ** 2
+    exh = dmean * r + xh.abs() * drel + 2 * E * xh.abs()
+    ww, bb = (w if w is not None else torch.ones(C, dtype=x.dtype, device=x.device)), (b if b is not None else torch.zeros(C, dtype=x.dtype, device=x.device))
+    u = xh * ww + bb
+    eu = exh * ww.abs() + 2 * E * ((xh * ww).abs() + bb.abs())
+    y, slope_at = act_of(u, act, slope)
+    ty = eu * max(1.0, abs(slope)) + (half + 8 * E) * y.abs() + least
+    out = [(y, ty)]
+    if dy is None:
+        return out, u
+    # the activation's slope: exact for the linear pieces, |d tanh'| <= 2 |du| for tanh
+    esl = 2 * eu + 16 * E if act == 2 else torch.zeros_like(u)
+    du = dy * slope_at
+    edu = dy.abs() * esl + 2 * E * du.abs()
+    g = du * ww
+    eg = edu * ww.abs() + 2 * E * g.abs()
+    m1, m2 = g.mean(1, keepdim=True), (g * xh).mean(1, keepdim=True)
+    em1 = (d + 2) * E * g.abs().mean(1, keepdim=True) + eg.mean(1, keepdim=True)
+    em2 = (d + 2) * E * (g * xh).abs().mean(1, keepdim=True) + (eg * xh.abs() + g.abs() * exh).mean(1, keepdim=True)
+    inner = g - m1 - xh * m2
+    dx = r * inner
+    tdx = r * (eg + em1 + xh.abs() * em2 + exh * m2.abs() + 4 * E * (g.abs() + m1.abs() + (xh * m2).abs())) + dx.abs() * (drel + half + 4 * E)
+    n = R + 16
+    dw, db = (du * xh).sum(0), du.sum(0)
+    tdw = n * E * (du * xh).abs().sum(0) + (edu * xh.abs() + du.abs() * exh).sum(0) + (halfw + 4 * E) * dw.abs()
+    tdb = n * E * du.abs().sum(0) + edu.sum(0) + (halfw + 4 * E) * db.abs()
+    return out + [(dx, tdx + least), (dw, tdw + leastw), (db, tdb + leastw)], u
+
+
+def near(got, want, what):
+    v, tol = want
+    got = got.double()
+    assert torch.isfinite(got).all(), what
+    off = (got - v).abs() / tol
+    assert float(off.max()) <= 1.0, "%s: %.3g of the tolerance" % (what, float(off.max()))
+
+
+def make(rows, c, t, tw, seed=0, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(rows, c, generator=g) * (0.3 + torch.rand(c, generator=g)) + spread * torch.randn(rows, 1, generator=g)).to(t)
+    w, b = (1 + 0.3 * torch.randn(c, generator=g)).to(tw), (0.3 * torch.randn(c, generator=g)).to(tw)
+    dy = torch.randn(rows, c, generator=g).to(t)
+    return [v.cuda() for v in (x, w, b, dy)]
+
+
+def run(ops, x, w, b, dy, eps=1e-5, act=0, slope=0.0):
+    x = x.detach().requires_grad_()
+    ps = [p.detach().requires_grad_() if p is not None else None for p in (w, b)]
+    y = ops.layer_norm(x, ps[0], ps[1], eps=eps, act=act, slope=slope)
+    grads = torch.autograd.grad(y, [x] + [p for p in ps if p is not None], dy)
+    return y.detach(), grads
+
+
+SIZES = [(1, 1), (3, 2), (1, 8), (5, 3), (17, 13), (64, 16), (33, 52), (9, 64), (130, 104), (7, 129), (1, 1021), (70, 416), (257, 1024),
+         (3, 2049), (1, 4096), (40, 4096), (2, 8195), (300, 512), (5, 16384), (2, 16389), (3, 40001), (1000, 7), (2049, 26)]
+
+
+@pytest.mark.parametrize("rows,c", SIZES)
+@pytest.mark.parametrize("types", ["f32/f32", "bf16/bf16", "bf16/f32", "f16/f16", "f16/f32"])
+def test_forward_and_gradients(ops, rows, c, types):
+    t, tw = (TYPES[k] for k in types.split("/"))
+    x, w, b, dy = make(rows, c, t, tw, seed=rows + c)
+    y, grads = run(ops, x, w, b, dy)
+    want, _ = oracle(x.double(), w.double(), b.double(), dy.double(), 1e-5, 0, 0.0, t, tw)
+    for got, ref, what in zip((y,) + tuple(grads), want, ("y", "dx", "dw", "db")):
+        near(got, ref, what)
+    assert y.dtype == t and grads[0].dtype == t and grads[1].dtype == tw and grads[2].dtype == tw
+
+
+@pytest.mark.parametrize("act,slope", [(1, 0.0), (1, 0.2), (2, 0.0)])
+@pytest.mark.parametrize("rows,c", [(50, 13), (31, 416), (6, 5000), (2, 20011)])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_activations(ops, rows, c, act, slope, t):
+    x, w, b, dy = make(rows, c, TYPES[t], torch.float32, seed=3)
+    want, u = oracle(x.double(), w.double(), b.double(), dy.double(), 1e-5, act, slope, TYPES[t], torch.float32)
+    if act == 1:      # a value whose sign fp32 cannot tell takes either slope: no gradient passes through it here
+        dy = torch.where(u.abs() < 1e-4, torch.zeros_like(dy), dy)
+        want, u = oracle(x.double(), w.double(), b.double(), dy.double(), 1e-5, act, slope, TYPES[t], torch.float32)
+    y, grads = run(ops, x, w, b, dy, act=act, slope=slope)
+    for got, ref, what in zip((y,) + tuple(grads), want, ("y", "dx", "dw", "db")):
+        near(got, ref, what)
+
+
+def test_gradients_against_differences(ops):
+    """fp32 central differences of <y, q>: an error of h^2 (third derivatives, O(1) here) and of 1e-6 / h in the quotient."""
+    x, w, b, q = make(4, 24, torch.float32, torch.float32, seed=5)
+    _, (dx, dw, db) = run(ops, x, w, b, q, act=2)
+    h = 1e-2
+
+    def f(x, w, b):
+        return float((ops.layer_norm(x, w, b, act=2).double() * q.double()).sum())
+    for t, d in ((x, dx), (w, dw), (b, db)):
+        for i in range(0, t.numel(), 7):
+            e = torch.zeros_like(t).view(-1)
+            e[i] = h
+            e = e.view(t.shape)
+            args = [[a + s * e if a is t else a for a in (x, w, b)] for s in (1, -1)]
+            num = (f(*args[0]) - f(*args[1])) / (2 * h)
+            assert abs(num - float(d.reshape(-1)[i])) < 5e-3 * max(1.0, abs(num)), (i, num, float(d.reshape(-1)[i]))
+
+
+@pytest.mark.parametrize("which", ["none", "gamma", "beta"])
+def test_without_gain_or_shift(ops, which):
+    x, w, b, dy = make(20, 100, torch.float32, torch.float32)
+    w, b = (w if which == "gamma" else None), (b if which == "beta" else None)
+    y, grads = run(ops, x, w, b, dy)
+    want, _ = oracle(x.double(), w.double() if w is not None else None, b.double() if b is not None else None, dy.double(), 1e-5, 0, 0.0,
+                     torch.float32, torch.float32)
+    near(y, want[0], "y")
+    near(grads[0], want[1], "dx")
+    if which != "none":
+        near(grads[1], want[2 if which == "gamma" else 3], which)
+
+
+@pytest.mark.parametrize("c", [1, 3, 13, 52, 104, 416, 700])
+def test_patch_grid(ops, c):
+    """channels 0 .. c of the grid are normalised, the padding channels are written as zeros whatever they held in dy"""
+    shape = (2, 3, 1, 4, 5)
+    n = 2 * 3 * 4 * 5
+    x, w, b, dy = make(n, c, torch.float32, torch.float32, seed=c)
+    ld = ops.ld_for(c)
+    xt = torch.nn.functional.pad(x, (0, ld - c)).view(*shape, ld).requires_grad_()
+    dyt = torch.nn.functional.pad(dy, (0, ld - c), value=7.0).view(*shape, ld)
+    w, b = w.requires_grad_(), b.requires_grad_()
+    y = ops.layer_norm(ops.GT(xt, c), w, b)
+    assert isinstance(y, ops.GT) and y.c == c and y.t.shape == xt.shape
+    grads = torch.autograd.grad(y.t, [xt, w, b], dyt)
+    want, _ = oracle(x.double(), w.detach().double(), b.detach().double(), dy.double(), 1e-5, 0, 0.0, torch.float32, torch.float32)
+    for got, ref, what in zip((y.t.view(n, ld), grads[0].view(n, ld)), want, ("y", "dx")):
+        near(got[:, :c].detach(), ref, what)
+        assert torch.equal(got[:, c:], torch.zeros_like(got[:, c:]))
+    near(grads[1], want[2], "dw")
+    near(grads[2], want[3], "db")
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_strides(ops, t):
+    """slices of a wider buffer (rows in place, also off any vector alignment), leading dimensions, transposes"""
+    t = TYPES[t]
+    base = torch.randn(6, 9, 70, device="cuda").to(t)
+    w, b = torch.randn(33, device="cuda"), torch.randn(33, device="cuda")
+    for x in (base[..., 1:34], base[:, 2:5, 3:36], base[1:4, :, :33], base[:, ::2, 5:38], base.transpose(0, 1)[..., 30:63],
+              base.permute(2, 0, 1)[:33].permute(1, 2, 0), base[0, 0, :33], base[:1, :1, 7:40]):
+        got = ops.layer_norm(x, w, b)
+        same = ops.layer_norm(x.contiguous(), w, b)
+        assert torch.equal(got, same) and got.shape == x.shape and got.is_contiguous()
+        xs, xc = x.detach().requires_grad_(), x.detach().contiguous().requires_grad_()
+        dy = torch.randn(x.shape, device="cuda").to(t)
+        dys = torch.empty(x.shape + (2,), device="cuda", dtype=t)[..., 0].copy_(dy)          # no unit stride
+        g1, = torch.autograd.grad(ops.layer_norm(xs, w, b), xs, dys)
+        g2, = torch.autograd.grad(ops.layer_norm(xc, w, b), xc, dy)
+        assert torch.equal(g1, g2)
+
+
+def test_buffer_behind_the_rows_is_left_alone(ops):
+    """the last row's end: neither the padding behind a strided row nor what follows the last one is written"""
+    import ctypes as C
+    from infinite_texture_gans_amd import _lib
+    for t, dt in ((torch.float32, 0), (torch.bfloat16, 1), (torch.float16, 2)):
+        for c, ld in ((13, 19), (100, 131), (1021, 1021), (5001, 5003)):
+            x = torch.randn(5, ld, device="cuda").to(t)
+            y = torch.full((5 * ld + 64,), 3.0, device="cuda", dtype=t)
+            _lib.call("itg_layer_norm_fwd", C.c_void_p(x.data_ptr()), ld, None, None, C.c_void_p(y.data_ptr()), ld, None, 5, c, 0, dt, dt,
+                      1e-5, 0, 0.0, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+            v = y[:5 * ld].view(5, ld)
+            assert torch.equal(v[:, :c], ops.layer_norm(x[:, :c]))
+            assert torch.equal(v[:, c:], torch.full_like(v[:, c:], 3.0)) and torch.equal(y[5 * ld:], torch.full_like(y[5 * ld:], 3.0))
+
+
+def test_no_rows_and_one_value(ops):
+    w, b = torch.randn(8, device="cuda", requires_grad=True), torch.randn(8, device="cuda", requires_grad=True)
+    x = torch.empty(0, 4, 8, device="cuda", requires_grad=True)
+    y = ops.layer_norm(x, w, b)
+    assert y.shape == x.shape
+    g = torch.autograd.grad(y, [x, w, b], torch.empty_like(y))
+    assert g[0].shape == x.shape and torch.equal(g[1], torch.zeros(8, device="cuda")) and torch.equal(g[2], torch.zeros(8, device="cuda"))
+    one = ops.layer_norm(torch.full((3, 1), 5.0, device="cuda"))          # a single channel: variance 0, y = 0
+    assert torch.equal(one, torch.zeros(3, 1, device="cuda"))
+
+
+@pytest.mark.parametrize("c", [13, 52, 1000, 9000, 40000])
+def test_extreme_rows(ops, c):
+    """constant rows, rows far from zero, rows with an infinity or a NaN: their neighbours stay as they are"""
+    x, w, b, dy = make(9, c, torch.float32, torch.float32, seed=1)
+    x[1] = 4.0
+    x[3] = x[3] + 1000.0
+    clean = ops.layer_norm(x, w, b)
+    want, _ = oracle(x.double(), w.double(), b.double(), None, 1e-5, 0, 0.0, torch.float32, torch.float32)
+    near(clean, want[0], "y")
+    bad = x.clone()
+    bad[5, c // 2], bad[7, c - 1] = float("inf"), float("nan")
+    got = ops.layer_norm(bad, w, b)
+    assert torch.isnan(got[5]).all() and torch.isnan(got[7]).all()
+    keep = [0, 1, 2, 3, 4, 6, 8]
+    assert torch.equal(got[keep], clean[keep])
+
+
+def test_same_result_every_time_and_in_a_graph(ops):
+    """sums have a fixed order: repeated calls, a call on another stream and every replay of a captured training pass agree bit for bit"""
+    x, w, b, dy = make(3000, 52, torch.float32, torch.float32, seed=2)
+    xs, ws, bs = x.clone().requires_grad_(), w.clone().requires_grad_(), b.clone().requires_grad_()
+    first = torch.autograd.grad(ops.layer_norm(xs, ws, bs), [xs, ws, bs], dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = torch.autograd.grad(ops.layer_norm(xs, ws, bs), [xs, ws, bs], dy)
+    torch.cuda.current_stream().wait_stream(side)
+    for p, q in zip(first, again):
+        assert torch.equal(p, q)
+    del first, again, xs, ws, bs
+    static = x.clone()
+    xg, wg, bg = static.requires_grad_(), w.clone().requires_grad_(), b.clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y = ops.layer_norm(xg, wg, bg, act=1, slope=0.1)
+        grads = torch.autograd.grad(y, [xg, wg, bg], dy)
+    for seed in (11, 12, 13):
+        new, _, _, _ = make(3000, 52, torch.float32, torch.float32, seed=seed)
+        with torch.no_grad():
+            static.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        out = [y.detach().clone()] + [t.clone() for t in grads]
+        xe, we, be = new.clone().requires_grad_(), w.clone().requires_grad_(), b.clone().requires_grad_()
+        ye = ops.layer_norm(xe, we, be, act=1, slope=0.1)
+        for p, q in zip(out, (ye.detach(),) + torch.autograd.grad(ye, [xe, we, be], dy)):
+            assert torch.equal(p, q)
+
+
+def test_sinks_accumulate(ops):
+    x, w, b, dy = make(200, 26, torch.float32, torch.float32)
+    w, b = w.requires_grad_(), b.requires_grad_()
+    plain = torch.autograd.grad(ops.layer_norm(x, w, b), [w, b], dy)
+    sinks = (torch.full((26,), 2.0, device="cuda"), torch.full((26,), -1.0, device="cuda"))
+    xs = x.clone().requires_grad_()
+    ops.layer_norm(xs, w, b, sinks=sinks).backward(dy)
+    assert w.grad is None and b.grad is None and xs.grad is not None
+    assert torch.equal(sinks[0], 2.0 + plain[0]) and torch.equal(sinks[1], -1.0 + plain[1])
+
+
+def test_only_some_gradients(ops):
+    x, w, b, dy = make(64, 48, torch.float32, torch.float32)
+    full = run(ops, x, w, b, dy)[1]
+    xs = x.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(ops.layer_norm(xs, w, b), xs, dy)[0], full[0])
+    ws = w.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(ops.layer_norm(x, ws, b), ws, dy)[0], full[1])
+    bs = b.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(ops.layer_norm(x, w, bs), bs, dy)[0], full[2])
+
+
+def test_refusals(ops):
+    from infinite_texture_gans_amd._lib import ItgError
+    x, w = torch.randn(4, 8, device="cuda"), torch.randn(8, device="cuda")
+    for bad in (lambda: ops.layer_norm(x.double()), lambda: ops.layer_norm(x.cpu()), lambda: ops.layer_norm(x, w[:4]),
+                lambda: ops.layer_norm(x, w.cpu()), lambda: ops.layer_norm(x, w.bfloat16()), lambda: ops.layer_norm(x, w.repeat(2)[::2]),
+                lambda: ops.layer_norm(x.bfloat16(), w, w.bfloat16()), lambda: ops.layer_norm(x, w, w, eps=-1.0),
+                lambda: ops.layer_norm(x, w, w, eps=float("nan")), lambda: ops.layer_norm(x, w, w, act=9),
+                lambda: ops.layer_norm(x, w, w, sinks=(w, None)), lambda: ops.layer_norm(x, None, w, sinks=(w, w)),
+                lambda: ops.layer_norm(torch.empty(3, 0, device="cuda")), lambda: ops.layer_norm(torch.zeros((), device="cuda")),
+                lambda: ops.layer_norm(x.int())):
+        with pytest.raises(ItgError):
+            bad()

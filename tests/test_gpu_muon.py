@@ -1,0 +1,254 @@
+"""Newton-Schulz orthogonalisation and the Muon step on the GPU against their definitions in 64 bits.
+
+Tolerances.  fp32 / fp16 matrices: the products are split so that they are as exact as fp32 products.  The oracle runs the same
+steps with torch's fp32 products on the CPU too; the kernel may be off by three times what those are off by (its planes carry 22
+bits where fp32 carries 24: at most twice the rounding of X, plus the products' own), or by 2e-6 where that is less.  fp16 results
+add their rounding, at most 2^-11 of each value; bf16 results: in the 2-norm, 2^-8 in all: rounding takes at most
+2^-9 / sqrt(3) * 1.5 of it (values spread over a binade), and the products of planes of 11 bits (2^-12 a value, two factors, 3.4x
+amplified once) the rest."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+ABC = (3.4445, -4.7750, 2.0315)
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from infinite_texture_gans_amd import ops as o
+    return o
+
+
+def steps_of(x, steps=5, abc=ABC):
+    """the definition on a (rows, cols) CPU matrix in its own precision"""
+    x = x / x.double().norm().to(x.dtype)
+    tall = x.shape[0] > x.shape[1]
+    x = x.T.contiguous() if tall else x
+    for k in range(steps):
+        a, b, c = abc if not isinstance(abc[0], tuple) else abc[k]
+        s = x @ x.T
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return x.T if tall else x
+
+
+def rel(x, y):
+    return float((x.double() - y).norm() / y.norm())
+
+
+def matrix(m, n, seed=0, kind="floor"):
+    g = torch.Generator().manual_seed(seed)
+    k = min(16, m, n)
+    x = torch.randn(m, n, generator=g)
+    if kind == "floor":
+        x = x + torch.randn(m, k, generator=g) @ torch.randn(k, n, generator=g)
+    elif kind == "rank1":
+        x = torch.randn(m, 1, generator=g) @ torch.randn(1, n, generator=g) + 1e-3 * x
+    elif kind == "powers":
+        u, _, v = torch.linalg.svd(x, full_matrices=False)
+        x = u @ torch.diag(1.0 / torch.arange(1, min(m, n) + 1)) @ v
+    return 1e-3 * x
+
+
+def check(got, g, t, steps=5, abc=ABC):
+    got, g = got.cpu(), g.cpu()
+    want = steps_of(g.double(), steps, abc)
+    own = rel(steps_of(g.float(), steps, abc), want)
+    off = rel(got, want)
+    if t == torch.bfloat16:
+        assert off <= 2.0 ** -8 + 3 * own, (off, own)
+    else:
+        assert off <= max(3 * own, 2e-6) + (2.0 ** -11 if t == torch.float16 else 0.0), (off, own)
+
+
+SIZES = [(1, 1), (1, 9), (7, 1), (2, 3), (3, 117), (13, 26), (64, 48), (48, 64), (64, 64), (65, 64), (63, 65), (128, 128), (13, 1000),
+         (1000, 13), (100, 130), (333, 200), (256, 256), (129, 1025), (512, 300), (1, 4099), (520, 700), (200, 4100)]
+
+
+@pytest.mark.parametrize("m,n", SIZES)
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_orthogonalize(ops, m, n, t):
+    g = matrix(m, n, seed=m * 7 + n).cuda().to(TYPES[t])
+    got = ops.orthogonalize(g)
+    assert got.shape == g.shape and got.dtype == g.dtype
+    check(got, g, TYPES[t])
+
+
+@pytest.mark.parametrize("m,n", [(1024, 1024), (1100, 2050), (2304, 1153)])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_orthogonalize_larger(ops, m, n, t):
+    g = matrix(m, n, seed=9).cuda().to(TYPES[t])
+    check(ops.orthogonalize(g), g, TYPES[t])
+
+
+@pytest.mark.parametrize("kind", ["rank1", "powers"])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n", [(64, 64), (40, 300), (256, 192)])
+def test_spectra(ops, kind, t, m, n):
+    """updates of low rank over a faint floor, and spectra that fall off: rounding noise must not be blown up in the empty directions"""
+    g = matrix(m, n, seed=4, kind=kind).cuda().to(TYPES[t])
+    check(ops.orthogonalize(g), g, TYPES[t])
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_batches_and_strides(ops, t):
+    t = TYPES[t]
+    g = torch.stack([matrix(70, 90, seed=s) for s in range(6)]).cuda().to(t).view(2, 3, 70, 90)
+    each = torch.stack([ops.orthogonalize(x) for x in g.view(6, 70, 90)]).view(2, 3, 70, 90)
+    assert torch.equal(ops.orthogonalize(g), each)
+    wide = torch.randn(2, 3, 75, 101, device="cuda").to(t)
+    wide[:, :, 2:72, 5:95] = g
+    assert torch.equal(ops.orthogonalize(wide[:, :, 2:72, 5:95]), each)                        # rows at a stride
+    cols = g.mT.contiguous().mT
+    assert torch.equal(ops.orthogonalize(cols), each)                                          # column-major: the transposes' results
+    assert torch.equal(ops.orthogonalize(g[0, 0].expand(4, 70, 90)), each[0, 0].expand(4, 70, 90))   # one matrix four times
+    inner = g.permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2)                             # no unit stride
+    assert torch.equal(ops.orthogonalize(inner), each)
+    assert torch.equal(ops.orthogonalize(g.transpose(0, 1)), each.transpose(0, 1))
+    vec = torch.randn(5, 40, device="cuda").to(t)
+    assert torch.equal(ops.orthogonalize(vec.T[:, 2:3]), ops.orthogonalize(vec.T[:, 2:3].contiguous()))
+    out = torch.empty_like(g)
+    assert ops.orthogonalize(g, out=out) is out and torch.equal(out, each)
+    same = g.clone()
+    assert ops.orthogonalize(same, out=same) is same and torch.equal(same, each)               # in place
+
+
+def test_scales_zero_and_not_finite(ops):
+    """the result does not depend on the matrix's scale; a zero matrix gives zeros; an infinity or a NaN stays in its own matrix"""
+    base = matrix(40, 60, seed=3).cuda()
+    want = ops.orthogonalize(base)
+    for s in (2.0 ** 70, 2.0 ** -20, 2.0 ** 90):
+        assert torch.equal(ops.orthogonalize(base * s), want)
+    assert torch.equal(ops.orthogonalize(base * 2.0 ** -100, eps=0.0), want)
+    tiny = ops.orthogonalize(base * 2.0 ** -60)                                               # a norm below eps
+    assert torch.equal(tiny, torch.zeros_like(tiny))
+    for t in (torch.float32, torch.bfloat16, torch.float16):
+        g = torch.stack([matrix(40, 60, seed=s) for s in range(5)]).cuda().to(t)
+        clean = ops.orthogonalize(g)
+        g[1], g[2, 3, 4], g[3, 0, 0] = 0.0, float("inf"), float("nan")
+        got = ops.orthogonalize(g, eps=0.0)
+        assert torch.equal(got[1], torch.zeros_like(got[1]))
+        assert torch.isnan(got[2]).all() and torch.isnan(got[3]).all()
+        assert torch.equal(got[0], clean[0]) and torch.equal(got[4], clean[4])
+    assert ops.orthogonalize(torch.empty(0, 4, 5, device="cuda")).shape == (0, 4, 5)
+    assert ops.orthogonalize(torch.empty(3, 0, 5, device="cuda")).shape == (3, 0, 5)
+
+
+def test_coefficients_and_steps(ops):
+    g = matrix(50, 80, seed=8).cuda()
+    check(ops.orthogonalize(g, steps=1), g, torch.float32, 1)
+    check(ops.orthogonalize(g, steps=8, coefficients=(1.875, -1.25, 0.375)), g, torch.float32, 8, (1.875, -1.25, 0.375))
+    each = ((3.4, -4.7, 2.0), (2.5, -2.5, 1.0), (1.875, -1.25, 0.375))
+    check(ops.orthogonalize(g, steps=3, coefficients=each), g, torch.float32, 3, each)
+
+
+def muon_oracle(p, g, m, ema, shapes, at, lr, mu, nesterov, wd, d, dtype):
+    p, g, m = (v.cpu().to(dtype).clone() for v in (p, g, m))
+    ema = ema.cpu().to(dtype).clone() if ema is not None else None
+    for r, c in shapes:
+        s = slice(at, at + r * c)
+        m[s] = mu * m[s] + g[s]
+        u = g[s] + mu * m[s] if nesterov else m[s]
+        p[s] = p[s] * (1 - lr * wd) - lr * math.sqrt(max(1.0, r / c)) * steps_of(u.view(r, c)).reshape(-1)
+        if ema is not None:
+            ema[s] = d * ema[s] + (1 - d) * p[s]
+        at += r * c
+    return p, m, ema
+
+
+SHAPES = [(13, 117), (3, 117), (64, 48), (48, 200), (1, 300), (130, 70), (5, 5)]
+
+
+@pytest.mark.parametrize("nesterov,wd,with_ema,offset", [(True, 0.0, True, 0), (True, 0.1, False, 7), (False, 0.01, True, 3)])
+def test_muon_step(ops, nesterov, wd, with_ema, offset):
+    total = offset + sum(r * c for r, c in SHAPES) + 11
+    gen = torch.Generator().manual_seed(1)
+    p, g, m = (torch.randn(total, generator=gen).cuda() * s for s in (0.05, 1e-3, 1e-3))
+    ema = p + 0.01 if with_ema else None
+    plan = ops.MuonPlan(SHAPES, "cuda", offset=offset)
+    want = muon_oracle(p, g, m, ema, SHAPES, offset, 0.3, 0.9, nesterov, wd, 0.99, torch.float64)
+    fp32 = muon_oracle(p, g, m, ema, SHAPES, offset, 0.3, 0.9, nesterov, wd, 0.99, torch.float32)
+    before = g.clone()
+    ops.muon_step(plan, p, g, m, ema, lr=0.3, momentum=0.9, nesterov=nesterov, weight_decay=wd, ema_decay=0.99)
+    assert torch.equal(g, before)
+    for got, ref, low, what in zip((p, m, ema), want, fp32, ("p", "m", "ema")):
+        if got is None:
+            continue
+        got = got.cpu()
+        assert rel(got, ref) <= max(3 * rel(low, ref), 1e-6), what
+        assert torch.equal(got[:offset].double(), ref[:offset]) and torch.equal(got[-11:].double(), ref[-11:])      # outside the matrices
+
+
+def test_muon_step_of_many_matrices(ops):
+    """more matrices than one call of the library takes"""
+    shapes = [(4 + i % 5, 6 + i % 7) for i in range(75)]
+    total = sum(r * c for r, c in shapes)
+    p, g, m = (torch.randn(total, device="cuda") * s for s in (0.05, 1e-3, 1e-3))
+    want = muon_oracle(p, g, m, None, shapes, 0, 0.1, 0.95, True, 0.0, 0.0, torch.float64)
+    fp32 = muon_oracle(p, g, m, None, shapes, 0, 0.1, 0.95, True, 0.0, 0.0, torch.float32)
+    ops.muon_step(ops.MuonPlan(shapes, "cuda"), p, g, m, lr=0.1)
+    assert rel(p.cpu(), want[0]) <= max(3 * rel(fp32[0], want[0]), 1e-6) and rel(m.cpu(), want[1]) <= 1e-6
+
+
+def test_every_replay_of_a_captured_step(ops):
+    total = sum(r * c for r, c in SHAPES)
+    p, g, m = (torch.randn(total, device="cuda") * s for s in (0.05, 1e-3, 1e-3))
+    ema = p.clone()
+    plan, other = ops.MuonPlan(SHAPES, "cuda"), ops.MuonPlan(SHAPES, "cuda")
+    q, n, f = p.clone(), m.clone(), ema.clone()
+    batch = torch.randn(3, 40, 70, device="cuda").bfloat16()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.muon_step(plan, p, g, m, ema)
+        o = ops.orthogonalize(batch)
+    for k in range(4):
+        g.copy_(torch.randn(total, device="cuda") * 1e-3)
+        batch.copy_(torch.randn(3, 40, 70, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        ops.muon_step(other, q, g, n, f)
+        assert torch.equal(p, q) and torch.equal(m, n) and torch.equal(ema, f), k
+        assert torch.equal(o, ops.orthogonalize(batch)), k
+
+
+def test_two_calls_at_once(ops):
+    """calls on two streams have workspaces of their own"""
+    a, b = matrix(300, 400, seed=1).cuda(), matrix(120, 700, seed=2).cuda()
+    want = ops.orthogonalize(a), ops.orthogonalize(b)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for s in (s1, s2):
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(5):
+        with torch.cuda.stream(s1):
+            x = ops.orthogonalize(a)
+        with torch.cuda.stream(s2):
+            y = ops.orthogonalize(b)
+        got.append((x, y))
+    torch.cuda.synchronize()
+    for x, y in got:
+        assert torch.equal(x, want[0]) and torch.equal(y, want[1])
+
+
+def test_refusals(ops):
+    from infinite_texture_gans_amd._lib import ItgError
+    g = torch.randn(4, 8, device="cuda")
+    plan = ops.MuonPlan([(4, 8)], "cuda")
+    flat = [torch.zeros(32, device="cuda") for _ in range(3)]
+    for bad in (lambda: ops.orthogonalize(g.cpu()), lambda: ops.orthogonalize(g.double()), lambda: ops.orthogonalize(g[0]),
+                lambda: ops.orthogonalize(g, steps=0), lambda: ops.orthogonalize(g, steps=17), lambda: ops.orthogonalize(g, eps=-1.0),
+                lambda: ops.orthogonalize(g, coefficients=(1.0, 2.0)), lambda: ops.orthogonalize(g, steps=3, coefficients=[(1.5, -0.5, 0.0)] * 2),
+                lambda: ops.orthogonalize(g, coefficients=(8.0, 0.0, 0.0)), lambda: ops.orthogonalize(g, coefficients=(float("nan"), 0.0, 0.0)),
+                lambda: ops.orthogonalize(g, out=torch.empty(8, 4, device="cuda")), lambda: ops.orthogonalize(g, out=torch.empty(4, 16, device="cuda")[:, ::2]),
+                lambda: ops.orthogonalize(g.mT, out=g.mT), lambda: ops.orthogonalize(torch.empty(1, 70000, device="cuda")),
+                lambda: ops.MuonPlan([], "cuda"), lambda: ops.MuonPlan([(0, 3)], "cuda"), lambda: ops.MuonPlan([(4, 8)], "cpu"),
+                lambda: ops.MuonPlan([(4, 8)], "cuda", offset=-1), lambda: ops.muon_step(plan, flat[0][:31], flat[1], flat[2]),
+                lambda: ops.muon_step(plan, flat[0], flat[1].half(), flat[2]), lambda: ops.muon_step(plan, flat[0], flat[1].cpu(), flat[2]),
+                lambda: ops.muon_step(plan, flat[0], flat[1], flat[2], steps=0),
+                lambda: ops.muon_step(plan, flat[0], torch.zeros(64, device="cuda")[::2], flat[2])):
+        with pytest.raises(ItgError):
+            bad()
