@@ -6,8 +6,6 @@
 // Statistics, sums and products are fp32 whatever the tensors' type; the variance is taken around the mean of the row (a second
 // sweep over values that are already on the chip), never as a difference of moments.  Every sum has a fixed order: results do
 // not change from call to call.
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 #include "itg_common.h"
 
 namespace {
@@ -23,139 +21,510 @@ struct LnP {
   int act;
 };
 
-template <typename T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
-template <typename T> __device__ __forceinline__ T from_f(float v) { return (T)v; }
-template <> __device__ __forceinline__ float to_f<__hip_bfloat16>(__hip_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ __hip_bfloat16 from_f<__hip_bfloat16>(float v) { return __float2bfloat16(v); }
-
 __device__ __forceinline__ float act_slope_at(float u, int act, float slope) {
   if (act == ITG_ACT_LRELU) return u > 0.f ? 1.f : slope;
   if (act == ITG_ACT_TANH) { const float t = tanhf(u); return 1.f - t * t; }
   return 1.f;
 }
 
-// sum over the workgroup's 256 threads, the same value in every thread; `lds` holds 4 floats and may be re-used after the call
-__device__ __forceinline__ float block_sum(float v, float* lds) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+// ---- rows held in registers.  A row of c values is cut into vectors of V (16 bytes; single values where c < V); TPR threads share a
+// row and a thread holds the R vectors tid, tid + TPR, ...  The last vector of a row that V does not divide either starts at c - V
+// and masks what it shares with its neighbour (both write the same values there), or, in rows with zero padding behind the
+// channels, lies where it belongs and masks the padding.  Vector loads and stores need the element's alignment only.
+struct LnV { int nv, off_last, lo_last, hi_last; };      // vectors per row; start of the last one and its valid elements [lo, hi)
+
+__host__ __device__ inline LnV ln_vectors(int c, int pad, int V) {
+  LnV v;
+  v.nv = (c + V - 1) / V;
+  const bool padded = pad > 0 && pad < V && (c + pad) % V == 0;
+  v.off_last = padded ? (v.nv - 1) * V : c - V;
+  v.lo_last = (v.nv - 1) * V - v.off_last;
+  v.hi_last = padded ? c - v.off_last : V;
+  return v;
 }
 
-// ---- any row length: one workgroup per row, the row is swept again from the cache for every quantity
-template <typename T, typename W>
-__global__ __launch_bounds__(256) void ln_fwd_any_kernel(LnP p) {
-  __shared__ float lds[4];
-  const T* X = (const T*)p.x;
+template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[V]; };
+
+// the R vectors of a thread in row `q` (nothing is read past the row's end)
+template <typename T, int V, int R>
+__device__ __forceinline__ void ln_fetch(const T* q, const int (&off)[R], const int (&hi)[R], Pack<T, V> (&u)[R]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (hi[r] > 0) u[r] = *reinterpret_cast<const Pack<T, V>*>(q + off[r]);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void ln_store(T* q, const float (&f)[V]) {
+  Pack<T, V> u;
+#pragma unroll
+  for (int e = 0; e < V; ++e) u.v[e] = (T)f[e];
+  *reinterpret_cast<Pack<T, V>*>(q) = u;
+}
+
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+
+// sum over aligned groups of G <= 64 lanes, in every lane: cross-lane moves inside 16 lanes, two shuffles beyond
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+  if (G >= 2) v += dpp<0xB1>(v);        // lane ^ 1
+  if (G >= 4) v += dpp<0x4E>(v);        // lane ^ 2
+  if (G >= 8) v += dpp<0x141>(v);       // mirror in 8: the other four
+  if (G >= 16) v += dpp<0x140>(v);      // mirror in 16: the other eight
+  if (G >= 32) v += __shfl_xor(v, 16, 64);
+  if (G >= 64) v += __shfl_xor(v, 32, 64);
+  return v;
+}
+
+// sum over the TPR threads of a row.  TPR > 64: through LDS, `red` = this call's TPR / 64 floats, one barrier
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  v = group_sum<(TPR < 64 ? TPR : 64)>(v);
+  if (TPR <= 64) return v;
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < (TPR > 64 ? TPR / 64 : 1); ++k) s += red[k];
+  return s;
+}
+
+// ANY: an activation, or rows that V does not divide; without it neither is looked at (a quarter of the instructions per value,
+// which at 2 bytes a value is time: 16384 x 4096 bf16 forward 61.6 us with the masks, 55.5 without)
+template <typename T, typename W, int V, int TPR, int R, bool ANY>
+__global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
+  constexpr int NT = TPR > 64 ? TPR : 256, GROUPS = NT / TPR;
+  __shared__ float red[4][TPR > 64 ? TPR / 64 : 1];      // two sums per row, two rows' worth: a row's sums outlive the next row's first barrier
+  const LnV lv = ln_vectors(p.c, p.pad, V);
+  const int tid = threadIdx.x % TPR;
+  int off[R], lo[R], hi[R];
+  float w[R][V], b[R][V];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = tid + r * TPR;
+    off[r] = i < lv.nv - 1 ? i * V : lv.off_last;
+    lo[r] = i < lv.nv - 1 ? 0 : lv.lo_last;
+    hi[r] = i < lv.nv - 1 ? V : i < lv.nv ? lv.hi_last : 0;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const bool in = e < hi[r];
+      w[r][e] = in && p.w ? (float)((const W*)p.w)[off[r] + e] : 1.f;
+      b[r][e] = in && p.b ? (float)((const W*)p.b)[off[r] + e] : 0.f;
+    }
+  }
+  const float inv = 1.f / (float)p.c;
+  int flip = 0;
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / TPR;
+  Pack<T, V> u[R] = {};
+  if (row < p.rows) ln_fetch<T, V, R>((const T*)p.x + row * p.ldx, off, hi, u);
+  for (; row < p.rows; row += step, flip ^= 2) {
+    float f[R][V], s = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        f[r][e] = (float)u[r].v[e];
+        s += !ANY || (e >= lo[r] && e < hi[r]) ? f[r][e] : 0.f;      // a vector past the row's end holds zeros
+      }
+    // the next row is on its way while this one is reduced and written
+    if (row + step < p.rows) ln_fetch<T, V, R>((const T*)p.x + (row + step) * p.ldx, off, hi, u);
+    const float mean = row_sum<TPR>(s, red[flip]) * inv;
+    s = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float q = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        f[r][e] -= mean;
+        q = fmaf(f[r][e], !ANY || (e >= lo[r] && e < hi[r]) ? f[r][e] : 0.f, q);
+      }
+      s += hi[r] > 0 ? q : 0.f;
+    }
+    const float rs = 1.f / sqrtf(row_sum<TPR>(s, red[flip + 1]) * inv + p.eps);
+    T* y = (T*)p.y + row * p.ldy;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (hi[r] <= 0) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        f[r][e] = fmaf(f[r][e] * rs, w[r][e], b[r][e]);
+        if (ANY) f[r][e] = e < hi[r] ? act_apply(f[r][e], p.act, p.slope) : 0.f;
+      }
+      ln_store<T, V>(y + off[r], f[r]);
+    }
+    if (ANY && p.pad && lv.hi_last == V)
+      for (int i = tid; i < p.pad; i += TPR) y[p.c + i] = (T)0.f;
+    if (p.stat && tid == 0) { p.stat[2 * row] = mean; p.stat[2 * row + 1] = rs; }
+  }
+}
+
+// dx, and this workgroup's share of dw | db (`part`), which a thread sums over the rows it sees for the channels it holds
+template <typename T, typename W, int V, int TPR, int R, bool ANY>
+__global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
+  constexpr int NT = TPR > 64 ? TPR : 256, GROUPS = NT / TPR;
+  __shared__ float red[4][TPR > 64 ? TPR / 64 : 1];
+  const LnV lv = ln_vectors(p.c, p.pad, V);
+  const int tid = threadIdx.x % TPR;
+  int off[R], lo[R], hi[R];
+  float w[R][V], b[R][V], aw[R][V], ab[R][V];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = tid + r * TPR;
+    off[r] = i < lv.nv - 1 ? i * V : lv.off_last;
+    lo[r] = i < lv.nv - 1 ? 0 : lv.lo_last;
+    hi[r] = i < lv.nv - 1 ? V : i < lv.nv ? lv.hi_last : 0;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const bool in = e < hi[r];
+      w[r][e] = in && p.w ? (float)((const W*)p.w)[off[r] + e] : 1.f;
+      b[r][e] = ANY && in && p.b && p.act ? (float)((const W*)p.b)[off[r] + e] : 0.f;
+      aw[r][e] = ab[r][e] = 0.f;
+    }
+  }
+  const float inv = 1.f / (float)p.c;
+  int flip = 0;
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / TPR;
+  Pack<T, V> ux[R] = {}, ug[R] = {};
+  float mean = 0.f, rs = 0.f;
+  auto fetch = [&](int64_t at) {
+    ln_fetch<T, V, R>((const T*)p.x + at * p.ldx, off, hi, ux);
+    ln_fetch<T, V, R>((const T*)p.dy + at * p.lddy, off, hi, ug);
+    mean = p.stat[2 * at]; rs = p.stat[2 * at + 1];
+  };
+  if (row < p.rows) fetch(row);
+  for (; row < p.rows; row += step, flip ^= 2) {
+    float xh[R][V], g[R][V], s1 = 0.f, s2 = 0.f;
+    const float r_now = rs;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {      // a vector past the row's end holds zeros in dy
+        const bool in = !ANY || (e >= lo[r] && e < hi[r]);
+        const float h = in ? ((float)ux[r].v[e] - mean) * rs : 0.f;
+        float du = in ? (float)ug[r].v[e] : 0.f;
+        xh[r][e] = ANY ? ((float)ux[r].v[e] - mean) * rs : h;
+        float all = ANY ? (float)ug[r].v[e] : du;
+        if (ANY && p.act) {
+          const float sl = act_slope_at(fmaf(xh[r][e], w[r][e], b[r][e]), p.act, p.slope);
+          all *= sl; du *= sl;
+        }
+        aw[r][e] = fmaf(du, h, aw[r][e]);
+        ab[r][e] += du;
+        g[r][e] = all * w[r][e];
+        const float gi = ANY ? du * w[r][e] : g[r][e];
+        s1 += gi;
+        s2 = fmaf(gi, h, s2);
+      }
+    // the next row is on its way while this one is reduced and written
+    if (row + step < p.rows) fetch(row + step);
+    if (p.y) {
+      const float m1 = row_sum<TPR>(s1, red[flip]) * inv, m2 = row_sum<TPR>(s2, red[flip + 1]) * inv;
+      T* dx = (T*)p.y + row * p.ldy;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (hi[r] <= 0) continue;
+#pragma unroll
+        for (int e = 0; e < V; ++e) g[r][e] = !ANY || e < hi[r] ? r_now * (g[r][e] - m1 - xh[r][e] * m2) : 0.f;
+        ln_store<T, V>(dx + off[r], g[r]);
+      }
+      if (ANY && p.pad && lv.hi_last == V)
+        for (int i = tid; i < p.pad; i += TPR) dx[p.c + i] = (T)0.f;
+    }
+  }
+  if (!p.part) return;
+  // the row groups of this workgroup: lanes of a wave by shuffles, waves in order through LDS
+  float* part = p.part + (int64_t)blockIdx.x * 2 * p.c;
+  constexpr int WAVES = TPR <= 64 ? NT / 64 : 1;
+  __shared__ float acc[WAVES > 1 ? WAVES - 1 : 1][2][WAVES > 1 ? (TPR < 64 ? TPR : 64) * R * V : 1];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (TPR < 64) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+#pragma unroll
+        for (int o = TPR; o < 64; o <<= 1) { aw[r][e] += __shfl_xor(aw[r][e], o, 64); ab[r][e] += __shfl_xor(ab[r][e], o, 64); }
+  }
+  if (WAVES > 1) {
+    if (wave > 0 && lane < TPR) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < V; ++e) { acc[wave - 1][0][(r * V + e) * (TPR < 64 ? TPR : 64) + tid] = aw[r][e]; acc[wave - 1][1][(r * V + e) * (TPR < 64 ? TPR : 64) + tid] = ab[r][e]; }
+    }
+    __syncthreads();
+    if (wave > 0 || lane >= TPR) return;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float vw = aw[r][e], vb = ab[r][e];
+      if (WAVES > 1) {
+#pragma unroll
+        for (int k = 0; k < WAVES - 1; ++k) { vw += acc[k][0][(r * V + e) * (TPR < 64 ? TPR : 64) + tid]; vb += acc[k][1][(r * V + e) * (TPR < 64 ? TPR : 64) + tid]; }
+      }
+      if (e >= lo[r] && e < hi[r]) { part[off[r] + e] = vw; part[p.c + off[r] + e] = vb; }
+    }
+}
+
+// ---- any row length: one workgroup of 1024 threads per row, which sweeps the row again (from the cache) for every quantity
+constexpr int LN_ANY = 1024;
+
+template <int N> struct Width { static constexpr int value = N; };
+
+// f(first channel, Width) over the row's whole vectors of V values, then over the values behind them
+template <int V, typename F>
+__device__ __forceinline__ void ln_sweep(int c, F f) {
+  const int full = c / V;
+  for (int i = threadIdx.x; i < full; i += LN_ANY) f(i * V, Width<V>{});
+  for (int i = full * V + threadIdx.x; i < c; i += LN_ANY) f(i, Width<1>{});
+}
+
+template <typename T, int N> __device__ __forceinline__ Pack<T, N> ln_at(const T* q) { return *reinterpret_cast<const Pack<T, N>*>(q); }
+
+template <typename T, typename W, int V>
+__global__ __launch_bounds__(LN_ANY) void ln_fwd_any_kernel(LnP p) {
+  __shared__ float red[4][LN_ANY / 64];
   const W* w = (const W*)p.w; const W* b = (const W*)p.b;
   const float inv = 1.f / (float)p.c;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const T* x = X + row * p.ldx;
+  int flip = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, flip ^= 2) {
+    const T* x = (const T*)p.x + row * p.ldx;
     float s = 0.f;
-    for (int i = threadIdx.x; i < p.c; i += 256) s += to_f(x[i]);
-    const float mean = block_sum(s, lds) * inv;
+    ln_sweep<V>(p.c, [&](int at, auto width) {
+      constexpr int N = decltype(width)::value;
+      const auto u = ln_at<T, N>(x + at);
+#pragma unroll
+      for (int e = 0; e < N; ++e) s += (float)u.v[e];
+    });
+    const float mean = row_sum<LN_ANY>(s, red[flip]) * inv;
     s = 0.f;
-    for (int i = threadIdx.x; i < p.c; i += 256) { const float d = to_f(x[i]) - mean; s = fmaf(d, d, s); }
-    const float r = 1.f / sqrtf(block_sum(s, lds) * inv + p.eps);
+    ln_sweep<V>(p.c, [&](int at, auto width) {
+      constexpr int N = decltype(width)::value;
+      const auto u = ln_at<T, N>(x + at);
+#pragma unroll
+      for (int e = 0; e < N; ++e) { const float d = (float)u.v[e] - mean; s = fmaf(d, d, s); }
+    });
+    const float r = 1.f / sqrtf(row_sum<LN_ANY>(s, red[flip + 1]) * inv + p.eps);
     T* y = (T*)p.y + row * p.ldy;
-    for (int i = threadIdx.x; i < p.c; i += 256) {
-      const float u = fmaf((to_f(x[i]) - mean) * r, w ? to_f(w[i]) : 1.f, b ? to_f(b[i]) : 0.f);
-      y[i] = from_f<T>(act_apply(u, p.act, p.slope));
-    }
-    for (int i = threadIdx.x; i < p.pad; i += 256) y[p.c + i] = from_f<T>(0.f);
+    ln_sweep<V>(p.c, [&](int at, auto width) {
+      constexpr int N = decltype(width)::value;
+      auto u = ln_at<T, N>(x + at);
+      Pack<W, N> uw, ub;
+      if (w) uw = ln_at<W, N>(w + at);
+      if (b) ub = ln_at<W, N>(b + at);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float v = fmaf(((float)u.v[e] - mean) * r, w ? (float)uw.v[e] : 1.f, b ? (float)ub.v[e] : 0.f);
+        u.v[e] = (T)act_apply(v, p.act, p.slope);
+      }
+      *reinterpret_cast<Pack<T, N>*>(y + at) = u;
+    });
+    for (int i = threadIdx.x; i < p.pad; i += LN_ANY) y[p.c + i] = (T)0.f;
     if (p.stat && threadIdx.x == 0) { p.stat[2 * row] = mean; p.stat[2 * row + 1] = r; }
   }
 }
 
-template <typename T, typename W>
-__global__ __launch_bounds__(256) void ln_dx_any_kernel(LnP p) {
-  __shared__ float lds[4];
+template <typename T, typename W, int V>
+__global__ __launch_bounds__(LN_ANY) void ln_dx_any_kernel(LnP p) {
+  __shared__ float red[4][LN_ANY / 64];
   const W* w = (const W*)p.w; const W* b = (const W*)p.b;
   const float inv = 1.f / (float)p.c;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+  int flip = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, flip ^= 2) {
     const T* x = (const T*)p.x + row * p.ldx;
     const T* dy = (const T*)p.dy + row * p.lddy;
     const float mean = p.stat[2 * row], r = p.stat[2 * row + 1];
     float s1 = 0.f, s2 = 0.f;
-    for (int i = threadIdx.x; i < p.c; i += 256) {
-      const float xh = (to_f(x[i]) - mean) * r, wi = w ? to_f(w[i]) : 1.f;
-      const float g = to_f(dy[i]) * act_slope_at(fmaf(xh, wi, b ? to_f(b[i]) : 0.f), p.act, p.slope) * wi;
-      s1 += g; s2 = fmaf(g, xh, s2);
-    }
-    const float m1 = block_sum(s1, lds) * inv, m2 = block_sum(s2, lds) * inv;
+    ln_sweep<V>(p.c, [&](int at, auto width) {
+      constexpr int N = decltype(width)::value;
+      const auto ux = ln_at<T, N>(x + at), ug = ln_at<T, N>(dy + at);
+      Pack<W, N> uw, ub;
+      if (w) uw = ln_at<W, N>(w + at);
+      if (b && p.act) ub = ln_at<W, N>(b + at);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float xh = ((float)ux.v[e] - mean) * r, wi = w ? (float)uw.v[e] : 1.f;
+        float g = (float)ug.v[e] * wi;
+        if (p.act) g *= act_slope_at(fmaf(xh, wi, b ? (float)ub.v[e] : 0.f), p.act, p.slope);
+        s1 += g; s2 = fmaf(g, xh, s2);
+      }
+    });
+    const float m1 = row_sum<LN_ANY>(s1, red[flip]) * inv, m2 = row_sum<LN_ANY>(s2, red[flip + 1]) * inv;
     T* dx = (T*)p.y + row * p.ldy;
-    for (int i = threadIdx.x; i < p.c; i += 256) {
-      const float xh = (to_f(x[i]) - mean) * r, wi = w ? to_f(w[i]) : 1.f;
-      const float g = to_f(dy[i]) * act_slope_at(fmaf(xh, wi, b ? to_f(b[i]) : 0.f), p.act, p.slope) * wi;
-      dx[i] = from_f<T>(r * (g - m1 - xh * m2));
-    }
-    for (int i = threadIdx.x; i < p.pad; i += 256) dx[p.c + i] = from_f<T>(0.f);
+    ln_sweep<V>(p.c, [&](int at, auto width) {
+      constexpr int N = decltype(width)::value;
+      auto ux = ln_at<T, N>(x + at);
+      const auto ug = ln_at<T, N>(dy + at);
+      Pack<W, N> uw, ub;
+      if (w) uw = ln_at<W, N>(w + at);
+      if (b && p.act) ub = ln_at<W, N>(b + at);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float xh = ((float)ux.v[e] - mean) * r, wi = w ? (float)uw.v[e] : 1.f;
+        float g = (float)ug.v[e] * wi;
+        if (p.act) g *= act_slope_at(fmaf(xh, wi, b ? (float)ub.v[e] : 0.f), p.act, p.slope);
+        ux.v[e] = (T)(r * (g - m1 - xh * m2));
+      }
+      *reinterpret_cast<Pack<T, N>*>(dx + at) = ux;
+    });
+    for (int i = threadIdx.x; i < p.pad; i += LN_ANY) dx[p.c + i] = (T)0.f;
   }
 }
 
-// shares of dw | db: a thread owns one channel and a chunk of the rows
-template <typename T, typename W>
+// shares of dw | db: a thread owns N channels (the last one starts at c - N and leaves what its neighbour holds) and a chunk of the rows
+template <typename T, typename W, int N>
 __global__ __launch_bounds__(256) void ln_dw_any_kernel(LnP p, int64_t chunk) {
   const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= p.c) return;
+  if (i * N >= p.c) return;
+  const int at = i * N + N <= p.c ? i * N : p.c - N, lo = i * N - at;
   const int64_t r0 = blockIdx.y * chunk, r1 = r0 + chunk < p.rows ? r0 + chunk : p.rows;
-  const float wi = p.w ? to_f(((const W*)p.w)[i]) : 1.f, bi = p.b ? to_f(((const W*)p.b)[i]) : 0.f;
-  float dw = 0.f, db = 0.f;
+  float w[N], b[N], dw[N], db[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    w[e] = p.w ? (float)((const W*)p.w)[at + e] : 1.f;
+    b[e] = p.b ? (float)((const W*)p.b)[at + e] : 0.f;
+    dw[e] = db[e] = 0.f;
+  }
+#pragma unroll 2
   for (int64_t row = r0; row < r1; ++row) {
-    const float xh = (to_f(((const T*)p.x)[row * p.ldx + i]) - p.stat[2 * row]) * p.stat[2 * row + 1];
-    const float du = to_f(((const T*)p.dy)[row * p.lddy + i]) * act_slope_at(fmaf(xh, wi, bi), p.act, p.slope);
-    dw = fmaf(du, xh, dw); db += du;
+    const auto ux = ln_at<T, N>((const T*)p.x + row * p.ldx + at), ug = ln_at<T, N>((const T*)p.dy + row * p.lddy + at);
+    const float mean = p.stat[2 * row], r = p.stat[2 * row + 1];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float xh = ((float)ux.v[e] - mean) * r;
+      float du = (float)ug.v[e];
+      if (p.act) du *= act_slope_at(fmaf(xh, w[e], b[e]), p.act, p.slope);
+      dw[e] = fmaf(du, xh, dw[e]); db[e] += du;
+    }
   }
   float* part = p.part + (int64_t)blockIdx.y * 2 * p.c;
-  part[i] = dw; part[p.c + i] = db;
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (e >= lo) { part[at + e] = dw[e]; part[p.c + at + e] = db[e]; }
 }
 
-// dw | db = the shares added in chunk order: 64 channels x 16 share lanes per workgroup
+// dw | db = the shares added in a fixed order: 16 channels x 64 share lanes per workgroup
 template <typename W>
 __global__ __launch_bounds__(1024) void ln_dw_reduce_kernel(const float* __restrict__ part, int chunks, int c, W* dw, W* db, int acc) {
-  __shared__ float lds[16][64];
-  const int col = blockIdx.x * 64 + (threadIdx.x & 63), lane = threadIdx.x >> 6;
+  __shared__ float lds[64][17];
+  const int k = threadIdx.x & 15, col = blockIdx.x * 16 + k, lane = threadIdx.x >> 4;
   float s = 0.f;
-  if (col < 2 * c)
-    for (int k = lane; k < chunks; k += 16) s += part[(int64_t)k * 2 * c + col];
-  lds[lane][threadIdx.x & 63] = s;
+  if (col < 2 * c) {
+#pragma unroll 4
+    for (int q = lane; q < chunks; q += 64) s += part[(int64_t)q * 2 * c + col];
+  }
+  lds[lane][k] = s;
   __syncthreads();
-  if (lane == 0 && col < 2 * c) {
-    float v = 0.f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) v += lds[k][threadIdx.x];
-    W* out = col < c ? dw : db;
-    const int i = col < c ? col : col - c;
-    if (out) out[i] = from_f<W>(acc ? to_f(out[i]) + v : v);
+  if (lane < 16) {                                 // 16 lanes x 4 shares, then the 16 sums of a channel (lanes of one row of 16)
+    const int ch = lane;                           // transposed: thread (lane, k) takes channel `lane`, shares k, k + 16, ...
+    float v = (lds[k][ch] + lds[k + 16][ch]) + (lds[k + 32][ch] + lds[k + 48][ch]);
+    v = group_sum<16>(v);
+    const int out_col = blockIdx.x * 16 + ch;
+    if (k == 0 && out_col < 2 * c) {
+      W* out = out_col < c ? dw : db;
+      const int i = out_col < c ? out_col : out_col - c;
+      if (out) out[i] = (W)(acc ? (float)out[i] + v : v);
+    }
   }
 }
 
-constexpr int LN_CHUNKS = 256;      // at most this many shares of dw | db
+constexpr int LN_CHUNKS = 1024;      // at most this many shares of dw | db
 inline int ln_chunks(int64_t rows) { return (int)(rows < LN_CHUNKS ? rows : LN_CHUNKS); }
 inline unsigned ln_grid(int64_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); }
 
+// ANY of the kernels: an activation, a row that V does not divide (padding included)
+template <int V> inline bool ln_any(const LnP& p) { return p.act != ITG_ACT_NONE || p.c % V != 0 || p.pad != 0; }
+
+template <typename T, typename W, int V, int TPR, int R>
+int ln_fwd_run(const LnP& p, hipStream_t s) {
+  constexpr int NT = TPR > 64 ? TPR : 256, GROUPS = NT / TPR;
+  const int64_t need = (p.rows + GROUPS - 1) / GROUPS, most = 256 * (2048 / NT);
+  const dim3 grid((unsigned)(need < most ? need : most));
+  if (ln_any<V>(p)) hipLaunchKernelGGL((ln_fwd_kernel<T, W, V, TPR, R, true>), grid, dim3(NT), 0, s, p);
+  else hipLaunchKernelGGL((ln_fwd_kernel<T, W, V, TPR, R, false>), grid, dim3(NT), 0, s, p);
+  ITG_CHECK_LAUNCH();
+  return ITG_OK;
+}
+
+// Threads per row and vectors per thread: as few threads as hold the row at one vector each up to a wave; beyond, workgroups of
+// 128 .. 1024 threads at one vector of 8 or two of 4 (the backward pass keeps six values per channel it holds: at 16 channels a
+// thread it spills).
 template <typename T, typename W>
 int ln_fwd_t(const LnP& p, hipStream_t s) {
-  hipLaunchKernelGGL((ln_fwd_any_kernel<T, W>), dim3(ln_grid(p.rows)), dim3(256), 0, s, p);
+  constexpr int V = 16 / sizeof(T);
+  const int padded = p.pad > 0 && p.pad < V && (p.c + p.pad) % V == 0;
+  if (p.c < V && !padded) return p.c <= 4 ? ln_fwd_run<T, W, 1, 4, 1>(p, s) : ln_fwd_run<T, W, 1, 8, 1>(p, s);
+  const int nv = (p.c + V - 1) / V;
+  if (nv <= 4) return ln_fwd_run<T, W, V, 4, 1>(p, s);
+  if (nv <= 8) return ln_fwd_run<T, W, V, 8, 1>(p, s);
+  if (nv <= 16) return ln_fwd_run<T, W, V, 16, 1>(p, s);
+  if (nv <= 32) return ln_fwd_run<T, W, V, 32, 1>(p, s);
+  if (nv <= 64) return ln_fwd_run<T, W, V, 64, 1>(p, s);
+  if (nv <= 128) return ln_fwd_run<T, W, V, 64, 2>(p, s);
+  if (nv <= 256) return ln_fwd_run<T, W, V, 128, 2>(p, s);
+  if (nv <= 512) return ln_fwd_run<T, W, V, 256, 2>(p, s);
+  if (nv <= 1024) return ln_fwd_run<T, W, V, 512, 2>(p, s);
+  if (nv <= 2048) return ln_fwd_run<T, W, V, 1024, 2>(p, s);
+  hipLaunchKernelGGL((ln_fwd_any_kernel<T, W, V>), dim3(ln_grid(p.rows)), dim3(LN_ANY), 0, s, p);
+  ITG_CHECK_LAUNCH();
+  return ITG_OK;
+}
+
+// workgroups of the backward pass over rows in registers: each leaves one share of dw | db
+template <typename T, typename W, int V, int TPR, int R>
+int ln_bwd_run(const LnP& p, int& chunks, hipStream_t s) {
+  constexpr int NT = TPR > 64 ? TPR : 256, GROUPS = NT / TPR;
+  const int64_t need = (p.rows + GROUPS - 1) / GROUPS, few = need / 4 > 256 ? need / 4 : 256;
+  // every CU has a workgroup before one gets fewer than four turns: a share costs a write and a read of 2 c floats
+  const int64_t most = 256 * (1024 / NT) < LN_CHUNKS ? (256 * (1024 / NT) < few ? 256 * (1024 / NT) : few) : (LN_CHUNKS < few ? LN_CHUNKS : few);
+  chunks = (int)(need < most ? need : most);
+  if (ln_any<V>(p)) hipLaunchKernelGGL((ln_bwd_kernel<T, W, V, TPR, R, true>), dim3(chunks), dim3(NT), 0, s, p);
+  else hipLaunchKernelGGL((ln_bwd_kernel<T, W, V, TPR, R, false>), dim3(chunks), dim3(NT), 0, s, p);
   ITG_CHECK_LAUNCH();
   return ITG_OK;
 }
 
 template <typename T, typename W>
-int ln_bwd_t(const LnP& p, void* dw, void* db, int acc, hipStream_t s) {
-  if (p.y) {
-    hipLaunchKernelGGL((ln_dx_any_kernel<T, W>), dim3(ln_grid(p.rows)), dim3(256), 0, s, p);
-    ITG_CHECK_LAUNCH();
+int ln_bwd_t(LnP p, void* dw, void* db, int acc, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T), K = V == 8 ? 1 : 2;      // K: vectors per thread of the workgroup sizes
+  const int nv = (p.c + V - 1) / V, padded = p.pad > 0 && p.pad < V && (p.c + p.pad) % V == 0;
+  const bool shares = dw || db;
+  int chunks = 0, rc = ITG_OK;
+  if (!shares) p.part = nullptr;
+  if (p.c < V && !padded) rc = p.c <= 4 ? ln_bwd_run<T, W, 1, 4, 1>(p, chunks, s) : ln_bwd_run<T, W, 1, 8, 1>(p, chunks, s);
+  else if (nv <= 4) rc = ln_bwd_run<T, W, V, 4, 1>(p, chunks, s);
+  else if (nv <= 8) rc = ln_bwd_run<T, W, V, 8, 1>(p, chunks, s);
+  else if (nv <= 16) rc = ln_bwd_run<T, W, V, 16, 1>(p, chunks, s);
+  else if (nv <= 32) rc = ln_bwd_run<T, W, V, 32, 1>(p, chunks, s);
+  else if (nv <= 64) rc = ln_bwd_run<T, W, V, 64, 1>(p, chunks, s);
+  else if (nv <= 64 * K) rc = ln_bwd_run<T, W, V, 64, K>(p, chunks, s);
+  else if (nv <= 128 * K) rc = ln_bwd_run<T, W, V, 128, K>(p, chunks, s);
+  else if (nv <= 256 * K) rc = ln_bwd_run<T, W, V, 256, K>(p, chunks, s);
+  else if (nv <= 512 * K) rc = ln_bwd_run<T, W, V, 512, K>(p, chunks, s);
+  else if (nv <= 1024 * K) rc = ln_bwd_run<T, W, V, 1024, K>(p, chunks, s);
+  else {
+    if (p.y) {
+      hipLaunchKernelGGL((ln_dx_any_kernel<T, W, V>), dim3(ln_grid(p.rows)), dim3(LN_ANY), 0, s, p);
+      ITG_CHECK_LAUNCH();
+    }
+    if (shares) {
+      // about 2048 workgroups in all, and no share of fewer than 8 rows
+      const int cols = (nv + 255) / 256;
+      const int64_t want = 2048 / cols + 1, most = (p.rows + 7) / 8, k = want < most ? want : most;
+      const int64_t chunk = (p.rows + k - 1) / k;
+      chunks = (int)((p.rows + chunk - 1) / chunk);
+      hipLaunchKernelGGL((ln_dw_any_kernel<T, W, V>), dim3(cols, chunks), dim3(256), 0, s, p, chunk);
+      ITG_CHECK_LAUNCH();
+    }
   }
-  if (dw || db) {
-    const int64_t chunk = (p.rows + ln_chunks(p.rows) - 1) / ln_chunks(p.rows);
-    const int chunks = (int)((p.rows + chunk - 1) / chunk);
-    hipLaunchKernelGGL((ln_dw_any_kernel<T, W>), dim3((p.c + 255) / 256, chunks), dim3(256), 0, s, p, chunk);
-    ITG_CHECK_LAUNCH();
-    hipLaunchKernelGGL((ln_dw_reduce_kernel<W>), dim3((2 * p.c + 63) / 64), dim3(1024), 0, s, p.part, chunks, p.c, (W*)dw, (W*)db, acc);
-    ITG_CHECK_LAUNCH();
-  }
+  if (rc || !shares) return rc;
+  hipLaunchKernelGGL((ln_dw_reduce_kernel<W>), dim3((2 * p.c + 15) / 16), dim3(1024), 0, s, p.part, chunks, p.c, (W*)dw, (W*)db, acc);
+  ITG_CHECK_LAUNCH();
   return ITG_OK;
 }
 
@@ -175,9 +544,9 @@ inline bool misaligned(const void* q, int dtype) { return ((uintptr_t)q & (dtype
 #define LN_TYPES(CALL)                                                          \
   if (dtype == ITG_F32) { typedef float T; typedef float W; return CALL; }      \
   if (dtype == ITG_BF16) {                                                      \
-    typedef __hip_bfloat16 T;                                                   \
+    typedef __bf16 T;                                                   \
     if (param_dtype == ITG_F32) { typedef float W; return CALL; }               \
-    typedef __hip_bfloat16 W; return CALL;                                      \
+    typedef __bf16 W; return CALL;                                      \
   }                                                                             \
   typedef _Float16 T;                                                           \
   if (param_dtype == ITG_F32) { typedef float W; return CALL; }                 \
@@ -188,7 +557,7 @@ extern "C" {
 int itg_layer_norm_fwd(const void* x, int64_t ldx, const void* gamma, const void* beta, void* y, int64_t ldy, float* mean_rstd,
                        int64_t rows, int c, int pad, int dtype, int param_dtype, float eps, int act, float slope, void* stream) {
   int rc;
-  if ((rc = ln_check(rows, c, 0, ldx, dtype, param_dtype, act)) || (rc = ln_check(rows, c, pad, ldy, dtype, param_dtype, act))) return rc;
+  if ((rc = ln_check(rows, c, pad, ldx, dtype, param_dtype, act)) || (rc = ln_check(rows, c, pad, ldy, dtype, param_dtype, act))) return rc;
   if (!x || !y || !(eps >= 0.f)) return ITG_ERR_ARG;
   if (misaligned(x, dtype) || misaligned(y, dtype) || misaligned(gamma, param_dtype) || misaligned(beta, param_dtype) ||
       misaligned(mean_rstd, ITG_F32)) return ITG_ERR_ALIGN;
@@ -209,7 +578,7 @@ int itg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy,
                        int pad, int dtype, int param_dtype, int act, float slope, float* workspace, int64_t workspace_floats,
                        void* stream) {
   int rc;
-  if ((rc = ln_check(rows, c, 0, ldx, dtype, param_dtype, act)) || (rc = ln_check(rows, c, 0, lddy, dtype, param_dtype, act)) ||
+  if ((rc = ln_check(rows, c, pad, ldx, dtype, param_dtype, act)) || (rc = ln_check(rows, c, pad, lddy, dtype, param_dtype, act)) ||
       (dx && (rc = ln_check(rows, c, pad, lddx, dtype, param_dtype, act)))) return rc;
   if (!x || !dy || !mean_rstd) return ITG_ERR_ARG;
   if (misaligned(x, dtype) || misaligned(dy, dtype) || misaligned(dx, dtype) || misaligned(gamma, param_dtype) ||
