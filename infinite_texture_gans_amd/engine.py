@@ -18,14 +18,19 @@ import torch.nn as nn
 
 from . import ops
 from .dist import SyncGroup, average_flat_gradient
-from .models.layers import _BNParams
+from .models.layers import _BNParams, _LNParams
 
 
 class FlatParams:
-    """Re-homes a module's parameters (and .grad) into flat buffers."""
+    """Re-homes a module's parameters (and .grad) into flat buffers.  ``matrices_last``: parameters of two and more dimensions
+    (the filters) behind all others, as :class:`FlatMuon` wants them; otherwise in module order."""
 
-    def __init__(self, module):
+    def __init__(self, module, matrices_last=False):
         self.params = [p for p in module.parameters()]
+        if matrices_last:
+            self.params.sort(key=lambda p: p.dim() >= 2)      # stable: module order within both kinds
+        self.vectors = sum(p.numel() for p in self.params if p.dim() < 2)
+        self.shapes = [(p.shape[0], p.numel() // p.shape[0]) for p in self.params if p.dim() >= 2]
         dev = self.params[0].device
         n = sum(p.numel() for p in self.params)
         self.data = torch.empty(n, device=dev, dtype=torch.float32)
@@ -71,6 +76,35 @@ class FlatAdam:
         self.t_dev.add_(1)
         ops.adam_ema_step(self.flat.data, self.flat.grad, self.m, self.v, self.ema, self.lr, self.betas[0],
                           self.betas[1], self.eps, self.t, self.ema_decay, step_dev=self.t_dev)
+
+
+class FlatMuon:
+    """Muon over a FlatParams(matrices_last=True): the filters as (output channels, everything else) matrices through
+    ops.muon_step, the vectors in front of them through Adam (as :class:`FlatAdam`), both with the EMA copy in the same launches.
+    ``lr`` is Adam's; the matrices take ``muon_lr`` in proportion to it, so that a decay of ``lr`` decays both."""
+
+    def __init__(self, flat, lr=2e-4, betas=(0.0, 0.999), eps=1e-8, ema=None, ema_decay=0.999, muon_lr=0.01, momentum=0.95,
+                 weight_decay=0.0):
+        self.flat, self.lr, self.betas, self.eps = flat, lr, (float(betas[0]), float(betas[1])), eps
+        self.muon_lr, self.lr0, self.momentum, self.weight_decay = float(muon_lr), float(lr), float(momentum), float(weight_decay)
+        self.m = torch.zeros_like(flat.data)               # Adam's first moment | momentum of the matrices
+        self.v = torch.zeros(flat.vectors, device=flat.data.device, dtype=torch.float32)
+        self.ema, self.ema_decay = ema, ema_decay
+        self.plan = ops.MuonPlan(flat.shapes, flat.data.device, offset=flat.vectors) if flat.shapes else None
+        self.t = 0
+        self.t_dev = torch.zeros((), device=flat.data.device, dtype=torch.int32)
+
+    def step(self):
+        self.t += 1
+        self.t_dev.add_(1)
+        f, n = self.flat, self.flat.vectors
+        if n:
+            ops.adam_ema_step(f.data[:n], f.grad[:n], self.m[:n], self.v, self.ema[:n] if self.ema is not None else None, self.lr,
+                              self.betas[0], self.betas[1], self.eps, self.t, self.ema_decay, step_dev=self.t_dev)
+        if self.plan is not None:
+            lr = self.muon_lr * (self.lr / self.lr0 if self.lr0 else 1.0)
+            ops.muon_step(self.plan, f.data, f.grad, self.m, self.ema, lr=lr, momentum=self.momentum,
+                          weight_decay=self.weight_decay, ema_decay=self.ema_decay)
 
 
 class GradExchange:
@@ -224,22 +258,30 @@ class Trainer:
                 for m in netD.modules():
                     if isinstance(m, _BNParams):
                         m.sync = sync
-        self.flatG, self.flatD = FlatParams(netG), FlatParams(netD)
+        optimizer = getattr(args, "optimizer", "adam")
+        if optimizer not in ("adam", "muon"):
+            raise ValueError("--optimizer must be adam or muon, got %r" % (optimizer,))
+        muon = optimizer == "muon"
+        self.flatG, self.flatD = FlatParams(netG, muon), FlatParams(netD, muon)
         from .models.layers import _ConvParams
         for net in (netG, netD):        # backward kernels accumulate straight into the flat .grad buffers
             for m in net.modules():
-                if isinstance(m, (_ConvParams, _BNParams)):
+                if isinstance(m, (_ConvParams, _BNParams, _LNParams)):
                     m.grad_sinks = True
         self.netG_ema, self.flatE = netG_ema, None
         if netG_ema is not None:
-            self.flatE = FlatParams(netG_ema)
+            self.flatE = FlatParams(netG_ema, muon)
             self.flatE.data.copy_(self.flatG.data)
             for (_, b), (_, e) in zip(netG.named_buffers(), netG_ema.named_buffers()):
                 e.copy_(b)
         b1, b2 = float(args.beta1), float(args.beta2)
-        self.optD = FlatAdam(self.flatD, args.lr_D, (b1, b2))
-        self.optG = FlatAdam(self.flatG, args.lr_G, (b1, b2), ema=self.flatE.data if self.flatE else None,
-                             ema_decay=args.ema_decay)
+        kind, more = FlatAdam, {}
+        if muon:
+            kind, more = FlatMuon, dict(muon_lr=getattr(args, "muon_lr", 0.01), momentum=getattr(args, "muon_momentum", 0.95),
+                                        weight_decay=getattr(args, "muon_wd", 0.0))
+        self.optD = kind(self.flatD, args.lr_D, (b1, b2), **more)
+        self.optG = kind(self.flatG, args.lr_G, (b1, b2), ema=self.flatE.data if self.flatE else None,
+                         ema_decay=args.ema_decay, **more)
         self.label_t = 0.9 if args.smooth else 1.0
         self._one = torch.ones((), device=device)               # the seed of every backward pass (no ones_like fill per pass)
         self.hinge = getattr(args, "loss", "standard") == "hinge"
@@ -281,7 +323,8 @@ class Trainer:
         if dist_group is not None and self.world > 1 and torch.device(device).type == "cuda":
             import torch.distributed as _dist
             multi_rccl = _dist.get_backend(dist_group) == "nccl"      # the backend of the group that was passed, not the environment
-        buckets = os.environ.get("ITG_BUCKETS", "0" if multi_rccl else "1") == "1"
+        # (muon: the flat buffers are not in module order, so their tail is not final first - one bucket)
+        buckets = os.environ.get("ITG_BUCKETS", "0" if multi_rccl else "1") == "1" and not muon
         self._check_switches_agree(buckets)
         if self.sync is not None and _active(self.sync) and buckets:
             # the early buckets travel on the D(real) branch stream: idle during both backward passes that are exchanged
@@ -290,7 +333,7 @@ class Trainer:
             self._exchange = {
                 id(self.flatD): GradExchange(self.flatD, netD, self.sync, device, issue_stream=issue, two_buckets=early),
                 id(self.flatG): GradExchange(self.flatG, netG, self.sync, device, issue_stream=issue,
-                                             two_buckets=early and getattr(netG, "type_norm", "BN") == "BN"),
+                                             two_buckets=early and getattr(netG, "type_norm", "BN") in ("BN", "LN")),
             }
 
         self._warm_collectives()

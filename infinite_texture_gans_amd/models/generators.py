@@ -4,7 +4,7 @@ import torch.nn as nn
 
 from .. import ops
 from ..ops import GT
-from .layers import LocalPadder, Attention, conv2d_lp, ResBlockGenerator, _BNParams, up2_fold_enabled
+from .layers import LocalPadder, Attention, conv2d_lp, ResBlockGenerator, _BNParams, _LNParams, up2_fold_enabled
 
 
 class ResidualPatchGenerator(nn.Module):
@@ -44,10 +44,12 @@ class ResidualPatchGenerator(nn.Module):
         # blocks 2.. sit behind the x2 upsample (forward_grid): their first conv folds it into its filter, and a step engine
         # keeps the folded panels for it (layers._ConvParams.up2); SSM modulates at the upsampled resolution: no fold there
         for i in range(2, n_layers_G + 1):
-            getattr(self, "block%d" % i).conv1.conv.up2 = type_norm == 'BN' and up2_fold_enabled()
+            getattr(self, "block%d" % i).conv1.conv.up2 = type_norm in ('BN', 'LN') and up2_fold_enabled()
         final_chin = widths[n_layers_G]
         if type_norm == 'BN':
             self.bn = _BNParams(final_chin)
+        elif type_norm == 'LN':
+            self.bn = _LNParams(final_chin)
         self.attention = Attention(c * 2, SN=SN) if attention else attention
         self.final = conv2d_lp(final_chin, img_ch, SN, padding_mode)
         for m in self.modules():
@@ -64,7 +66,7 @@ class ResidualPatchGenerator(nn.Module):
             names.append("block%d" % i)
             if i == 3 and self.attention:
                 names.append("attention")
-        if self.type_norm == 'BN':
+        if self.type_norm in ('BN', 'LN'):
             names.append("bn")
         return names + ["final"]
 
@@ -109,7 +111,7 @@ class ResidualPatchGenerator(nn.Module):
                     h = GT(o.t.permute(0, 1, 3, 2, 4, 5).reshape(n, 1, 1, H, W, ld), o.c)
                 else:
                     h = self.attention.run(h)
-        if self.type_norm == 'BN':
+        if self.type_norm in ('BN', 'LN'):
             return self.final.forward_grid(h, image_location, act=ops.ACT_TANH, bn=self.bn, bn_act=(A, s))
         h = ops.act(h, A, s)
         return self.final.forward_grid(h, image_location, act=ops.ACT_TANH)

@@ -512,6 +512,38 @@ class _INParams(nn.Module):
         return ops.to_nchw(self.run(ops.to_grid(x, 1, 1, True)), True)
 
 
+class _LNParams(nn.Module):
+    """Layer norm over the channels of every pixel (`--type_norm_G LN`; not in the reference, which has BN and SSM): gain and
+    shift as :class:`_BNParams` holds them, no buffers - one pixel's result depends on that pixel alone, so training, evaluation,
+    streamed tiles and row-sharded bands compute the same function and no statistics are exchanged."""
+    grad_sinks = False
+
+    def __init__(self, num_features, eps=1e-5):
+        super().__init__()
+        self.num_features, self.eps = num_features, eps
+        self.weight = nn.Parameter(torch.ones(num_features))
+        self.bias = nn.Parameter(torch.zeros(num_features))
+
+    def extra_repr(self):
+        return "%d, eps=%g" % (self.num_features, self.eps)
+
+    def _sinks(self):
+        if self.grad_sinks and self.weight.requires_grad and self.bias.requires_grad and self.weight.grad is not None:
+            return (self.weight.grad, self.bias.grad)
+        return None
+
+    def run(self, x, act=ops.ACT_NONE, slope=0.0, upsample=False, consumer_upsamples=False, fork=False, pad_rows=False):
+        """:meth:`_BNParams.run`'s signature: the norm is per pixel and commutes with the nearest x2 upsample behind it (which
+        ``consumer_upsamples`` leaves to the conv); ``fork`` / ``pad_rows`` are offers that the result does not take up."""
+        y = ops.layer_norm(x, self.weight, self.bias, eps=self.eps, act=act, slope=slope, sinks=self._sinks())
+        return ops.upsample2x(y) if upsample else y
+
+    def forward(self, x):
+        if isinstance(x, GT):
+            return self.run(x)
+        return ops.to_nchw(self.run(ops.to_grid(x, 1, 1, True)), True)
+
+
 class StochasticSpatialModulation(nn.Module):
     """(1+gamma)*BN(x)+beta with [gamma,beta] = embed(ReLU(mlp_shared(map))).
     reference models/layers.py:203-234."""
@@ -632,13 +664,16 @@ class ResBlockGenerator(nn.Module):
         if self.type_norm == "BN":
             self.bn1 = _BNParams(in_channels)
             self.bn2 = _BNParams(hidden_channels)
+        elif self.type_norm == "LN":
+            self.bn1 = _LNParams(in_channels)
+            self.bn2 = _LNParams(hidden_channels)
         elif self.type_norm == "SSM":
             self.bn1 = StochasticSpatialModulation(in_channels, self.map_dim, self.SN, padding_mode)
             self.bn2 = StochasticSpatialModulation(hidden_channels, self.map_dim, self.SN, padding_mode)
             if self.learnable_sc:
                 self.bn3 = StochasticSpatialModulation(in_channels, self.map_dim, self.SN, padding_mode)
         else:
-            raise ValueError("type_norm must be 'BN' or 'SSM', got %r" % (self.type_norm,))
+            raise ValueError("type_norm must be 'BN', 'LN' or 'SSM', got %r" % (self.type_norm,))
         # nn.LeakyReLU(leak) if leak > 0 else nn.ReLU(): both are ACT_LRELU with slope = leak
         self.activation = nn.LeakyReLU(self.leak) if self.leak > 0 else nn.ReLU()
 

@@ -41,7 +41,7 @@ _FLAGS = [
     ("norm_layer_D", str, None, "normalisation layer in the discriminator (None | batch | instance)"),
     ("base_res", int, 4, "base resolution of G"),
     ("padding_mode", str, "zeros", "padding used in G: zeros or local"),
-    ("type_norm_G", str, "BN", "normalisation used in G: BN or SSM"),
+    ("type_norm_G", str, "BN", "normalisation used in G: BN, SSM, or LN (build-side extra: layer norm over the channels of a pixel)"),
     ("lr_G", float, 2e-4, "generator learning rate"),
     ("lr_D", float, 2e-4, "discriminator learning rate"),
     ("beta1", float, 0, "Adam beta1"),
@@ -68,6 +68,11 @@ _FLAGS = [
     ("fname", str, "models_cp", "folder for checkpoints"),
     ("bf16", "flag", False, "build-side extra: run the convolutions on bf16-operand MFMA (fp32 tensors and "
                             "accumulation; BASELINE config 3)"),
+    ("optimizer", str, "adam", "build-side extra: adam | muon.  muon = orthogonalised momentum updates for the filter matrices of G and D, "
+                               "Adam for biases, gains and shifts"),
+    ("muon_lr", float, 0.01, "learning rate of the filter matrices under --optimizer muon (decays with --decay_lr as lr_G / lr_D do)"),
+    ("muon_momentum", float, 0.95, "momentum of the filter matrices under --optimizer muon"),
+    ("muon_wd", float, 0.0, "decoupled weight decay of the filter matrices under --optimizer muon"),
     ("sync_bn", "flag", False, "build-side extra: all-reduce the BatchNorm statistics over the data-parallel ranks "
                                "(default: per-rank statistics, as the reference's nn.DataParallel)"),
     ("launch_mode", str, "auto", "build-side extra: eager | graph | auto.  graph = the whole iteration is recorded once into a "

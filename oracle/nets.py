@@ -149,9 +149,18 @@ def _ssm(sd, name, x, m, ctx):
 def _norm(sd, name, x, m, ctx):
     if ctx.cfg.type_norm == "SSM":
         return _ssm(sd, name, x, m, ctx)
+    if ctx.cfg.type_norm == "LN":
+        return _ln(sd, name, x)
     y = _bn(sd, name, x, ctx.training)
     _bump(sd, name, ctx.training)
     return y
+
+
+def _ln(sd, name, x):
+    """Layer norm over the channels of a pixel (not in the reference): biased variance, eps 1e-5, gain and shift per channel."""
+    d = x - x.mean(1, keepdim=True)
+    y = d / torch.sqrt((d * d).mean(1, keepdim=True) + 1e-5)
+    return y * sd[name + ".weight"][:, None, None] + sd[name + ".bias"][:, None, None]
 
 
 def _block(sd, name, x, m, ctx):
@@ -204,6 +213,8 @@ def g_forward(sd, cfg, z, maps=None, training=True, loc="1st_row_1st_col", padde
     if cfg.type_norm == "BN":
         h = _bn(sd, "bn", h, training)
         _bump(sd, "bn", training)
+    elif cfg.type_norm == "LN":
+        h = _ln(sd, "bn", h)
     h = _act(h, cfg.leak)
     h = _conv_lp(sd, "final", h, ctx)
     return torch.tanh(h)

@@ -87,6 +87,41 @@ class Adam:
             p.addcdiv_(m, denom, value=-self.lr / bc1)
 
 
+class Muon:
+    """Muon for the matrices among ``params`` (two and more dimensions, as rows x everything else), Adam for the others
+    (not in the reference): m = mu m + g, u = g + mu m, five Newton-Schulz steps on u / |u|,
+    p = (1 - lr wd) p - lr sqrt(max(1, rows / columns)) NS(u)."""
+
+    def __init__(self, params, lr=2e-4, betas=(0.0, 0.999), muon_lr=0.01, momentum=0.95, weight_decay=0.0):
+        params = list(params)
+        self.adam = Adam([p for p in params if p.dim() < 2], lr, betas)
+        self.params = [p for p in params if p.dim() >= 2]
+        self.lr, self.mu, self.wd = muon_lr, momentum, weight_decay
+        self.m = [torch.zeros_like(p) for p in self.params]
+
+    @staticmethod
+    def newton_schulz(g, steps=5, abc=(3.4445, -4.7750, 2.0315)):
+        norm = g.double().norm().to(g.dtype)
+        x = g / norm if norm > 0 else g      # no gradient, no direction
+        tall = x.shape[0] > x.shape[1]
+        x = x.T if tall else x
+        for _ in range(steps):
+            s = x @ x.T
+            x = abc[0] * x + (abc[1] * s + abc[2] * (s @ s)) @ x
+        return x.T if tall else x
+
+    @torch.no_grad()
+    def step(self):
+        self.adam.step()
+        for p, m in zip(self.params, self.m):
+            if p.grad is None:
+                continue
+            m.mul_(self.mu).add_(p.grad)
+            u = (p.grad + self.mu * m).reshape(p.shape[0], -1)
+            o = self.newton_schulz(u) * math.sqrt(max(1.0, u.shape[0] / u.shape[1]))
+            p.mul_(1 - self.lr * self.wd).sub_(self.lr * o.reshape(p.shape))
+
+
 def trainable(sd):
     """Names of the nn.Parameters inside a reference state_dict (buffers excluded)."""
     skip = ("running_mean", "running_var", "num_batches_tracked", "weight_u", "weight_v")
