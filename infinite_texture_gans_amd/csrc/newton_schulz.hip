@@ -16,8 +16,6 @@
 //
 // All matrices of a call share one sequence of launches (norm, conversion, three per step): a launch covers the tiles of every
 // matrix.  Planes are padded with zeros to whole tiles; zeros stay zeros under the iteration, so no product needs a mask.
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 #include <math.h>
 #include "itg_common.h"
 
@@ -27,12 +25,17 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float SX = 4096.f, SA = 4096.f, SB = 1024.f;
-constexpr int NORM_ELEMS = 16384, NORM_BLOCKS = 512;      // elements per partial sum of squares, partial sums per matrix
+constexpr int NORM_ELEMS = 16384, NORM_BLOCKS = 512;      // values per partial sum of squares (at least), partial sums per matrix (at most)
+constexpr int KSHARE = 256, KLONG = 1024;                 // a tile's K is split into shares of KSHARE or more, from KLONG on
+
+// the three products of a step, the last of which writes the result after the last step
+enum { PH_A = 0, PH_B = 1, PH_X = 2, PH_LAST = 3 };
 
 struct NsMat {                 // one job: `count` matrices of the same shape
   int m, n, mp, np;            // short and long side, and their padded extents
   int count, tall, nblk;       // tall: the matrix has more rows than columns (X is its transpose)
-  int norm0, conv0, sym0, x0;  // first workgroup of this job in the launches
+  int norm0, conv0;            // first workgroup of this job in the launches
+  int tile0[3], share0[3], shares[3], cut[3];      // per product (A, B, X): first tile, first share, shares of a split tile, split tiles
   float scale;                 // muon: sqrt(max(1, rows / cols))
   int64_t in, ldi, sti, out, ldo, sto;      // element offsets, row strides, matrix strides
   int64_t ws, wst;             // bytes: first matrix's workspace, stride between matrices
@@ -41,22 +44,23 @@ struct NsMat {                 // one job: `count` matrices of the same shape
 struct NsArgs {
   NsMat j[ITG_NS_MAX_JOBS];
   int n, nesterov;
-  char* ws;
+  int direct[3];               // per product: tiles that one workgroup does whole; those behind them are split along K
+  char* ws; float* slab;       // slab: the split tiles' shares
   const void* g; void* out; float* mom; float* ema;
   float eps, mu, lr, wd, ema_decay;
 };
 
-// a matrix's workspace: double norm2[NORM_BLOCKS] | X, X^T planes (two generations) | A | B planes | their diagonals
+// a matrix's workspace: double norm2[NORM_BLOCKS] | X planes (two generations) | A | B planes | their diagonals
 struct NsWs {
   double* part;
-  _Float16 *xr[2][2], *xt[2][2];      // [generation][hi, lo]: [mp][np] and [np][mp]
+  _Float16* x[2][2];                  // [generation][hi, lo]: [mp][np]
   _Float16 *a[2], *b[2];              // [hi, lo]: [mp][mp]
   float *da, *db;                     // diagonals of A and B (single)
 };
 
 __host__ __device__ inline int64_t ns_ws_bytes(int mp, int np, bool split) {
   const int64_t x = (int64_t)mp * np * 2, a = (int64_t)mp * mp * 2;
-  return (int64_t)NORM_BLOCKS * 8 + 2 * x * (split ? 4 : 3) + a * (split ? 4 : 2) + (int64_t)mp * 8;
+  return (int64_t)NORM_BLOCKS * 8 + 4 * x + a * (split ? 4 : 2) + (int64_t)mp * 8;
 }
 
 __device__ inline NsWs ns_ws(char* base, int mp, int np, bool split) {
@@ -65,10 +69,8 @@ __device__ inline NsWs ns_ws(char* base, int mp, int np, bool split) {
   w.part = (double*)base;
   _Float16* q = (_Float16*)(base + (int64_t)NORM_BLOCKS * 8);
   for (int g = 0; g < 2; ++g) {
-    w.xr[g][0] = q; q += x;
-    w.xr[g][1] = q; q += x;
-    w.xt[g][0] = q; q += x;
-    w.xt[g][1] = q; q += split ? x : 0;
+    w.x[g][0] = q; q += x;
+    w.x[g][1] = q; q += x;
   }
   w.a[0] = q; q += a;
   w.a[1] = q; q += split ? a : 0;
@@ -78,13 +80,13 @@ __device__ inline NsWs ns_ws(char* base, int mp, int np, bool split) {
   return w;
 }
 
-// the job that owns workgroup `bid` of a launch; FIRST is the launch's offset field
-template <int NsMat::*FIRST>
-__device__ __forceinline__ int ns_job(const NsArgs& p, int bid) {
+// the job that owns workgroup `bid` of a launch; first(j): the launch's first workgroup of job j
+template <typename F>
+__device__ __forceinline__ int ns_job(const NsArgs& p, int bid, F first) {
   int lo = 0, hi = p.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (p.j[mid].*FIRST <= bid) lo = mid; else hi = mid - 1;
+    if (first(p.j[mid]) <= bid) lo = mid; else hi = mid - 1;
   }
   return lo;
 }
@@ -94,43 +96,65 @@ __device__ __forceinline__ void split_f16(float v, _Float16& hi, _Float16& lo) {
   lo = (_Float16)(v - (float)hi);
 }
 
-template <typename T> __device__ __forceinline__ float ld_f(const T* q) { return (float)*q; }
-template <> __device__ __forceinline__ float ld_f<__hip_bfloat16>(const __hip_bfloat16* q) { return __bfloat162float(*q); }
-template <typename T> __device__ __forceinline__ void st_f(T* q, float v) { *q = (T)v; }
-template <> __device__ __forceinline__ void st_f<__hip_bfloat16>(__hip_bfloat16* q, float v) { *q = __float2bfloat16(v); }
+template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[V]; };      // 16 bytes at the type's alignment
 
 // ---- sum of squares (fp64: the range of fp32 gradients squared) in fixed shares; muon: the momentum is advanced here
 template <typename T, bool MUON>
-__global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs p, bool split) {
-  const NsMat& j = p.j[ns_job<&NsMat::norm0>(p, blockIdx.x)];
+__global__ __launch_bounds__(1024) void ns_norm_kernel(NsArgs p, bool split) {
+  constexpr int V = 16 / sizeof(T);
+  const NsMat& j = p.j[ns_job(p, blockIdx.x, [](const NsMat& q) { return q.norm0; })];
   const int local = blockIdx.x - j.norm0, z = local / j.nblk, k = local - z * j.nblk;
   const int rows = j.tall ? j.n : j.m, cols = j.tall ? j.m : j.n;
-  const int64_t total = (int64_t)rows * cols, per = (total + j.nblk - 1) / j.nblk;
+  const int64_t total = (int64_t)rows * cols, per = ((total + j.nblk - 1) / j.nblk + V - 1) / V * V;
   const int64_t e0 = k * per, e1 = e0 + per < total ? e0 + per : total;
   const T* g = (const T*)p.g + j.in + z * j.sti;
+  float* mom = MUON ? p.mom + j.in : nullptr;
   double s = 0.0;
-  for (int64_t e = e0 + threadIdx.x; e < e1; e += 256) {
-    const int64_t r = e / cols, at = r * j.ldi + (e - r * cols);
-    float u = ld_f(g + at);
-    if (MUON) {
-      float* mom = p.mom + j.in + at;
-      const float v = fmaf(p.mu, *mom, u);
-      *mom = v;
-      u = p.nesterov ? fmaf(p.mu, v, u) : v;
+  auto add = [&](float u) { s = fma((double)u, (double)u, s); };
+  if (j.ldi == cols) {                      // one run of values
+    for (int64_t e = e0 + (int64_t)threadIdx.x * V; e < e1; e += 1024 * V) {
+      if (e + V <= e1) {
+        const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(g + e);
+        if (MUON) {
+          Pack<float, V> m = *reinterpret_cast<const Pack<float, V>*>(mom + e);
+#pragma unroll
+          for (int q = 0; q < V; ++q) { m.v[q] = fmaf(p.mu, m.v[q], (float)u.v[q]); add(p.nesterov ? fmaf(p.mu, m.v[q], (float)u.v[q]) : m.v[q]); }
+          *reinterpret_cast<Pack<float, V>*>(mom + e) = m;
+        } else {
+#pragma unroll
+          for (int q = 0; q < V; ++q) add((float)u.v[q]);
+        }
+      } else {
+        for (int64_t q = e; q < e1; ++q) {
+          const float u = (float)g[q];
+          if (MUON) {
+            const float m = fmaf(p.mu, mom[q], u);
+            mom[q] = m;
+            add(p.nesterov ? fmaf(p.mu, m, u) : m);
+          } else {
+            add(u);
+          }
+        }
+      }
     }
-    s += (double)u * (double)u;
+  } else {
+    for (int64_t e = e0 + threadIdx.x; e < e1; e += 1024) { const int64_t r = e / cols; add((float)g[r * j.ldi + (e - r * cols)]); }
   }
   s = wave_sum_d(s);
-  __shared__ double lds[4];
+  __shared__ double lds[16];
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np, split).part[k] = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+  if (threadIdx.x == 0) {
+    double v = 0.0;
+    for (int q = 0; q < 16; ++q) v += lds[q];
+    ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np, split).part[k] = v;
+  }
 }
 
-// ---- X = G / |G| as planes, both orientations: 64 x 64 tiles of the padded matrix in G's own orientation
+// ---- X = G / |G| as planes: 64 x 64 tiles of the padded matrix in G's own orientation, turned in LDS where G is tall
 template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void ns_convert_kernel(NsArgs p, bool split) {
-  const NsMat& j = p.j[ns_job<&NsMat::conv0>(p, blockIdx.x)];
+  const NsMat& j = p.j[ns_job(p, blockIdx.x, [](const NsMat& q) { return q.conv0; })];
   const int rp = j.tall ? j.np : j.mp, cp = j.tall ? j.mp : j.np;        // padded extents in G's orientation
   const int tc = cp / 64, per = tc * (rp / 64);
   int local = blockIdx.x - j.conv0;
@@ -141,6 +165,32 @@ __global__ __launch_bounds__(256) void ns_convert_kernel(NsArgs p, bool split) {
   const NsWs w = ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np, split);
   __shared__ double lds[4];
   __shared__ float tile[64][65];
+  const int c = (threadIdx.x & 15) * 4, rt = threadIdx.x >> 4;
+  const T* g = (const T*)p.g + j.in + z * j.sti;
+  f32x4 v[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int r = r0 + rt + q * 16;
+    const int64_t at = (int64_t)r * j.ldi + c0 + c;
+    v[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (r < rows && c0 + c + 4 <= cols) {
+      const Pack<T, 4> u = *reinterpret_cast<const Pack<T, 4>*>(g + at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[q][e] = (float)u.v[e];
+      if (MUON) {
+        const Pack<float, 4> m = *reinterpret_cast<const Pack<float, 4>*>(p.mom + j.in + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[q][e] = p.nesterov ? fmaf(p.mu, m.v[e], v[q][e]) : m.v[e];
+      }
+    } else if (r < rows) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c0 + c + e < cols) {
+          v[q][e] = (float)g[at + e];
+          if (MUON) v[q][e] = p.nesterov ? fmaf(p.mu, p.mom[j.in + at + e], v[q][e]) : p.mom[j.in + at + e];
+        }
+    }
+  }
   double s = 0.0;
   for (int k = threadIdx.x; k < j.nblk; k += 256) s += w.part[k];
   s = wave_sum_d(s);
@@ -149,77 +199,343 @@ __global__ __launch_bounds__(256) void ns_convert_kernel(NsArgs p, bool split) {
   const double norm = sqrt((lds[0] + lds[1]) + (lds[2] + lds[3]));
   // an infinity or a NaN in the matrix makes every value of it NaN
   const double inv = norm <= (double)p.eps ? 0.0 : norm < INFINITY ? (double)SX / norm : (double)NAN;
-  const T* g = (const T*)p.g + j.in + z * j.sti;
-  _Float16* nh = j.tall ? w.xt[0][0] : w.xr[0][0];
-  _Float16* nl = j.tall ? w.xt[0][1] : w.xr[0][1];
-  _Float16* oh = j.tall ? w.xr[0][0] : w.xt[0][0];
-  _Float16* ol = j.tall ? w.xr[0][1] : w.xt[0][1];
-  const bool keep_nl = split || !j.tall, keep_ol = split || j.tall;        // single: lo beside X only, not beside X^T
-  const int c = threadIdx.x & 63;
-  for (int r = threadIdx.x >> 6; r < 64; r += 4) {
-    float v = 0.f;
-    if (r0 + r < rows && c0 + c < cols) {
-      const int64_t at = (int64_t)(r0 + r) * j.ldi + c0 + c;
-      v = ld_f(g + at);
-      if (MUON) {
-        const float mv = p.mom[j.in + at];
-        v = p.nesterov ? fmaf(p.mu, mv, v) : mv;
-      }
-      v = inv == 0.0 ? 0.f : (float)((double)v * inv);
+  if (!j.tall) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t at = (int64_t)(r0 + rt + q * 16) * cp + c0 + c;
+      f16x4 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { _Float16 h, l; split_f16(inv == 0.0 ? 0.f : (float)((double)v[q][e] * inv), h, l); hi[e] = h; lo[e] = l; }
+      *reinterpret_cast<f16x4*>(w.x[0][0] + at) = hi;
+      *reinterpret_cast<f16x4*>(w.x[0][1] + at) = lo;
     }
-    tile[r][c] = v;
-    _Float16 hi, lo;
-    split_f16(v, hi, lo);
-    nh[(int64_t)(r0 + r) * cp + c0 + c] = hi;
-    if (keep_nl) nl[(int64_t)(r0 + r) * cp + c0 + c] = lo;
+    return;
   }
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tile[rt + q * 16][c + e] = inv == 0.0 ? 0.f : (float)((double)v[q][e] * inv);
   __syncthreads();
-  for (int r = threadIdx.x >> 6; r < 64; r += 4) {
-    _Float16 hi, lo;
-    split_f16(tile[c][r], hi, lo);
-    oh[(int64_t)(c0 + r) * rp + r0 + c] = hi;
-    if (keep_ol) ol[(int64_t)(c0 + r) * rp + r0 + c] = lo;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int r = rt + q * 16;
+    const int64_t at = (int64_t)(c0 + r) * rp + r0 + c;
+    f16x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { _Float16 h, l; split_f16(tile[c + e][r], h, l); hi[e] = h; lo[e] = l; }
+    *reinterpret_cast<f16x4*>(w.x[0][0] + at) = hi;
+    *reinterpret_cast<f16x4*>(w.x[0][1] + at) = lo;
   }
 }
 
-// ---- the three products of a step: D[row][col] = sum_k P[row][k] Q[col][k] over T x T tiles, both operands K-contiguous
-enum { PH_A = 0, PH_B = 1, PH_X = 2, PH_LAST = 3 };
-
+// ---- the products: D[row][col] = sum_k P[row][k] Q[col][k] over T x T tiles, both operands K-contiguous
+//
 // Staging: 16-byte chunks go from global memory straight into LDS.  A wave's 64 lanes fill 1 KiB in lane order, so the chunk a
 // lane FETCHES is permuted instead: chunk c of row r sits in slot c ^ f(r), which spreads the 16 rows an MFMA operand read
 // touches over all banks (BK 64: 8 chunks a row, f = r; BK 32: 4 chunks a row, f = r / 2).
 template <int BK> __device__ __forceinline__ int slot(int r, int c) { return BK == 64 ? c ^ (r & 7) : c ^ ((r >> 1) & 3); }
 
-template <int T, int BK>
-__device__ __forceinline__ void stage(_Float16* lds, const _Float16* src, int64_t ld, int k0) {
-  constexpr int CH = BK / 8, ROWS = 64 / CH;             // chunks per row, rows per wave load
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int r = lane / CH, pos = lane % CH;
+// Product X takes its first operand, whose rows are X's COLUMNS, from X itself: slices of BK rows of X, T columns wide, read by the
+// transposing LDS read (16 lanes give four rows of 16 columns, lane l gets column l).  A copy of X^T instead would be half of all
+// bytes that product X moves.  The 16 rows a read touches are spread over the banks: rows of 128 bytes (T 64) lie on alternating
+// halves of the banks, longer ones all on the same.
+template <int T> __device__ __forceinline__ int slot_t(int r, int c) {
+  return T == 64 ? c ^ (((r >> 1) & 1) * 2 + ((r >> 3) & 1) * 4) : c ^ (2 * ((r & 3) | ((r >> 1) & 4)));
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// columns .. + 15 of the 8 rows from `at` on (pitch T): what a lane of a fragment holds
+template <int T> __device__ __forceinline__ f16x8 frag_t(const _Float16* at) {
+  typedef __attribute__((address_space(3))) s16x4* P;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(const_cast<_Float16*>(at))), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(const_cast<_Float16*>(at + 4 * T)));
+  const f16x4 u = __builtin_bit_cast(f16x4, a), v = __builtin_bit_cast(f16x4, b);
+  return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// T: tile; WR x WC waves share it, each with FR x FC fragments of 16 x 16
+template <int T_, bool SPLIT> struct Tile {
+  static constexpr int T = T_, WR = 2, WC = T_ == 256 ? 4 : 2, WAVES = WR * WC, NT = WAVES * 64;
+  static constexpr int FR = T / WR / 16, FC = T / WC / 16;
+  static constexpr int NP = SPLIT ? 2 : 1, BK = SPLIT ? 32 : 64;
+  static constexpr int PLANE = T * BK, BUF = 2 * NP * PLANE;            // halves: one operand plane, one buffer
+  static constexpr int LP = PLANE * 2 / 1024 / WAVES;                    // loads of a wave per plane
+};
+
+template <typename C>
+struct Acc { f32x4 v[C::FR][C::FC]; };
+
+template <typename C>
+__device__ __forceinline__ void acc_zero(Acc<C>& a) {
 #pragma unroll
-  for (int q = wave; q < T / ROWS; q += 4) {
-    const int row = q * ROWS + r;
-    const _Float16* src_l = src + (int64_t)row * ld + k0 + slot<BK>(row, pos) * 8;
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src_l,
-                                     (__attribute__((address_space(3))) void*)(lds + q * ROWS * BK), 16, 0, 0);
+  for (int i = 0; i < C::FR; ++i)
+#pragma unroll
+    for (int k = 0; k < C::FC; ++k) a.v[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+}
+
+// DEPTH LDS buffers: DEPTH - 1 slices of K are on their way while one is multiplied
+// acc = the product over k0 .. k1 (multiples of BK) of the T rows from P[plane] and Q[plane] on
+// TURN: P[plane] holds the operand by column (row k of it at k * ldp)
+template <typename C, bool SPLIT, int DEPTH, bool TURN>
+__device__ __forceinline__ void ns_product(Acc<C>& acc, const _Float16* const* P, int ldp, const _Float16* const* Q, int ldq, int k0, int k1, _Float16* lds) {
+  constexpr int BK = C::BK, NP = C::NP, T = C::T, CH = BK / 8, ROWS = 64 / CH, CHT = T / 8, ROWST = 64 / CHT;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l15 = lane & 15, lk = lane >> 4;
+  uint32_t from_p[C::LP], from_q[C::LP];                   // bytes from a slice's first value to what this lane fetches
+#pragma unroll
+  for (int u = 0; u < C::LP; ++u) {
+    const int r = (wave * C::LP + u) * ROWS + lane / CH, rt = (wave * C::LP + u) * ROWST + lane / CHT;
+    from_q[u] = (uint32_t)(r * ldq + slot<BK>(r, lane % CH) * 8) * 2u;
+    from_p[u] = TURN ? (uint32_t)(rt * ldp + slot_t<T>(rt, lane % CHT) * 8) * 2u : (uint32_t)(r * ldp + slot<BK>(r, lane % CH) * 8) * 2u;
+  }
+  auto stage = [&](int buf, int k) {
+#pragma unroll
+    for (int o = 0; o < 2; ++o)
+#pragma unroll
+      for (int q = 0; q < NP; ++q) {
+        const char* base = (const char*)(o ? Q[q] + k : TURN ? P[q] + (int64_t)k * ldp : P[q] + k);
+        _Float16* to = lds + buf * C::BUF + (o * NP + q) * C::PLANE + wave * C::LP * 512;
+#pragma unroll
+        for (int u = 0; u < C::LP; ++u)
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + (o ? from_q[u] : from_p[u])),
+                                           (__attribute__((address_space(3))) void*)(to + u * 512), 16, 0, 0);
+      }
+  };
+  const int wr = (wave / C::WC) * (T / C::WR), wc = (wave % C::WC) * (T / C::WC);
+  const int row_q = (wc + l15) * BK;
+  int at_p[C::FR], ch[BK / 32];
+#pragma unroll
+  for (int ks = 0; ks < BK / 32; ++ks) ch[ks] = slot<BK>(l15, ks * 4 + lk) * 8;
+#pragma unroll
+  for (int i = 0; i < C::FR; ++i) {
+    const int r = lk * 8 + (l15 >> 2);
+    at_p[i] = TURN ? r * T + slot_t<T>(r, wr / 8 + 2 * i + ((l15 >> 1) & 1)) * 8 + (l15 & 1) * 4 : (wr + i * 16 + l15) * BK;
+  }
+  // split: sums in two levels, a fresh accumulator every 256 of K.  One accumulator over all of K drifts: each MFMA adds to it
+  // with an error of one step of the sum, and on the diagonal of X X^T, a sum of squares, these do not cancel (a 1 x 4099 matrix:
+  // 2.9e-6 off with one level, fp32 products in torch 6e-7)
+  constexpr int FLUSH = KSHARE / BK;
+  Acc<C> part;
+  acc_zero(acc);
+  if (SPLIT) acc_zero(part);
+  Acc<C>& run = SPLIT ? part : acc;
+  const int nk = (k1 - k0) / BK;
+  constexpr int LOADS = 2 * NP * C::LP;                    // of a wave per buffer
+#pragma unroll
+  for (int b = 0; b < DEPTH - 1; ++b) stage(b, k0 + (b < nk ? b : nk - 1) * BK);
+  int buf = 0, into = DEPTH - 1;
+  for (int kk = 0; kk < nk; ++kk) {
+    // buffer kk has arrived: this wave's loads by its own count (those of the DEPTH - 2 buffers behind it may be in flight), the
+    // other waves' by the barrier, which also tells that buffer kk - 1 has been read and may be filled again
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((DEPTH - 2) * LOADS) : "memory");
+    const int next = kk + DEPTH - 1;
+    stage(into, k0 + (next < nk ? next : nk - 1) * BK);    // past the end: the last slice again, so that the count stays
+    const _Float16* at = lds + buf * C::BUF;
+#pragma unroll
+    for (int ks = 0; ks < BK / 32; ++ks) {
+      f16x8 fp[NP][C::FR], fq[NP][C::FC];
+#pragma unroll
+      for (int q = 0; q < NP; ++q) {
+#pragma unroll
+        for (int i = 0; i < C::FR; ++i)
+          fp[q][i] = TURN ? frag_t<T>(at + q * C::PLANE + at_p[i] + ks * 32 * T) : *reinterpret_cast<const f16x8*>(at + q * C::PLANE + at_p[i] + ch[ks]);
+#pragma unroll
+        for (int k = 0; k < C::FC; ++k) fq[q][k] = *reinterpret_cast<const f16x8*>(at + (NP + q) * C::PLANE + row_q + ch[ks] + k * 16 * BK);
+      }
+#pragma unroll
+      for (int i = 0; i < C::FR; ++i)
+#pragma unroll
+        for (int k = 0; k < C::FC; ++k) {
+          if (SPLIT) {
+            run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[NP - 1][i], fq[0][k], run.v[i][k], 0, 0, 0);
+            run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][i], fq[NP - 1][k], run.v[i][k], 0, 0, 0);
+          }
+          run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][i], fq[0][k], run.v[i][k], 0, 0, 0);
+        }
+    }
+    if (SPLIT && ((kk + 1) % FLUSH == 0 || kk + 1 == nk)) {
+#pragma unroll
+      for (int i = 0; i < C::FR; ++i)
+#pragma unroll
+        for (int k = 0; k < C::FC; ++k) { acc.v[i][k] += part.v[i][k]; part.v[i][k] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+    }
+    buf = buf + 1 == DEPTH ? 0 : buf + 1;
+    into = into + 1 == DEPTH ? 0 : into + 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no load into LDS outlives the workgroup
+}
+
+// halves of LDS a wave needs to turn N x FC fragments into rows of 16-byte stores
+template <int N, int FC> constexpr int ns_turn() { return FC * 16 * (N * 16 + 8) > N * 16 * (FC * 16 + 8) ? FC * 16 * (N * 16 + 8) : N * 16 * (FC * 16 + 8); }
+
+// N x FC fragments (a lane: rows 4 lk .. + 3 of column l15) to dst, the address of the first row and column, through this wave's own
+// LDS: as [row][column] or, BYCOL, as [column][row].  Rows of 32 halves and more leave in 16-byte stores; straight from the
+// fragments they would be stores of 8 and of 2 bytes, in pieces of 32.
+template <int N, int FC, bool BYCOL>
+__device__ __forceinline__ void ns_store(_Float16* turn, const f16x4 (&v)[N][FC], _Float16* dst, int64_t ld) {
+  constexpr int ROWS = BYCOL ? FC * 16 : N * 16, LEN = BYCOL ? N * 16 : FC * 16, PITCH = LEN + 8, CH = LEN / 8;
+  const int lane = threadIdx.x & 63, l15 = lane & 15, lk = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int k = 0; k < FC; ++k) {
+      if (BYCOL) {
+        *reinterpret_cast<f16x4*>(turn + (k * 16 + l15) * PITCH + i * 16 + lk * 4) = v[i][k];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) turn[(i * 16 + lk * 4 + e) * PITCH + k * 16 + l15] = v[i][k][e];
+      }
+    }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the wave's own writes, read by its other lanes
+#pragma unroll
+  for (int q = 0; q < ROWS * CH / 64; ++q) {
+    const int id = q * 64 + lane, r = id / CH, c = id % CH * 8;
+    *reinterpret_cast<f16x8*>(dst + (int64_t)r * ld + c) = *reinterpret_cast<const f16x8*>(turn + r * PITCH + c);
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next call writes
+}
+
+// The operand whose tile a product's result is added to: A (product B) or X (product X), hi and lo, and the diagonals (single).
+template <typename C, bool SPLIT, int PH, int N>
+struct Addend {
+  f16x4 h[N][C::FC], l[N][C::FC];
+  f32x4 drow[N];
+  float dcol[C::FC];
+  __device__ __forceinline__ void load(const NsMat& j, const NsWs& w, int ti, int tj, int gen, int i0) {
+    if (PH == PH_A) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int rbase = ti * C::T + (wave / C::WC) * (C::T / C::WR) + i0 * 16 + (lane >> 4) * 4, cbase = tj * C::T + (wave % C::WC) * (C::T / C::WC) + (lane & 15);
+    const _Float16* hi = PH == PH_B ? w.a[0] : w.x[gen][0];
+    const _Float16* lo = PH == PH_B ? w.a[1] : w.x[gen][1];
+    const int64_t ld = PH == PH_B ? j.mp : j.np;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int k = 0; k < C::FC; ++k) {
+        const int64_t at = (cbase + k * 16) * ld + rbase + i * 16;
+        h[i][k] = *reinterpret_cast<const f16x4*>(hi + at);
+        if (SPLIT || PH != PH_B) l[i][k] = *reinterpret_cast<const f16x4*>(lo + at);
+      }
+    if (!SPLIT) {
+#pragma unroll
+      for (int k = 0; k < C::FC; ++k) dcol[k] = PH == PH_B ? w.da[cbase + k * 16] : w.db[cbase + k * 16];
+      if (PH == PH_B)
+#pragma unroll
+        for (int i = 0; i < N; ++i) drow[i] = *reinterpret_cast<const f32x4*>(w.da + rbase + i * 16);
+    }
+  }
+};
+
+// What a product's tile (ti, tj) of a matrix becomes; N fragment rows of it, from i0 on.  A lane holds rows row0 .. row0 + 3 of
+// column col of each fragment.  The addend is read before the first store: loads and stores share one counter, so a load behind a
+// store waits for it (reading fragment by fragment cost 15 us a tile).
+template <typename C, bool SPLIT, int PH, typename OUT, bool MUON, int N>
+__device__ __forceinline__ void ns_write_rows(const f32x4 (*acc)[C::FC], int i0, const Addend<C, SPLIT, PH, N>& ad, _Float16* lds, const NsArgs& p,
+                                              const NsMat& j, const NsWs& w, int z, int ti, int tj, int gen, float ca, float cb, float cc) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, lk = lane >> 4;
+  const int r0 = ti * C::T + (wave / C::WC) * (C::T / C::WR) + i0 * 16, c0 = tj * C::T + (wave % C::WC) * (C::T / C::WC);
+  f16x4 hi[N][C::FC], lo[N][C::FC];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int k = 0; k < C::FC; ++k) {
+      const int row0 = r0 + i * 16 + lk * 4, col = c0 + k * 16 + l15;
+      const f32x4 sum = acc[i][k];
+      f32x4 v;
+      if (PH == PH_A) {
+        v = sum * (SA / (SX * SX));
+      } else if (PH == PH_B) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float a1 = (float)ad.h[i][k][e] * (1.f / SA), a2 = sum[e] * (1.f / (SA * SA));
+          if (SPLIT) a1 += (float)ad.l[i][k][e] * (1.f / SA);
+          else if (row0 + e == col) { a1 = ad.drow[i][e]; a2 = fmaf(a1, a1, a2); }
+          else a2 = fmaf(ad.drow[i][e] + ad.dcol[k], a1, a2);
+          v[e] = (cb * a1 + cc * a2) * SB;
+        }
+      } else {      // row: column of X, col: row of X
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = fmaf(ca, (float)ad.h[i][k][e] + (float)ad.l[i][k][e], sum[e] * (1.f / SB));
+          if (!SPLIT) v[e] = fmaf(ad.dcol[k], (float)ad.h[i][k][e], v[e]);
+        }
+      }
+      if (PH == PH_LAST) {
+        if (col >= j.m || row0 >= j.n) continue;
+        const int64_t o = j.out + z * j.sto + (j.tall ? (int64_t)row0 * j.ldo + col : (int64_t)col * j.ldo + row0), step = j.tall ? j.ldo : 1;
+        OUT* out = (OUT*)p.out + o;
+        const bool four = !j.tall && row0 + 4 <= j.n;        // four values side by side
+        Pack<OUT, 4> old, res;
+        Pack<float, 4> ema;
+        if (MUON) {
+          if (four) {
+            old = *reinterpret_cast<const Pack<OUT, 4>*>(out);
+            if (p.ema) ema = *reinterpret_cast<const Pack<float, 4>*>(p.ema + o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (row0 + e < j.n) { old.v[e] = out[e * step]; if (p.ema) ema.v[e] = p.ema[o + e * step]; }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = v[e] * (1.f / SX);
+          if (MUON) {
+            x = fmaf(-p.lr * j.scale, x, (float)old.v[e] * (1.f - p.lr * p.wd));
+            ema.v[e] = fmaf(p.ema_decay, ema.v[e], (1.f - p.ema_decay) * x);
+          }
+          res.v[e] = (OUT)x;
+        }
+        if (four) {
+          *reinterpret_cast<Pack<OUT, 4>*>(out) = res;
+          if (MUON && p.ema) *reinterpret_cast<Pack<float, 4>*>(p.ema + o) = ema;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (row0 + e < j.n) { out[e * step] = res.v[e]; if (MUON && p.ema) p.ema[o + e * step] = ema.v[e]; }
+        }
+        continue;
+      }
+      if (PH < PH_X && !SPLIT) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (row0 + e == col) {
+            if (PH == PH_A) w.da[col] = v[e] * (1.f / SA); else w.db[col] = v[e] * (1.f / SB);
+            v[e] = 0.f;
+          }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { _Float16 h, l; split_f16(v[e], h, l); hi[i][k][e] = h; lo[i][k][e] = l; }
+    }
+  if (PH == PH_LAST) return;
+  _Float16* turn = lds + wave * ns_turn<N, C::FC>();
+  if (PH < PH_X) {
+    _Float16* th = PH == PH_A ? w.a[0] : w.b[0];
+    _Float16* tl = PH == PH_A ? w.a[1] : w.b[1];
+    const int64_t down = (int64_t)c0 * j.mp + r0, across = (int64_t)r0 * j.mp + c0;
+    ns_store<N, C::FC, true>(turn, hi, th + down, j.mp);
+    if (SPLIT) ns_store<N, C::FC, true>(turn, lo, tl + down, j.mp);
+    if (ti != tj) {
+      ns_store<N, C::FC, false>(turn, hi, th + across, j.mp);
+      if (SPLIT) ns_store<N, C::FC, false>(turn, lo, tl + across, j.mp);
+    }
+  } else {
+    const int64_t at = (int64_t)c0 * j.np + r0;
+    ns_store<N, C::FC, true>(turn, hi, w.x[gen ^ 1][0] + at, j.np);
+    ns_store<N, C::FC, true>(turn, lo, w.x[gen ^ 1][1] + at, j.np);
   }
 }
 
-template <int T, int BK>
-__device__ __forceinline__ f16x8 frag(const _Float16* lds, int row, int chunk) {
-  return *reinterpret_cast<const f16x8*>(lds + row * BK + slot<BK>(row, chunk) * 8);
-}
-
-template <int T, bool SPLIT, int PH, typename OUT, bool MUON>
-__global__ __launch_bounds__(256) void ns_gemm_kernel(NsArgs p, int gen, float ca, float cb, float cc) {
-  constexpr int BK = SPLIT ? 32 : 64, NP = SPLIT ? 2 : 1, F = T / 32;      // F x F fragments of 16 x 16 per wave
-  __shared__ __attribute__((aligned(16))) _Float16 lds[2][2][NP][T * BK];  // [buffer][operand][plane]
-  const NsMat& j = p.j[PH >= PH_X ? ns_job<&NsMat::x0>(p, blockIdx.x) : ns_job<&NsMat::sym0>(p, blockIdx.x)];
-  int local = blockIdx.x - (PH >= PH_X ? j.x0 : j.sym0), z, ti, tj;
+// matrix z and tile (ti, tj) of tile `local` of a job
+template <int T, int PH>
+__device__ __forceinline__ void ns_tile(const NsMat& j, int local, int& z, int& ti, int& tj) {
   const int nt = j.mp / T;
   if (PH >= PH_X) {
     const int per = nt * (j.np / T);
     z = local / per; local -= z * per;
-    ti = local / nt; tj = local - ti * nt;               // rows: X's columns, columns: X's rows
+    // rows: X's columns, columns: X's rows.  Bands of 8 tile rows: the tiles a die works on at a time form a square, which reads
+    // the fewest operand rows
+    const int nr = j.np / T, band = local / (8 * nt), in = local - band * 8 * nt, high = nr - band * 8 < 8 ? nr - band * 8 : 8;
+    tj = in / high; ti = band * 8 + (in - tj * high);
   } else {
     const int per = nt * (nt + 1) / 2;
     z = local / per; local -= z * per;
@@ -227,183 +543,173 @@ __global__ __launch_bounds__(256) void ns_gemm_kernel(NsArgs p, int gen, float c
     while (local >= nt - ti) { local -= nt - ti; ++ti; }
     tj = ti + local;                                     // upper triangle: the product is symmetric
   }
+}
+
+// One workgroup per tile, or, of the tiles behind direct[], per share of a tile's K, which goes to the slab: the tiles of a small
+// call do not fill the chip, and neither do those that are left over from its last full round.
+template <int T, bool SPLIT, int DEPTH, int PH, typename OUT, bool MUON>
+__global__ __launch_bounds__((Tile<T, SPLIT>::NT), 2) void ns_gemm_kernel(NsArgs p, int gen, float ca, float cb, float cc) {
+  typedef Tile<T, SPLIT> C;
+  constexpr int Q3 = PH < PH_X ? PH : 2;
+  extern __shared__ __attribute__((aligned(16))) _Float16 lds[];
+  const int direct = p.direct[Q3], bid = blockIdx.x;
+  const bool whole = bid < direct;
+  int job, tile, share = 0, slot_at = 0;
+  if (whole) {
+    // neighbouring workgroups go to different dies (8, each with an L2 of its own): give each die a run of neighbouring tiles
+    const int run = direct >> 3;
+    const int t = bid < run * 8 ? (bid & 7) * run + (bid >> 3) : bid;
+    job = ns_job(p, t, [](const NsMat& q) { return q.tile0[Q3]; });
+    tile = t - p.j[job].tile0[Q3];
+  } else {
+    // the shares of a slice of K side by side, and on one die: they read the same operands
+    slot_at = bid - direct;
+    const int run = ((int)gridDim.x - direct) >> 3;
+    if (slot_at < run * 8) slot_at = (slot_at & 7) * run + (slot_at >> 3);
+    job = ns_job(p, slot_at, [](const NsMat& q) { return q.share0[Q3]; });
+    const int at = slot_at - p.j[job].share0[Q3], n = p.j[job].cut[Q3];
+    share = at / n;
+    tile = at - share * n;
+    if (p.j[job].tile0[Q3] < direct) tile += direct - p.j[job].tile0[Q3];
+  }
+  const NsMat& j = p.j[job];
+  int z, ti, tj;
+  ns_tile<T, PH>(j, tile, z, ti, tj);
   const NsWs w = ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np, SPLIT);
-  const int64_t ld = PH == PH_A ? j.np : j.mp;
-  const int K = (int)ld;
+  const int ld = PH == PH_A ? j.np : j.mp;                 // of the second operand, and K
   const _Float16* P[2]; const _Float16* Q[2];
 #pragma unroll
-  for (int q = 0; q < NP; ++q) {
-    P[q] = (PH == PH_A ? w.xr[gen][q] : PH == PH_B ? w.a[q] : w.xt[gen][q]) + (int64_t)ti * T * ld;
-    Q[q] = (PH == PH_A ? w.xr[gen][q] : PH == PH_B ? w.a[q] : w.b[q]) + (int64_t)tj * T * ld;
+  for (int q = 0; q < C::NP; ++q) {
+    P[q] = PH >= PH_X ? w.x[gen][q] + ti * T : (PH == PH_A ? w.x[gen][q] : w.a[q]) + (int64_t)ti * T * ld;
+    Q[q] = (PH == PH_A ? w.x[gen][q] : PH == PH_B ? w.a[q] : w.b[q]) + (int64_t)tj * T * ld;
   }
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, lk = lane >> 4;
-  const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
-  f32x4 acc[F][F];
-#pragma unroll
-  for (int i = 0; i < F; ++i)
-#pragma unroll
-    for (int k = 0; k < F; ++k) acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
-  // split: sums in two levels, a fresh accumulator every 256 of K.  One accumulator over all of K drifts: each MFMA adds to it
-  // with an error of one step of the sum, and on the diagonal of X X^T, a sum of squares, these do not cancel (a 1 x 4099 matrix:
-  // 2.9e-6 off with one level, fp32 products in torch 6e-7)
-  constexpr int FLUSH = 256 / BK;
-  f32x4 sum[SPLIT ? F : 1][SPLIT ? F : 1];
-  if (SPLIT) {
-#pragma unroll
-    for (int i = 0; i < F; ++i)
-#pragma unroll
-      for (int k = 0; k < F; ++k) sum[SPLIT ? i : 0][SPLIT ? k : 0] = f32x4{0.f, 0.f, 0.f, 0.f};
+  int k0 = 0, k1 = ld;
+  if (!whole) {
+    const int per = (ld + j.shares[Q3] * 64 - 1) / (j.shares[Q3] * 64) * 64;      // shares are multiples of 64
+    k0 = share * per;
+    k1 = k0 + per < ld ? k0 + per : ld;
   }
-  const int nk = K / BK;
-#pragma unroll
-  for (int q = 0; q < NP; ++q) { stage<T, BK>(lds[0][0][q], P[q], ld, 0); stage<T, BK>(lds[0][1][q], Q[q], ld, 0); }
-  for (int kk = 0; kk < nk; ++kk) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this buffer's chunks have arrived (mine; the barrier covers the others')
-    __syncthreads();
-    const int cur = kk & 1;
-    if (kk + 1 < nk) {
-#pragma unroll
-      for (int q = 0; q < NP; ++q) {
-        stage<T, BK>(lds[cur ^ 1][0][q], P[q], ld, (kk + 1) * BK);
-        stage<T, BK>(lds[cur ^ 1][1][q], Q[q], ld, (kk + 1) * BK);
-      }
+  // 64: the addend waits in registers through the product; larger tiles read it behind it, in halves
+  constexpr int N = T == 256 ? 4 : 2;
+  Acc<C> acc;
+  Addend<C, SPLIT, PH, N> ad;
+  if (T == 64 && whole) ad.load(j, w, ti, tj, gen, 0);
+  ns_product<C, SPLIT, DEPTH, (PH >= PH_X)>(acc, P, PH >= PH_X ? j.np : ld, Q, ld, k0, k1, lds);
+  if (whole) {
+    if (T != 64) ad.load(j, w, ti, tj, gen, 0);
+    __syncthreads();                                       // the slices in LDS have been read: it turns the results now
+    ns_write_rows<C, SPLIT, PH, OUT, MUON, N>(acc.v, 0, ad, lds, p, j, w, z, ti, tj, gen, ca, cb, cc);
+    if (C::FR > N) {
+      ad.load(j, w, ti, tj, gen, N);
+      ns_write_rows<C, SPLIT, PH, OUT, MUON, N>(acc.v + C::FR - N, N, ad, lds, p, j, w, z, ti, tj, gen, ca, cb, cc);
     }
+  } else {
+    f32x4* to = reinterpret_cast<f32x4*>(p.slab) + (int64_t)slot_at * (T * T / 4) + threadIdx.x;
 #pragma unroll
-    for (int ks = 0; ks < BK / 32; ++ks) {
-      f16x8 fp[NP][F], fq[NP][F];
+    for (int i = 0; i < C::FR; ++i)
 #pragma unroll
-      for (int q = 0; q < NP; ++q)
-#pragma unroll
-        for (int i = 0; i < F; ++i) {
-          fp[q][i] = frag<T, BK>(lds[cur][0][q], wr + i * 16 + l15, ks * 4 + lk);
-          fq[q][i] = frag<T, BK>(lds[cur][1][q], wc + i * 16 + l15, ks * 4 + lk);
-        }
-#pragma unroll
-      for (int i = 0; i < F; ++i)
-#pragma unroll
-        for (int k = 0; k < F; ++k) {
-          if (SPLIT) {
-            acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[NP - 1][i], fq[0][k], acc[i][k], 0, 0, 0);
-            acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][i], fq[NP - 1][k], acc[i][k], 0, 0, 0);
-          }
-          acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][i], fq[0][k], acc[i][k], 0, 0, 0);
-        }
-    }
-    if (SPLIT && ((kk + 1) % FLUSH == 0 || kk + 1 == nk)) {
-#pragma unroll
-      for (int i = 0; i < F; ++i)
-#pragma unroll
-        for (int k = 0; k < F; ++k) { sum[SPLIT ? i : 0][SPLIT ? k : 0] += acc[i][k]; acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f}; }
-    }
+      for (int k = 0; k < C::FC; ++k) to[(i * C::FC + k) * C::NT] = acc.v[i][k];
   }
-  if (SPLIT) {
+}
+
+// the split tiles: their shares added in order, then as any other tile; a workgroup per row of fragments
+template <int T, bool SPLIT, int PH, typename OUT, bool MUON>
+__global__ __launch_bounds__((Tile<T, SPLIT>::NT)) void ns_join_kernel(NsArgs p, int gen, float ca, float cb, float cc) {
+  typedef Tile<T, SPLIT> C;
+  constexpr int Q3 = PH < PH_X ? PH : 2;
+  const int direct = p.direct[Q3], t = direct + blockIdx.x / C::FR, i = blockIdx.x % C::FR;
+  const NsMat& j = p.j[ns_job(p, t, [](const NsMat& q) { return q.tile0[Q3]; })];
+  const int first = j.tile0[Q3] > direct ? j.tile0[Q3] : direct, n = j.shares[Q3];
+  const f32x4* from = reinterpret_cast<const f32x4*>(p.slab) + (int64_t)(j.share0[Q3] + t - first) * (T * T / 4) + i * C::FC * C::NT + threadIdx.x;
+  const int64_t next = (int64_t)j.cut[Q3] * (T * T / 4);
+  __shared__ __attribute__((aligned(16))) _Float16 lds[C::WAVES * ns_turn<1, C::FC>()];
+  int z, ti, tj;
+  ns_tile<T, PH>(j, t - j.tile0[Q3], z, ti, tj);
+  const NsWs w = ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np, SPLIT);
+  Addend<C, SPLIT, PH, 1> ad;
+  ad.load(j, w, ti, tj, gen, i);
+  f32x4 v[1][C::FC];
 #pragma unroll
-    for (int i = 0; i < F; ++i)
+  for (int k = 0; k < C::FC; ++k) v[0][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < n; ++s)
 #pragma unroll
-      for (int k = 0; k < F; ++k) acc[i][k] = sum[SPLIT ? i : 0][SPLIT ? k : 0];
-  }
-  // a lane holds rows row0 .. row0 + 3 of column col of each fragment
-#pragma unroll
-  for (int i = 0; i < F; ++i)
-#pragma unroll
-    for (int k = 0; k < F; ++k) {
-      const int row0 = ti * T + wr + i * 16 + lk * 4, col = tj * T + wc + k * 16 + l15;
-      f16x4 hi, lo;
-      if (PH < PH_X) {
-        f32x4 v;
-        if (PH == PH_A) {
-          v = acc[i][k] * (SA / (SX * SX));
-        } else {
-          const int64_t at = (int64_t)col * j.mp + row0;                    // A is symmetric: four consecutive values
-          const f16x4 ah = *reinterpret_cast<const f16x4*>(w.a[0] + at);
-          f16x4 al;
-          if (SPLIT) al = *reinterpret_cast<const f16x4*>(w.a[1] + at);
-          const float dcol = SPLIT ? 0.f : w.da[col];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float a1 = (float)ah[e] * (1.f / SA), a2 = acc[i][k][e] * (1.f / (SA * SA));
-            if (SPLIT) {
-              a1 += (float)al[e] * (1.f / SA);
-            } else {
-              const float drow = w.da[row0 + e];
-              if (row0 + e == col) { a1 = drow; a2 = fmaf(drow, drow, a2); }
-              else a2 = fmaf(drow + dcol, a1, a2);
-            }
-            v[e] = (cb * a1 + cc * a2) * SB;
-          }
-        }
-        if (!SPLIT) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (row0 + e == col) {
-              if (PH == PH_A) w.da[col] = v[e] * (1.f / SA); else w.db[col] = v[e] * (1.f / SB);
-              v[e] = 0.f;
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { _Float16 h, l; split_f16(v[e], h, l); hi[e] = h; lo[e] = l; }
-        _Float16* oh = PH == PH_A ? w.a[0] : w.b[0];
-        _Float16* ol = PH == PH_A ? w.a[1] : w.b[1];
-        *reinterpret_cast<f16x4*>(oh + (int64_t)col * j.mp + row0) = hi;
-        if (SPLIT) *reinterpret_cast<f16x4*>(ol + (int64_t)col * j.mp + row0) = lo;
-        if (ti != tj) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            oh[(int64_t)(row0 + e) * j.mp + col] = hi[e];
-            if (SPLIT) ol[(int64_t)(row0 + e) * j.mp + col] = lo[e];
-          }
-        }
-      } else {
-        // row: column of X, col: row of X
-        const int64_t at = (int64_t)col * j.np + row0;
-        const f16x4 xh = *reinterpret_cast<const f16x4*>(w.xr[gen][0] + at), xl = *reinterpret_cast<const f16x4*>(w.xr[gen][1] + at);
-        const float dcol = SPLIT ? 0.f : w.db[col];
-        f32x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = fmaf(ca, (float)xh[e] + (float)xl[e], acc[i][k][e] * (1.f / SB));
-          if (!SPLIT) v[e] = fmaf(dcol, (float)xh[e], v[e]);
-        }
-        if (PH == PH_X) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { _Float16 h, l; split_f16(v[e], h, l); hi[e] = h; lo[e] = l; }
-          *reinterpret_cast<f16x4*>(w.xr[gen ^ 1][0] + at) = hi;
-          *reinterpret_cast<f16x4*>(w.xr[gen ^ 1][1] + at) = lo;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            w.xt[gen ^ 1][0][(int64_t)(row0 + e) * j.mp + col] = hi[e];
-            if (SPLIT) w.xt[gen ^ 1][1][(int64_t)(row0 + e) * j.mp + col] = lo[e];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (row0 + e >= j.n || col >= j.m) continue;
-            const float x = v[e] * (1.f / SX);
-            const int64_t o = j.out + z * j.sto + (j.tall ? (int64_t)(row0 + e) * j.ldo + col : (int64_t)col * j.ldo + row0 + e);
-            OUT* out = (OUT*)p.out + o;
-            if (MUON) {
-              const float q = fmaf(-p.lr * j.scale, x, ld_f(out) * (1.f - p.lr * p.wd));
-              st_f(out, q);
-              if (p.ema) p.ema[o] = fmaf(p.ema_decay, p.ema[o], (1.f - p.ema_decay) * q);
-            } else {
-              st_f(out, x);
-            }
-          }
-        }
-      }
-    }
+    for (int k = 0; k < C::FC; ++k) v[0][k] += from[s * next + k * C::NT];
+  ns_write_rows<C, SPLIT, PH, OUT, MUON, 1>(v, i, ad, lds, p, j, w, z, ti, tj, gen, ca, cb, cc);
 }
 
 // ---- host side
-struct NsPlan { int64_t bytes; int64_t norm, conv, sym, x; int T; };
+// launches of a call: workgroups of norm and conversion; per product its tile size, workgroups (whole tiles and shares) and split tiles
+struct NsPlan { int64_t bytes, norm, conv; int T[3]; int64_t grid[3], join[3]; };
 
 inline int64_t up(int64_t v, int64_t k) { return (v + k - 1) / k * k; }
+
+// Tile sizes of the products, from the number of tiles that each size would make.
+// X: 128 from 384 tiles on (1024 x 8192 fp32, 512 tiles: 820 -> 712 us a call; 1024 x 4096, 256 tiles: 508 -> 566), and 256 (single
+//   only: split has no registers for it) from a full round of 256 tiles on (4096 x 8192 bf16: 3207 -> 3056 us).
+// A and B, whose leftover tiles are split along K, go by tiles x K: split 128 from 192 K on (1024 x 8192, A 288 K: 712 -> 673 us;
+//   4 x 1024 x 1024, 144 K: 634 -> 642), single from 400 K on (1536 x 6144, A 468 K: 626 -> 598 us; 1024 x 8192, 288 K: 406 -> 413).
+void ns_tile_sizes(const NsArgs& p, bool split, NsPlan& pl) {
+  int64_t a = 0, b = 0, x = 0, x256 = 0;
+  for (int i = 0; i < p.n; ++i) {
+    const NsMat& j = p.j[i];
+    const int64_t m = up(j.m, 128) / 128, n = up(j.n, 128) / 128, sym = m * (m + 1) / 2 * j.count;
+    a += sym * n * 128;
+    b += sym * m * 128;
+    x += m * n * j.count;
+    x256 += ((m + 1) / 2) * ((n + 1) / 2) * j.count;
+  }
+  const int64_t least = (split ? 192 : 400) * 1024;
+  pl.T[0] = a >= least ? 128 : 64;
+  pl.T[1] = b >= least ? 128 : 64;
+  pl.T[2] = !split && x256 >= 256 ? 256 : x >= 384 ? 128 : 64;
+}
+
+// Tiles and shares of product q (A, B, X).  `slots` workgroups run at a time; whole rounds of them take a tile each, and what is
+// left over is split along K until it fills a round of its own, in shares of no less than KSHARE.
+int ns_tiles(NsArgs& p, NsPlan& pl, int q, int64_t& slab) {
+  const int T = pl.T[q];
+  int64_t tiles = 0;
+  for (int i = 0; i < p.n; ++i) {
+    NsMat& j = p.j[i];
+    const int64_t nt = j.mp / T, nx = j.np / T;
+    j.tile0[q] = (int)tiles;
+    tiles += (q == 2 ? nt * nx : nt * (nt + 1) / 2) * j.count;
+    if (tiles > INT32_MAX / 64) return ITG_ERR_ARG;
+  }
+  const int64_t slots = 256 * (T == 256 ? 1 : 2);
+  int64_t direct = tiles / slots * slots, rest = tiles - direct, shares = 0;
+  // more than half a round left, or nothing to split: the last round stays as it is
+  bool splits = false;
+  for (int i = 0; i < p.n; ++i) splits |= (q == 0 ? p.j[i].np : p.j[i].mp) >= KLONG;
+  if (!splits || rest * 2 > slots) { direct = tiles; rest = 0; }
+  if (rest) {
+    for (int64_t per = KSHARE;; per += KSHARE) {           // the shortest shares that fit one round
+      shares = 0;
+      for (int i = 0; i < p.n; ++i) {
+        NsMat& j = p.j[i];
+        const int64_t end = i + 1 < p.n ? p.j[i + 1].tile0[q] : tiles, first = j.tile0[q] > direct ? j.tile0[q] : direct;
+        const int K = q == 0 ? j.np : j.mp;
+        j.share0[q] = (int)shares;
+        j.shares[q] = (int)((K + per - 1) / per);
+        j.cut[q] = (int)(end > first ? end - first : 0);
+        shares += (int64_t)j.cut[q] * j.shares[q];
+      }
+      if (shares <= slots || per >= ITG_NS_MAX_DIM) break;
+    }
+  }
+  p.direct[q] = (int)direct;
+  pl.grid[q] = direct + shares;
+  pl.join[q] = rest;
+  if (shares * T * T * 4 > slab) slab = shares * T * T * 4;
+  return ITG_OK;
+}
 
 // fills p.j[] from the jobs; returns a status
 int ns_plan(const itg_ns_job* jobs, int n, bool split, bool muon, NsArgs& p, NsPlan& pl) {
   if (!jobs || n < 1 || n > ITG_NS_MAX_JOBS) return ITG_ERR_ARG;
   p.n = n;
-  pl = NsPlan{0, 0, 0, 0, 0, 64};
+  pl = NsPlan{};
   for (int i = 0; i < n; ++i) {
     const itg_ns_job& q = jobs[i];
     if (q.rows < 1 || q.cols < 1 || q.rows > ITG_NS_MAX_DIM || q.cols > ITG_NS_MAX_DIM || q.count < 1 || q.reserved) return ITG_ERR_ARG;
@@ -416,25 +722,35 @@ int ns_plan(const itg_ns_job* jobs, int n, bool split, bool muon, NsArgs& p, NsP
     NsMat& j = p.j[i];
     j.tall = q.rows > q.cols;
     j.m = j.tall ? q.cols : q.rows; j.n = j.tall ? q.rows : q.cols;
-    j.mp = (int)up(j.m, pl.T); j.np = (int)up(j.n, pl.T);
     j.count = q.count;
+  }
+  ns_tile_sizes(p, split, pl);
+  const int T = pl.T[2] > pl.T[0] ? pl.T[2] : pl.T[0] > pl.T[1] ? pl.T[0] : pl.T[1];
+  for (int i = 0; i < n; ++i) {
+    const itg_ns_job& q = jobs[i];
+    NsMat& j = p.j[i];
+    j.mp = (int)up(j.m, T); j.np = (int)up(j.n, T);
     const int64_t blocks = ((int64_t)j.m * j.n + NORM_ELEMS - 1) / NORM_ELEMS;
     j.nblk = (int)(blocks < NORM_BLOCKS ? blocks : NORM_BLOCKS);
     j.scale = sqrtf(fmaxf(1.f, (float)q.rows / (float)q.cols));
     j.in = q.in_offset; j.ldi = q.in_ld; j.sti = q.in_stride;
     j.out = q.out_offset; j.ldo = q.out_ld; j.sto = q.out_stride;
-    const int64_t nt = j.mp / pl.T, nx = j.np / pl.T;
-    j.norm0 = (int)pl.norm; j.conv0 = (int)pl.conv; j.sym0 = (int)pl.sym; j.x0 = (int)pl.x;
+    j.norm0 = (int)pl.norm; j.conv0 = (int)pl.conv;
     pl.norm += (int64_t)j.nblk * j.count;
     pl.conv += (int64_t)(j.mp / 64) * (j.np / 64) * j.count;
-    pl.sym += nt * (nt + 1) / 2 * j.count;
-    pl.x += nt * nx * j.count;
-    if (pl.norm > INT32_MAX || pl.conv > INT32_MAX || pl.sym > INT32_MAX || pl.x > INT32_MAX) return ITG_ERR_ARG;
+    if (pl.norm > INT32_MAX || pl.conv > INT32_MAX) return ITG_ERR_ARG;
     j.wst = up(ns_ws_bytes(j.mp, j.np, split), 256);
     j.ws = pl.bytes;
     if (j.wst > ((int64_t)1 << 60) / j.count) return ITG_ERR_ARG;
     pl.bytes += j.wst * j.count;
   }
+  int64_t slab = 0;
+  for (int q = 0; q < 3; ++q) {
+    const int rc = ns_tiles(p, pl, q, slab);
+    if (rc) return rc;
+  }
+  p.slab = (float*)pl.bytes;      // an offset until the call has its workspace
+  pl.bytes += slab;
   return ITG_OK;
 }
 
@@ -456,24 +772,48 @@ bool ns_coefficients_ok(const float* abc, int steps) {
   return true;
 }
 
+template <int T, bool SPLIT, int DEPTH, int PH, typename OUT, bool MUON>
+int ns_launch(const NsArgs& p, const NsPlan& pl, int gen, const float* abc, hipStream_t s) {
+  typedef Tile<T, SPLIT> C;
+  constexpr int Q3 = PH < PH_X ? PH : 2, LDS = DEPTH * C::BUF * 2;
+  if (LDS > 64 * 1024 &&
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&ns_gemm_kernel<T, SPLIT, DEPTH, PH, OUT, MUON>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
+    return ITG_ERR_LAUNCH;
+  hipLaunchKernelGGL((ns_gemm_kernel<T, SPLIT, DEPTH, PH, OUT, MUON>), dim3((unsigned)pl.grid[Q3]), dim3(C::NT), LDS, s, p, gen, abc[0], abc[1], abc[2]);
+  ITG_CHECK_LAUNCH();
+  if (pl.join[Q3]) {
+    hipLaunchKernelGGL((ns_join_kernel<T, SPLIT, PH, OUT, MUON>), dim3((unsigned)(pl.join[Q3] * C::FR)), dim3(C::NT), 0, s, p, gen, abc[0], abc[1], abc[2]);
+    ITG_CHECK_LAUNCH();
+  }
+  return ITG_OK;
+}
+
+template <bool SPLIT, int PH, typename OUT, bool MUON>
+int ns_phase(const NsArgs& p, const NsPlan& pl, int gen, const float* abc, hipStream_t s) {
+  const int T = pl.T[PH < PH_X ? PH : 2];
+  const int64_t grid = pl.grid[PH < PH_X ? PH : 2];
+  // 64: four buffers while two workgroups a CU take the whole launch (2 x 333 x 1501 bf16: 156 us against 162 with two), two buffers
+  // and up to five workgroups a CU beyond
+  if (T == 64 && grid <= 512) return ns_launch<64, SPLIT, 4, PH, OUT, MUON>(p, pl, gen, abc, s);
+  if (T == 64) return ns_launch<64, SPLIT, 2, PH, OUT, MUON>(p, pl, gen, abc, s);
+  if (SPLIT || T == 128) return ns_launch<128, SPLIT, 2, PH, OUT, MUON>(p, pl, gen, abc, s);
+  constexpr int BIG = !SPLIT && PH >= PH_X ? 256 : 128;
+  return ns_launch<BIG, SPLIT, 2, PH, OUT, MUON>(p, pl, gen, abc, s);
+}
+
 template <typename T, bool SPLIT, bool MUON>
-int ns_run(const NsArgs& p, const NsPlan& pl, const float* abc, int steps, hipStream_t s) {
-  hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)pl.norm), dim3(256), 0, s, p, SPLIT);
+int ns_run(NsArgs& p, const NsPlan& pl, const float* abc, int steps, hipStream_t s) {
+  p.slab = (float*)(p.ws + (int64_t)p.slab);
+  hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)pl.norm), dim3(1024), 0, s, p, SPLIT);
   ITG_CHECK_LAUNCH();
   hipLaunchKernelGGL((ns_convert_kernel<T, MUON>), dim3((unsigned)pl.conv), dim3(256), 0, s, p, SPLIT);
   ITG_CHECK_LAUNCH();
-  const dim3 sym((unsigned)pl.sym), x((unsigned)pl.x);
   for (int k = 0; k < steps; ++k, abc += 3) {
     const int gen = k & 1;
-    hipLaunchKernelGGL((ns_gemm_kernel<64, SPLIT, PH_A, T, MUON>), sym, dim3(256), 0, s, p, gen, abc[0], abc[1], abc[2]);
-    ITG_CHECK_LAUNCH();
-    hipLaunchKernelGGL((ns_gemm_kernel<64, SPLIT, PH_B, T, MUON>), sym, dim3(256), 0, s, p, gen, abc[0], abc[1], abc[2]);
-    ITG_CHECK_LAUNCH();
-    if (k + 1 < steps)
-      hipLaunchKernelGGL((ns_gemm_kernel<64, SPLIT, PH_X, T, MUON>), x, dim3(256), 0, s, p, gen, abc[0], abc[1], abc[2]);
-    else
-      hipLaunchKernelGGL((ns_gemm_kernel<64, SPLIT, PH_LAST, T, MUON>), x, dim3(256), 0, s, p, gen, abc[0], abc[1], abc[2]);
-    ITG_CHECK_LAUNCH();
+    int rc = ns_phase<SPLIT, PH_A, T, MUON>(p, pl, gen, abc, s);
+    if (!rc) rc = ns_phase<SPLIT, PH_B, T, MUON>(p, pl, gen, abc, s);
+    if (!rc) rc = k + 1 < steps ? ns_phase<SPLIT, PH_X, T, MUON>(p, pl, gen, abc, s) : ns_phase<SPLIT, PH_LAST, T, MUON>(p, pl, gen, abc, s);
+    if (rc) return rc;
   }
   return ITG_OK;
 }
@@ -503,7 +843,7 @@ int itg_newton_schulz(const itg_ns_job* jobs, int n, int dtype, const void* g, v
   p.mu = p.lr = p.wd = p.ema_decay = 0.f;
   hipStream_t s = (hipStream_t)stream;
   if (dtype == ITG_F32) return ns_run<float, true, false>(p, pl, coefficients, steps, s);
-  if (dtype == ITG_BF16) return ns_run<__hip_bfloat16, false, false>(p, pl, coefficients, steps, s);
+  if (dtype == ITG_BF16) return ns_run<__bf16, false, false>(p, pl, coefficients, steps, s);
   return ns_run<_Float16, true, false>(p, pl, coefficients, steps, s);
 }
 

@@ -252,3 +252,17 @@ def test_refusals(ops):
                 lambda: ops.muon_step(plan, flat[0], torch.zeros(64, device="cuda")[::2], flat[2])):
         with pytest.raises(ItgError):
             bad()
+
+
+@pytest.mark.parametrize("t,m,n,batch", [("f32", 2048, 2048, 1), ("f32", 1408, 5000, 1), ("f32", 2600, 2500, 1), ("f32", 6000, 900, 2), ("f16", 1030, 8200, 1),
+                                         ("bf16", 2560, 2560, 1), ("bf16", 4096, 4100, 1), ("bf16", 9000, 2050, 1), ("bf16", 700, 1100, 9)])
+def test_every_tile_size(ops, t, m, n, batch):
+    """calls large enough for the larger tiles, alone and mixed between the three products, with whole rounds of tiles and with a
+    rest that is split along K; the oracle's products run in 64 bits on the GPU"""
+    g = torch.stack([matrix(m, n, seed=s) for s in range(batch)]).cuda().to(TYPES[t])
+    got = ops.orthogonalize(g)
+    for z in range(batch):
+        want, own = steps_of(g[z].double()), steps_of(g[z].float().cpu()).cuda() if m * n < 3e6 else None
+        off = rel(got[z], want)
+        own = rel(own, want) if own is not None else 4e-6      # fp32 chains of this kind: 2e-6 .. 4e-6 off
+        assert off <= (2.0 ** -8 if t == "bf16" else 3 * own + (2.0 ** -11 if t == "f16" else 0.0)), (z, off, own)
