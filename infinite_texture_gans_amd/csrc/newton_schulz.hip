@@ -36,6 +36,7 @@ struct NsMat {                 // one job: `count` matrices of the same shape
   int count, tall, nblk;       // tall: the matrix has more rows than columns (X is its transpose)
   int norm0, conv0;            // first workgroup of this job in the launches
   int tile0[3], share0[3], shares[3], cut[3];      // per product (A, B, X): first tile, first share, shares of a split tile, split tiles
+  int block0, blocks, subs;    // short sides: first workgroup, workgroups per matrix, column blocks per workgroup
   float scale;                 // muon: sqrt(max(1, rows / cols))
   int64_t in, ldi, sti, out, ldo, sto;      // element offsets, row strides, matrix strides
   int64_t ws, wst;             // bytes: first matrix's workspace, stride between matrices
@@ -98,9 +99,54 @@ __device__ __forceinline__ void split_f16(float v, _Float16& hi, _Float16& lo) {
 
 template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[V]; };      // 16 bytes at the type's alignment
 
+// what G is multiplied with, from the sum of its squares: 0 = a matrix without a direction; an infinity or a NaN in the matrix makes
+// every value of it NaN
+__device__ __forceinline__ double ns_scale(double sum, float eps) {
+  const double norm = sqrt(sum);
+  return norm <= (double)eps ? 0.0 : norm < INFINITY ? (double)SX / norm : (double)NAN;
+}
+
+// four values of the result (columns row0 .. + 3 of X's row `col`), or what the optimiser step makes of them
+template <typename OUT, bool MUON>
+__device__ __forceinline__ void ns_result(const NsArgs& p, const NsMat& j, int z, int row0, int col, const f32x4& v) {
+  if (col >= j.m || row0 >= j.n) return;
+  const int64_t o = j.out + z * j.sto + (j.tall ? (int64_t)row0 * j.ldo + col : (int64_t)col * j.ldo + row0), step = j.tall ? j.ldo : 1;
+  OUT* out = (OUT*)p.out + o;
+  const bool four = !j.tall && row0 + 4 <= j.n;        // four values side by side
+  Pack<OUT, 4> old, res;
+  Pack<float, 4> ema;
+  if (MUON) {
+    if (four) {
+      old = *reinterpret_cast<const Pack<OUT, 4>*>(out);
+      if (p.ema) ema = *reinterpret_cast<const Pack<float, 4>*>(p.ema + o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (row0 + e < j.n) { old.v[e] = out[e * step]; if (p.ema) ema.v[e] = p.ema[o + e * step]; }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float x = v[e] * (1.f / SX);
+    if (MUON) {
+      x = fmaf(-p.lr * j.scale, x, (float)old.v[e] * (1.f - p.lr * p.wd));
+      ema.v[e] = fmaf(p.ema_decay, ema.v[e], (1.f - p.ema_decay) * x);
+    }
+    res.v[e] = (OUT)x;
+  }
+  if (four) {
+    *reinterpret_cast<Pack<OUT, 4>*>(out) = res;
+    if (MUON && p.ema) *reinterpret_cast<Pack<float, 4>*>(p.ema + o) = ema;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (row0 + e < j.n) { out[e * step] = res.v[e]; if (MUON && p.ema) p.ema[o + e * step] = ema.v[e]; }
+  }
+}
+
 // ---- sum of squares (fp64: the range of fp32 gradients squared) in fixed shares; muon: the momentum is advanced here
 template <typename T, bool MUON>
-__global__ __launch_bounds__(1024) void ns_norm_kernel(NsArgs p, bool split) {
+__global__ __launch_bounds__(1024) void ns_norm_kernel(NsArgs p) {
   constexpr int V = 16 / sizeof(T);
   const NsMat& j = p.j[ns_job(p, blockIdx.x, [](const NsMat& q) { return q.norm0; })];
   const int local = blockIdx.x - j.norm0, z = local / j.nblk, k = local - z * j.nblk;
@@ -147,7 +193,7 @@ __global__ __launch_bounds__(1024) void ns_norm_kernel(NsArgs p, bool split) {
   if (threadIdx.x == 0) {
     double v = 0.0;
     for (int q = 0; q < 16; ++q) v += lds[q];
-    ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np, split).part[k] = v;
+    ((double*)(p.ws + j.ws + z * j.wst))[k] = v;
   }
 }
 
@@ -196,9 +242,7 @@ __global__ __launch_bounds__(256) void ns_convert_kernel(NsArgs p, bool split) {
   s = wave_sum_d(s);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
   __syncthreads();
-  const double norm = sqrt((lds[0] + lds[1]) + (lds[2] + lds[3]));
-  // an infinity or a NaN in the matrix makes every value of it NaN
-  const double inv = norm <= (double)p.eps ? 0.0 : norm < INFINITY ? (double)SX / norm : (double)NAN;
+  const double inv = ns_scale((lds[0] + lds[1]) + (lds[2] + lds[3]), p.eps);
   if (!j.tall) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -460,39 +504,7 @@ __device__ __forceinline__ void ns_write_rows(const f32x4 (*acc)[C::FC], int i0,
         }
       }
       if (PH == PH_LAST) {
-        if (col >= j.m || row0 >= j.n) continue;
-        const int64_t o = j.out + z * j.sto + (j.tall ? (int64_t)row0 * j.ldo + col : (int64_t)col * j.ldo + row0), step = j.tall ? j.ldo : 1;
-        OUT* out = (OUT*)p.out + o;
-        const bool four = !j.tall && row0 + 4 <= j.n;        // four values side by side
-        Pack<OUT, 4> old, res;
-        Pack<float, 4> ema;
-        if (MUON) {
-          if (four) {
-            old = *reinterpret_cast<const Pack<OUT, 4>*>(out);
-            if (p.ema) ema = *reinterpret_cast<const Pack<float, 4>*>(p.ema + o);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (row0 + e < j.n) { old.v[e] = out[e * step]; if (p.ema) ema.v[e] = p.ema[o + e * step]; }
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = v[e] * (1.f / SX);
-          if (MUON) {
-            x = fmaf(-p.lr * j.scale, x, (float)old.v[e] * (1.f - p.lr * p.wd));
-            ema.v[e] = fmaf(p.ema_decay, ema.v[e], (1.f - p.ema_decay) * x);
-          }
-          res.v[e] = (OUT)x;
-        }
-        if (four) {
-          *reinterpret_cast<Pack<OUT, 4>*>(out) = res;
-          if (MUON && p.ema) *reinterpret_cast<Pack<float, 4>*>(p.ema + o) = ema;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (row0 + e < j.n) { out[e * step] = res.v[e]; if (MUON && p.ema) p.ema[o + e * step] = ema.v[e]; }
-        }
+        ns_result<OUT, MUON>(p, j, z, row0, col, v);
         continue;
       }
       if (PH < PH_X && !SPLIT) {
@@ -638,9 +650,12 @@ __global__ __launch_bounds__((Tile<T, SPLIT>::NT)) void ns_join_kernel(NsArgs p,
   ns_write_rows<C, SPLIT, PH, OUT, MUON, 1>(v, i, ad, lds, p, j, w, z, ti, tj, gen, ca, cb, cc);
 }
 
+#include "newton_schulz_thin.h"
+
 // ---- host side
 // launches of a call: workgroups of norm and conversion; per product its tile size, workgroups (whole tiles and shares) and split tiles
-struct NsPlan { int64_t bytes, norm, conv; int T[3]; int64_t grid[3], join[3]; };
+// thin: 0, or the short side that newton_schulz_thin.h holds; blocks: its workgroups; one: a matrix is one block
+struct NsPlan { int64_t bytes, norm, conv; int T[3]; int64_t grid[3], join[3]; int thin; int64_t blocks; bool one; };
 
 inline int64_t up(int64_t v, int64_t k) { return (v + k - 1) / k * k; }
 
@@ -705,6 +720,34 @@ int ns_tiles(NsArgs& p, NsPlan& pl, int q, int64_t& slab) {
   return ITG_OK;
 }
 
+void ns_job_fields(const itg_ns_job& q, NsMat& j) {
+  const int64_t blocks = ((int64_t)j.m * j.n + NORM_ELEMS - 1) / NORM_ELEMS;
+  j.nblk = (int)(blocks < NORM_BLOCKS ? blocks : NORM_BLOCKS);
+  j.scale = sqrtf(fmaxf(1.f, (float)q.rows / (float)q.cols));
+  j.in = q.in_offset; j.ldi = q.in_ld; j.sti = q.in_stride;
+  j.out = q.out_offset; j.ldo = q.out_ld; j.sto = q.out_stride;
+}
+
+// Short sides: every matrix of the call has at most 64 rows or columns, or 128, and its blocks of 128 columns make no more workgroups
+// than a workgroup can add up shares of A in passing: 16 KiB each at 64, 32 of them with up to 4 blocks a workgroup (64 x 8192 fp32:
+// 99 us, general path 129), 64 KiB at 128, 8 of them (128 x 1024: 116 us against 122; 128 x 2048 in 16: 140 against 127).
+bool ns_thin(NsArgs& p, NsPlan& pl) {
+  int m = 0, n = 0;
+  for (int i = 0; i < p.n; ++i) { m = p.j[i].m > m ? p.j[i].m : m; n = p.j[i].n > n ? p.j[i].n : n; }
+  if (m > 128) return false;
+  const int M = m > 64 ? 128 : 64, most = M == 64 ? 32 : 8, turns = M == 64 ? 4 : 1;
+  if (up(n, 128) / 128 > most * turns) return false;
+  pl.thin = M;
+  pl.one = n <= 128;
+  for (int i = 0; i < p.n; ++i) {
+    NsMat& j = p.j[i];
+    const int cols = (int)(up(j.n, 128) / 128);
+    j.subs = (cols + most - 1) / most;
+    j.blocks = (cols + j.subs - 1) / j.subs;
+  }
+  return true;
+}
+
 // fills p.j[] from the jobs; returns a status
 int ns_plan(const itg_ns_job* jobs, int n, bool split, bool muon, NsArgs& p, NsPlan& pl) {
   if (!jobs || n < 1 || n > ITG_NS_MAX_JOBS) return ITG_ERR_ARG;
@@ -724,17 +767,31 @@ int ns_plan(const itg_ns_job* jobs, int n, bool split, bool muon, NsArgs& p, NsP
     j.m = j.tall ? q.cols : q.rows; j.n = j.tall ? q.rows : q.cols;
     j.count = q.count;
   }
+  if (ns_thin(p, pl)) {
+    for (int i = 0; i < n; ++i) {
+      const itg_ns_job& q = jobs[i];
+      NsMat& j = p.j[i];
+      j.mp = pl.thin; j.np = (int)up(j.n, 128);
+      ns_job_fields(q, j);
+      j.norm0 = (int)pl.norm; j.block0 = (int)pl.blocks;
+      pl.norm += (int64_t)j.nblk * j.count;
+      pl.blocks += (int64_t)j.blocks * j.count;
+      if (pl.norm > INT32_MAX || pl.blocks > INT32_MAX) return ITG_ERR_ARG;
+      j.wst = pl.one ? 0 : up(thin_ws_bytes(pl.thin, j.np, j.blocks), 256);
+      j.ws = pl.bytes;
+      if (j.wst > ((int64_t)1 << 60) / j.count) return ITG_ERR_ARG;
+      pl.bytes += j.wst * j.count;
+    }
+    if (pl.one) pl.bytes = 16;
+    return ITG_OK;
+  }
   ns_tile_sizes(p, split, pl);
   const int T = pl.T[2] > pl.T[0] ? pl.T[2] : pl.T[0] > pl.T[1] ? pl.T[0] : pl.T[1];
   for (int i = 0; i < n; ++i) {
     const itg_ns_job& q = jobs[i];
     NsMat& j = p.j[i];
     j.mp = (int)up(j.m, T); j.np = (int)up(j.n, T);
-    const int64_t blocks = ((int64_t)j.m * j.n + NORM_ELEMS - 1) / NORM_ELEMS;
-    j.nblk = (int)(blocks < NORM_BLOCKS ? blocks : NORM_BLOCKS);
-    j.scale = sqrtf(fmaxf(1.f, (float)q.rows / (float)q.cols));
-    j.in = q.in_offset; j.ldi = q.in_ld; j.sti = q.in_stride;
-    j.out = q.out_offset; j.ldo = q.out_ld; j.sto = q.out_stride;
+    ns_job_fields(q, j);
     j.norm0 = (int)pl.norm; j.conv0 = (int)pl.conv;
     pl.norm += (int64_t)j.nblk * j.count;
     pl.conv += (int64_t)(j.mp / 64) * (j.np / 64) * j.count;
@@ -762,8 +819,8 @@ bool ns_coefficients_ok(const float* abc, int steps) {
     const double a = abc[0], b = abc[1], c = abc[2];
     if (!isfinite(a) || !isfinite(b) || !isfinite(c)) return false;
     double next = 0.0;
-    for (int i = 0; i <= 4096; ++i) {
-      const double x = top * i / 4096.0, q = x * x, poly = q * (b + c * q), y = fabs(x * (a + poly));
+    for (int i = 0; i <= 128; ++i) {
+      const double x = top * i / 128.0, q = x * x, poly = q * (b + c * q), y = fabs(x * (a + poly));
       if (!(fabs(poly) <= 60.0) || !(y <= 3.9)) return false;
       if (y > next) next = y;
     }
@@ -772,13 +829,17 @@ bool ns_coefficients_ok(const float* abc, int steps) {
   return true;
 }
 
+template <typename K>
+int ns_lds(K kernel, int bytes) {
+  return bytes <= 64 * 1024 || hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess
+             ? ITG_OK : ITG_ERR_LAUNCH;
+}
+
 template <int T, bool SPLIT, int DEPTH, int PH, typename OUT, bool MUON>
 int ns_launch(const NsArgs& p, const NsPlan& pl, int gen, const float* abc, hipStream_t s) {
   typedef Tile<T, SPLIT> C;
   constexpr int Q3 = PH < PH_X ? PH : 2, LDS = DEPTH * C::BUF * 2;
-  if (LDS > 64 * 1024 &&
-      hipFuncSetAttribute(reinterpret_cast<const void*>(&ns_gemm_kernel<T, SPLIT, DEPTH, PH, OUT, MUON>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
-    return ITG_ERR_LAUNCH;
+  if (ns_lds(&ns_gemm_kernel<T, SPLIT, DEPTH, PH, OUT, MUON>, LDS)) return ITG_ERR_LAUNCH;
   hipLaunchKernelGGL((ns_gemm_kernel<T, SPLIT, DEPTH, PH, OUT, MUON>), dim3((unsigned)pl.grid[Q3]), dim3(C::NT), LDS, s, p, gen, abc[0], abc[1], abc[2]);
   ITG_CHECK_LAUNCH();
   if (pl.join[Q3]) {
@@ -801,10 +862,38 @@ int ns_phase(const NsArgs& p, const NsPlan& pl, int gen, const float* abc, hipSt
   return ns_launch<BIG, SPLIT, 2, PH, OUT, MUON>(p, pl, gen, abc, s);
 }
 
+template <int M, typename T, bool SPLIT, bool MUON>
+int ns_thin_run(const NsArgs& p, const NsPlan& pl, const float* abc, int steps, hipStream_t s) {
+  typedef Thin<M, SPLIT> C;
+  const dim3 grid((unsigned)pl.blocks), nt(C::NT);
+  if (pl.one) {
+    NsSteps st;
+    for (int i = 0; i < 3 * steps; ++i) st.abc[i] = abc[i];
+    st.n = steps;
+    if (ns_lds(&ns_thin_all_kernel<M, SPLIT, T, MUON>, C::LDS)) return ITG_ERR_LAUNCH;
+    hipLaunchKernelGGL((ns_thin_all_kernel<M, SPLIT, T, MUON>), grid, nt, C::LDS, s, p, st);
+    ITG_CHECK_LAUNCH();
+    return ITG_OK;
+  }
+  if (ns_lds(&ns_thin_first_kernel<M, SPLIT, T, MUON>, C::LDS) || ns_lds(&ns_thin_step_kernel<M, SPLIT, false, T, MUON>, C::LDS) ||
+      ns_lds(&ns_thin_step_kernel<M, SPLIT, true, T, MUON>, C::LDS)) return ITG_ERR_LAUNCH;
+  hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)pl.norm), dim3(1024), 0, s, p);
+  ITG_CHECK_LAUNCH();
+  hipLaunchKernelGGL((ns_thin_first_kernel<M, SPLIT, T, MUON>), grid, nt, C::LDS, s, p);
+  ITG_CHECK_LAUNCH();
+  for (int k = 0; k < steps; ++k, abc += 3) {
+    if (k + 1 < steps) hipLaunchKernelGGL((ns_thin_step_kernel<M, SPLIT, false, T, MUON>), grid, nt, C::LDS, s, p, k & 1, abc[0], abc[1], abc[2]);
+    else hipLaunchKernelGGL((ns_thin_step_kernel<M, SPLIT, true, T, MUON>), grid, nt, C::LDS, s, p, k & 1, abc[0], abc[1], abc[2]);
+    ITG_CHECK_LAUNCH();
+  }
+  return ITG_OK;
+}
+
 template <typename T, bool SPLIT, bool MUON>
 int ns_run(NsArgs& p, const NsPlan& pl, const float* abc, int steps, hipStream_t s) {
+  if (pl.thin) return pl.thin == 64 ? ns_thin_run<64, T, SPLIT, MUON>(p, pl, abc, steps, s) : ns_thin_run<128, T, SPLIT, MUON>(p, pl, abc, steps, s);
   p.slab = (float*)(p.ws + (int64_t)p.slab);
-  hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)pl.norm), dim3(1024), 0, s, p, SPLIT);
+  hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)pl.norm), dim3(1024), 0, s, p);
   ITG_CHECK_LAUNCH();
   hipLaunchKernelGGL((ns_convert_kernel<T, MUON>), dim3((unsigned)pl.conv), dim3(256), 0, s, p, SPLIT);
   ITG_CHECK_LAUNCH();

@@ -1726,10 +1726,13 @@ def adam_ema_step(p, g, m, v, ema, lr, beta1, beta2, eps, step, ema_decay=0.999,
 
 # ------------------------------------------------------------------------------- orthogonalised updates
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_NS_FIVE = (C.c_float * 15)(*(NS_COEFFICIENTS * 5))
 
 
 def _ns_coefficients(coefficients, steps):
     """(ctypes array of 3 * steps floats, steps) of one (a, b, c) for every step or of one triple per step."""
+    if coefficients is NS_COEFFICIENTS and steps == 5:
+        return _NS_FIVE, 5
     co = list(coefficients)
     if len(co) == 3 and not isinstance(co[0], (tuple, list)):
         co = [tuple(co)] * int(steps)
