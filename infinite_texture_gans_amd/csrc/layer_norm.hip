@@ -61,6 +61,24 @@ __device__ __forceinline__ void ln_store(T* q, const float (&f)[V]) {
   *reinterpret_cast<Pack<T, V>*>(q) = u;
 }
 
+// V values of gamma or beta, `none` without one.  A vector of a padded row that ends in the padding (hi < V) is read value by value.
+template <typename W, int V, bool ANY>
+__device__ __forceinline__ void ln_param(const void* q, int off, int hi, float none, float (&f)[V]) {
+  Pack<W, V> u = {};
+  const W* at = (const W*)q + off;
+  if (q && hi > 0) {
+    if (!ANY || hi == V) {
+      u = *reinterpret_cast<const Pack<W, V>*>(at);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < hi) u.v[e] = at[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) f[e] = q ? (float)u.v[e] : none;
+}
+
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
 }
@@ -106,12 +124,6 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
     off[r] = i < lv.nv - 1 ? i * V : lv.off_last;
     lo[r] = i < lv.nv - 1 ? 0 : lv.lo_last;
     hi[r] = i < lv.nv - 1 ? V : i < lv.nv ? lv.hi_last : 0;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const bool in = e < hi[r];
-      w[r][e] = in && p.w ? (float)((const W*)p.w)[off[r] + e] : 1.f;
-      b[r][e] = in && p.b ? (float)((const W*)p.b)[off[r] + e] : 0.f;
-    }
   }
   const float inv = 1.f / (float)p.c;
   int flip = 0;
@@ -119,6 +131,8 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
   int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / TPR;
   Pack<T, V> u[R] = {};
   if (row < p.rows) ln_fetch<T, V, R>((const T*)p.x + row * p.ldx, off, hi, u);
+#pragma unroll
+  for (int r = 0; r < R; ++r) { ln_param<W, V, ANY>(p.w, off[r], hi[r], 1.f, w[r]); ln_param<W, V, ANY>(p.b, off[r], hi[r], 0.f, b[r]); }
   for (; row < p.rows; row += step, flip ^= 2) {
     float f[R][V], s = 0.f;
 #pragma unroll
@@ -175,13 +189,10 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
     off[r] = i < lv.nv - 1 ? i * V : lv.off_last;
     lo[r] = i < lv.nv - 1 ? 0 : lv.lo_last;
     hi[r] = i < lv.nv - 1 ? V : i < lv.nv ? lv.hi_last : 0;
+    ln_param<W, V, ANY>(p.w, off[r], hi[r], 1.f, w[r]);
+    ln_param<W, V, ANY>(ANY && p.act ? p.b : nullptr, off[r], hi[r], 0.f, b[r]);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const bool in = e < hi[r];
-      w[r][e] = in && p.w ? (float)((const W*)p.w)[off[r] + e] : 1.f;
-      b[r][e] = ANY && in && p.b && p.act ? (float)((const W*)p.b)[off[r] + e] : 0.f;
-      aw[r][e] = ab[r][e] = 0.f;
-    }
+    for (int e = 0; e < V; ++e) aw[r][e] = ab[r][e] = 0.f;
   }
   const float inv = 1.f / (float)p.c;
   int flip = 0;

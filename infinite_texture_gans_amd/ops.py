@@ -1168,6 +1168,8 @@ def _on(t):
 
 def _row_stride(t):
     """Elements between two rows of ``t`` seen as (rows, t.shape[-1]), or None where it has no single row stride."""
+    if t.is_contiguous():
+        return t.shape[-1]
     if t.dim() == 1 or t.numel() == t.shape[-1]:
         return t.shape[-1] if t.shape[-1] == 1 or t.stride(-1) == 1 else None
     if t.shape[-1] != 1 and t.stride(-1) != 1:
@@ -1185,30 +1187,36 @@ def _rows(t):
     return (t, ld) if ld is not None else (t.contiguous(), t.shape[-1])
 
 
+def _ln_forward(x, ldx, gamma, beta, c, eps, act, slope, stats):
+    """-> (y, mean and 1 / deviation of every row or None, ITG_* type of x, of gamma and beta); x's rows at a stride of ``ldx``."""
+    dt = _DTYPES[x.dtype]
+    p = gamma if gamma is not None else beta
+    pdt = _DTYPES[p.dtype] if p is not None else dt
+    width = x.shape[-1]
+    rows = x.numel() // width
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    stat = torch.empty(2 * rows, device=x.device, dtype=torch.float32) if stats else None
+    if rows:
+        with _on(x):
+            _lib.call("itg_layer_norm_fwd", _ptr(x), ldx, _ptr(gamma), _ptr(beta), _ptr(y), width, _ptr(stat), rows, c, width - c,
+                      dt, pdt, eps, act, slope, _stream())
+    if act == ACT_LRELU and dt == _lib.DT_F32:
+        _sink_act(y, c, act, "ln")
+    return y, stat, dt, pdt
+
+
 class _LayerNorm(torch.autograd.Function):
     """y = act(gamma * xhat + beta), xhat = the row's values normalised with their own mean and variance; ``c`` of the
     x.shape[-1] values of a row are channels, the rest (patch-grid padding) is written as zeros."""
 
     @staticmethod
     def forward(ctx, x, gamma, beta, c, eps, act, slope, sinks):
-        dt = _DTYPES[x.dtype]
-        pdt = _DTYPES[gamma.dtype if gamma is not None else beta.dtype] if gamma is not None or beta is not None else dt
         x, ldx = _rows(x)
-        width = x.shape[-1]
-        rows = x.numel() // width
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        grads = any(ctx.needs_input_grad[:3])
-        stat = torch.empty(2 * rows, device=x.device, dtype=torch.float32) if grads else None
-        if rows:
-            with _on(x):
-                _lib.call("itg_layer_norm_fwd", _ptr(x), ldx, _ptr(gamma), _ptr(beta), _ptr(y), width, _ptr(stat), rows, c, width - c,
-                          dt, pdt, eps, act, slope, _stream())
-        if grads:
+        y, stat, dt, pdt = _ln_forward(x, ldx, gamma, beta, c, eps, act, slope, any(ctx.needs_input_grad[:3]))
+        if stat is not None:
             ctx.meta = (c, dt, pdt, act, slope)
             ctx.sinks = sinks
             ctx.save_for_backward(x, gamma, beta, stat)
-        if act == ACT_LRELU and dt == _lib.DT_F32:
-            _sink_act(y, c, act, "ln")
         return y
 
     @staticmethod
@@ -1255,22 +1263,21 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, slope=0.0, sink
         raise _lib.ItgError("layer_norm: x must be a float32, bfloat16 or float16 tensor on the GPU, got %s on %s" % (t.dtype, t.device))
     if c < 1 or c > _lib.LN_MAX_C:
         raise _lib.ItgError("layer_norm: %d channels (1 .. %d are supported)" % (c, _lib.LN_MAX_C))
-    types = set()
     for name, v in (("gamma", gamma), ("beta", beta)):
-        if v is None:
-            continue
-        if tuple(v.shape) != (c,) or v.device != t.device or not v.is_contiguous() or v.dtype not in (torch.float32, t.dtype):
+        if v is not None and (v.shape != (c,) or v.device != t.device or not v.is_contiguous() or (v.dtype != torch.float32 and v.dtype != t.dtype)):
             raise _lib.ItgError("layer_norm: %s must be %d contiguous values on x's device, float32 or x's type, got %s %s"
                                 % (name, c, tuple(v.shape), v.dtype))
-        types.add(v.dtype)
-    if len(types) > 1:
+    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
         raise _lib.ItgError("layer_norm: gamma and beta must be of one type")
     if act not in (ACT_NONE, ACT_LRELU, ACT_TANH) or not eps >= 0.0:
         raise _lib.ItgError("layer_norm: unknown activation %r or negative eps %r" % (act, eps))
     if sinks is not None and (gamma is None or beta is None or any(s is None or s.dtype != gamma.dtype or tuple(s.shape) != (c,)
                                                                    or not s.is_contiguous() or s.device != t.device for s in sinks)):
         raise _lib.ItgError("layer_norm: sinks are two contiguous buffers like gamma and beta")
-    y = _LayerNorm.apply(t, gamma, beta, c, float(eps), int(act), float(slope), sinks)
+    if torch.is_grad_enabled() and (t.requires_grad or (gamma is not None and gamma.requires_grad) or (beta is not None and beta.requires_grad)):
+        y = _LayerNorm.apply(t, gamma, beta, c, float(eps), int(act), float(slope), sinks)
+    else:      # no tape: a quarter of the host's time for a call
+        y = _ln_forward(*_rows(t), gamma, beta, c, float(eps), int(act), float(slope), False)[0]
     return GT(y, c) if grid else y
 
 
