@@ -1161,9 +1161,12 @@ def ssm_modulate(x, emb, rm, rv, nbt, training=True, eps=1e-5, momentum=0.1, act
 _DTYPES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 
 
+_HERE = _NullCtx()
+
+
 def _on(t):
     """Launch on ``t``'s device: a device guard where it is not the current one."""
-    return _NullCtx() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _row_stride(t):
@@ -1198,8 +1201,9 @@ def _ln_forward(x, ldx, gamma, beta, c, eps, act, slope, stats):
     stat = torch.empty(2 * rows, device=x.device, dtype=torch.float32) if stats else None
     if rows:
         with _on(x):
-            _lib.call("itg_layer_norm_fwd", _ptr(x), ldx, _ptr(gamma), _ptr(beta), _ptr(y), width, _ptr(stat), rows, c, width - c,
-                      dt, pdt, eps, act, slope, _stream())
+            _lib.call("itg_layer_norm_fwd", x.data_ptr(), ldx, gamma.data_ptr() if gamma is not None else None,
+                      beta.data_ptr() if beta is not None else None, y.data_ptr(), width, stat.data_ptr() if stats else None, rows, c,
+                      width - c, dt, pdt, eps, act, slope, _stream())
     if act == ACT_LRELU and dt == _lib.DT_F32:
         _sink_act(y, c, act, "ln")
     return y, stat, dt, pdt
@@ -1212,39 +1216,38 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, c, eps, act, slope, sinks):
         x, ldx = _rows(x)
-        y, stat, dt, pdt = _ln_forward(x, ldx, gamma, beta, c, eps, act, slope, any(ctx.needs_input_grad[:3]))
-        if stat is not None:
-            ctx.meta = (c, dt, pdt, act, slope)
-            ctx.sinks = sinks
-            ctx.save_for_backward(x, gamma, beta, stat)
+        y, stat, dt, pdt = _ln_forward(x, ldx, gamma, beta, c, eps, act, slope, True)
+        ctx.meta = (c, x.shape[-1], ldx, dt, pdt, act, slope, sinks)
+        ctx.save_for_backward(x, gamma, beta, stat)
         return y
 
+    # (the engine runs this on a thread of its own, where Python is twice as slow: addresses go to the library as they are)
     @staticmethod
     def backward(ctx, dy):
         x, gamma, beta, stat = ctx.saved_tensors
-        c, dt, pdt, act, slope = ctx.meta
-        need = ctx.needs_input_grad
-        x, ldx = _rows(x)
+        c, width, ldx, dt, pdt, act, slope, sinks = ctx.meta
+        need_x, need_g, need_b = ctx.needs_input_grad[:3]
         dy, ldy = _rows(dy)
-        width = x.shape[-1]
-        rows = x.numel() // width
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
-        acc = 0
-        dg = db = None
-        if ctx.sinks is not None and (need[1] or need[2]):
-            (dg, db), acc = ctx.sinks, ACC_DW
+        rows = stat.numel() // 2
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
+        acc, dg, db = 0, None, None
+        if sinks is not None and (need_g or need_b):
+            (dg, db), acc = sinks, ACC_DW
         else:
-            dg = torch.empty_like(gamma) if need[1] else None
-            db = torch.empty_like(beta) if need[2] else None
+            dg = torch.empty_like(gamma) if need_g else None
+            db = torch.empty_like(beta) if need_b else None
         if rows:
-            n = _lib.fn("itg_layer_norm_bwd_workspace")(rows, c) if dg is not None or db is not None else 0
-            ws = torch.empty(n, device=x.device, dtype=torch.float32) if n else None
+            n, ws = 0, None
+            if dg is not None or db is not None:
+                n = _lib.fn("itg_layer_norm_bwd_workspace")(rows, c)
+                ws = torch.empty(n, device=x.device, dtype=torch.float32)
+            at = [t.data_ptr() if t is not None else None for t in (x, dy, stat, gamma, beta, dx, dg, db, ws)]
             with _on(x):
-                _lib.call("itg_layer_norm_bwd", _ptr(x), ldx, _ptr(dy), ldy, _ptr(stat), _ptr(gamma), _ptr(beta), _ptr(dx), width,
-                          _ptr(dg), _ptr(db), acc, rows, c, width - c, dt, pdt, act, slope, _ptr(ws), n, _stream())
+                _lib.call("itg_layer_norm_bwd", at[0], ldx, at[1], ldy, at[2], at[3], at[4], at[5], width, at[6], at[7], acc, rows, c,
+                          width - c, dt, pdt, act, slope, at[8], n, _stream())
         elif not acc:
             dg, db = (t.zero_() if t is not None else None for t in (dg, db))
-        return (dx, None, None) + (None,) * 5 if acc else (dx, dg, db) + (None,) * 5
+        return (dx, None, None, None, None, None, None, None) if acc else (dx, dg, db, None, None, None, None, None)
 
 
 def layer_norm(x, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, slope=0.0, sinks=None):
