@@ -364,46 +364,76 @@ __device__ __forceinline__ void ns_product(Acc<C>& acc, const _Float16* const* P
   Acc<C>& run = SPLIT ? part : acc;
   const int nk = (k1 - k0) / BK;
   constexpr int LOADS = 2 * NP * C::LP;                    // of a wave per buffer
-#pragma unroll
-  for (int b = 0; b < DEPTH - 1; ++b) stage(b, k0 + (b < nk ? b : nk - 1) * BK);
-  int buf = 0, into = DEPTH - 1;
-  for (int kk = 0; kk < nk; ++kk) {
-    // buffer kk has arrived: this wave's loads by its own count (those of the DEPTH - 2 buffers behind it may be in flight), the
-    // other waves' by the barrier, which also tells that buffer kk - 1 has been read and may be filled again
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((DEPTH - 2) * LOADS) : "memory");
-    const int next = kk + DEPTH - 1;
-    stage(into, k0 + (next < nk ? next : nk - 1) * BK);    // past the end: the last slice again, so that the count stays
+  struct Frags { f16x8 p[NP][C::FR], q[NP][C::FC]; };
+  auto read = [&](int buf, int ks, Frags& f) {
     const _Float16* at = lds + buf * C::BUF;
 #pragma unroll
-    for (int ks = 0; ks < BK / 32; ++ks) {
-      f16x8 fp[NP][C::FR], fq[NP][C::FC];
-#pragma unroll
-      for (int q = 0; q < NP; ++q) {
-#pragma unroll
-        for (int i = 0; i < C::FR; ++i)
-          fp[q][i] = TURN ? frag_t<T>(at + q * C::PLANE + at_p[i] + ks * 32 * T) : *reinterpret_cast<const f16x8*>(at + q * C::PLANE + at_p[i] + ch[ks]);
-#pragma unroll
-        for (int k = 0; k < C::FC; ++k) fq[q][k] = *reinterpret_cast<const f16x8*>(at + (NP + q) * C::PLANE + row_q + ch[ks] + k * 16 * BK);
-      }
+    for (int q = 0; q < NP; ++q) {
 #pragma unroll
       for (int i = 0; i < C::FR; ++i)
+        f.p[q][i] = TURN ? frag_t<T>(at + q * C::PLANE + at_p[i] + ks * 32 * T) : *reinterpret_cast<const f16x8*>(at + q * C::PLANE + at_p[i] + ch[ks]);
 #pragma unroll
-        for (int k = 0; k < C::FC; ++k) {
-          if (SPLIT) {
-            run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[NP - 1][i], fq[0][k], run.v[i][k], 0, 0, 0);
-            run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][i], fq[NP - 1][k], run.v[i][k], 0, 0, 0);
-          }
-          run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][i], fq[0][k], run.v[i][k], 0, 0, 0);
+      for (int k = 0; k < C::FC; ++k) f.q[q][k] = *reinterpret_cast<const f16x8*>(at + (NP + q) * C::PLANE + row_q + ch[ks] + k * 16 * BK);
+    }
+  };
+  auto multiply = [&](const Frags& f) {
+#pragma unroll
+    for (int i = 0; i < C::FR; ++i)
+#pragma unroll
+      for (int k = 0; k < C::FC; ++k) {
+        if (SPLIT) {
+          run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[NP - 1][i], f.q[0][k], run.v[i][k], 0, 0, 0);
+          run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[0][i], f.q[NP - 1][k], run.v[i][k], 0, 0, 0);
         }
-    }
-    if (SPLIT && ((kk + 1) % FLUSH == 0 || kk + 1 == nk)) {
+        run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[0][i], f.q[0][k], run.v[i][k], 0, 0, 0);
+      }
+  };
+  auto flush = [&](int kk) {
+    if (!SPLIT || ((kk + 1) % FLUSH != 0 && kk + 1 != nk)) return;
 #pragma unroll
-      for (int i = 0; i < C::FR; ++i)
+    for (int i = 0; i < C::FR; ++i)
 #pragma unroll
-        for (int k = 0; k < C::FC; ++k) { acc.v[i][k] += part.v[i][k]; part.v[i][k] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+      for (int k = 0; k < C::FC; ++k) { acc.v[i][k] += part.v[i][k]; part.v[i][k] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+  };
+  auto slice = [&](int k) { return k0 + (k < nk ? k : nk - 1) * BK; };      // past the end: the last slice again, so that the counts stay
+  // A buffer has arrived when this wave's loads have (its own count: those of the buffers behind it may be in flight) and, by the
+  // barrier, the other waves'.  The barrier also tells that the buffer before has been read and may be filled again.
+  if (DEPTH == 4) {
+    // few workgroups: nothing else hides the LDS reads, so a slice is read while the one before is multiplied
+    constexpr int KS = BK / 32;
+    Frags f[2][KS];
+    auto all = [&](int buf, Frags (&g)[KS]) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) read(buf, ks, g[ks]);
+    };
+#pragma unroll
+    for (int b = 0; b < DEPTH; ++b) stage(b, slice(b));
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((DEPTH - 1) * LOADS) : "memory");
+    all(0, f[0]);
+    auto turn = [&](int kk, Frags (&now)[KS], Frags (&next)[KS]) {
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((DEPTH - 2) * LOADS) : "memory");
+      stage(kk & 3, slice(kk + DEPTH));
+      all((kk + 1) & 3, next);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) multiply(now[ks]);
+      flush(kk);
+    };
+    int kk = 0;
+    for (; kk + 1 < nk; kk += 2) { turn(kk, f[0], f[1]); turn(kk + 1, f[1], f[0]); }
+    if (kk < nk) turn(kk, f[0], f[1]);
+  } else {
+#pragma unroll
+    for (int b = 0; b < DEPTH - 1; ++b) stage(b, slice(b));
+    int buf = 0, into = DEPTH - 1;
+    for (int kk = 0; kk < nk; ++kk) {
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((DEPTH - 2) * LOADS) : "memory");
+      stage(into, slice(kk + DEPTH - 1));
+#pragma unroll
+      for (int ks = 0; ks < BK / 32; ++ks) { Frags f; read(buf, ks, f); multiply(f); }
+      flush(kk);
+      buf = buf + 1 == DEPTH ? 0 : buf + 1;
+      into = into + 1 == DEPTH ? 0 : into + 1;
     }
-    buf = buf + 1 == DEPTH ? 0 : buf + 1;
-    into = into + 1 == DEPTH ? 0 : into + 1;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // no load into LDS outlives the workgroup
 }
