@@ -376,17 +376,15 @@ __device__ __forceinline__ void ns_product(Acc<C>& acc, const _Float16* const* P
       for (int k = 0; k < C::FC; ++k) f.q[q][k] = *reinterpret_cast<const f16x8*>(at + (NP + q) * C::PLANE + row_q + ch[ks] + k * 16 * BK);
     }
   };
+  // lo hi, hi lo, hi hi: each over all fragments, so that no product waits for the one before it
   auto multiply = [&](const Frags& f) {
 #pragma unroll
-    for (int i = 0; i < C::FR; ++i)
+    for (int q = SPLIT ? 0 : 2; q < 3; ++q)
 #pragma unroll
-      for (int k = 0; k < C::FC; ++k) {
-        if (SPLIT) {
-          run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[NP - 1][i], f.q[0][k], run.v[i][k], 0, 0, 0);
-          run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[0][i], f.q[NP - 1][k], run.v[i][k], 0, 0, 0);
-        }
-        run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[0][i], f.q[0][k], run.v[i][k], 0, 0, 0);
-      }
+      for (int i = 0; i < C::FR; ++i)
+#pragma unroll
+        for (int k = 0; k < C::FC; ++k)
+          run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[q == 0 ? NP - 1 : 0][i], f.q[q == 1 ? NP - 1 : 0][k], run.v[i][k], 0, 0, 0);
   };
   auto flush = [&](int kk) {
     if (!SPLIT || ((kk + 1) % FLUSH != 0 && kk + 1 != nk)) return;
@@ -694,20 +692,24 @@ inline int64_t up(int64_t v, int64_t k) { return (v + k - 1) / k * k; }
 //   only: split has no registers for it) from a full round of 256 tiles on (4096 x 8192 bf16: 3207 -> 3056 us).
 // A and B, whose leftover tiles are split along K, go by tiles x K: split 128 from 192 K on (1024 x 8192, A 288 K: 712 -> 673 us;
 //   4 x 1024 x 1024, 144 K: 634 -> 642), single from 400 K on (1536 x 6144, A 468 K: 626 -> 598 us; 1024 x 8192, 288 K: 406 -> 413).
+// A size whose padding adds more than an eighth to the planes is not taken (the default generator's matrices of 3 to 416 rows: 448 us
+// a Muon step with X at 128, 430 without).
 void ns_tile_sizes(const NsArgs& p, bool split, NsPlan& pl) {
-  int64_t a = 0, b = 0, x = 0, x256 = 0;
+  int64_t a = 0, b = 0, x = 0, x64 = 0, x256 = 0;
   for (int i = 0; i < p.n; ++i) {
     const NsMat& j = p.j[i];
     const int64_t m = up(j.m, 128) / 128, n = up(j.n, 128) / 128, sym = m * (m + 1) / 2 * j.count;
     a += sym * n * 128;
     b += sym * m * 128;
     x += m * n * j.count;
+    x64 += up(j.m, 64) / 64 * (up(j.n, 64) / 64) * j.count;
     x256 += ((m + 1) / 2) * ((n + 1) / 2) * j.count;
   }
   const int64_t least = (split ? 192 : 400) * 1024;
-  pl.T[0] = a >= least ? 128 : 64;
-  pl.T[1] = b >= least ? 128 : 64;
-  pl.T[2] = !split && x256 >= 256 ? 256 : x >= 384 ? 128 : 64;
+  const bool fits = 32 * x <= 9 * x64, fits256 = 128 * x256 <= 9 * x64;
+  pl.T[0] = fits && a >= least ? 128 : 64;
+  pl.T[1] = fits && b >= least ? 128 : 64;
+  pl.T[2] = !split && fits256 && x256 >= 256 ? 256 : fits && x >= 384 ? 128 : 64;
 }
 
 // Tiles and shares of product q (A, B, X).  `slots` workgroups run at a time; whole rounds of them take a tile each, and what is

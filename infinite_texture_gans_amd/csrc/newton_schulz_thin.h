@@ -97,15 +97,11 @@ template <bool SPLIT, int R, int N>
 __device__ __forceinline__ void thin_mfma(f32x4 (&acc)[R][N], const f16x8 (&P)[SPLIT ? 2 : 1][R], const f16x8 (&Q)[SPLIT ? 2 : 1][N]) {
   constexpr int L = SPLIT ? 1 : 0;
 #pragma unroll
-  for (int i = 0; i < R; ++i)
+  for (int q = SPLIT ? 0 : 2; q < 3; ++q)
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      if (SPLIT) {
-        acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[L][i], Q[0][k], acc[i][k], 0, 0, 0);
-        acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[0][i], Q[L][k], acc[i][k], 0, 0, 0);
-      }
-      acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[0][i], Q[0][k], acc[i][k], 0, 0, 0);
-    }
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[q == 0 ? L : 0][i], Q[q == 1 ? L : 0][k], acc[i][k], 0, 0, 0);
 }
 
 // this wave's part of S S^T over `slices` x 32 of the planes' columns (pitch PITCH), added to acc
