@@ -425,8 +425,9 @@ int itg_adam_ema_step(float* p, const float* g, float* m, float* v, float* ema, 
  * Rows of c values at a stride of ld* elements (any stride >= c; any alignment the element type allows):
  *   y = act(gamma (x - mean) / sqrt(var + eps) + beta)     mean, var: of the row's c values, fp32 for every type
  * gamma / beta: c values or NULL (1 / 0).  pad > 0: the rows of every tensor hold c + pad values (a patch-grid tensor: pad =
- * ld - c), of which the last pad are ignored in x and dy and written as zeros in y and dx.  dtype: ITG_F32 | ITG_BF16 | ITG_F16 of x, y, dy, dx; param_dtype: of gamma, beta and their gradients,
- * ITG_F32 or dtype.  mean_rstd: [rows][2] floats for the backward pass, or NULL.  y may be x (dx may be dy or x).
+ * ld - c), of which the last pad are ignored in x and dy (whatever they hold) and written as zeros in y and dx.  dtype:
+ * ITG_F32 | ITG_BF16 | ITG_F16 of x, y, dy, dx; param_dtype: of gamma, beta and their gradients, ITG_F32 or dtype.  mean_rstd: [rows][2] floats for the backward pass, or NULL.  y may be x (dx may be dy or x)
+ * at the same stride; otherwise outputs overlap nothing.
  * bwd: dx, dgamma, dbeta may each be NULL; accumulate: ITG_ACC_DW adds into dgamma / dbeta.  workspace:
  * itg_layer_norm_bwd_workspace(rows, c) floats (shares of dgamma | dbeta, added in a fixed order), needed with dgamma / dbeta.  */
 enum { ITG_F32 = 0, ITG_BF16 = 1, ITG_F16 = 2 };

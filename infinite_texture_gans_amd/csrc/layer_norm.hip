@@ -152,7 +152,8 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         f[r][e] -= mean;
-        q = fmaf(f[r][e], !ANY || (e >= lo[r] && e < hi[r]) ? f[r][e] : 0.f, q);
+        const float d = !ANY || (e >= lo[r] && e < hi[r]) ? f[r][e] : 0.f;      // (padding may hold anything, a NaN too)
+        q = fmaf(d, d, q);
       }
       s += hi[r] > 0 ? q : 0.f;
     }
@@ -215,13 +216,10 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
       for (int e = 0; e < V; ++e) {      // a vector past the row's end holds zeros in dy
         const bool in = !ANY || (e >= lo[r] && e < hi[r]);
         const float h = in ? ((float)ux[r].v[e] - mean) * rs : 0.f;
-        float du = in ? (float)ug[r].v[e] : 0.f;
         xh[r][e] = ANY ? ((float)ux[r].v[e] - mean) * rs : h;
-        float all = ANY ? (float)ug[r].v[e] : du;
-        if (ANY && p.act) {
-          const float sl = act_slope_at(fmaf(xh[r][e], w[r][e], b[r][e]), p.act, p.slope);
-          all *= sl; du *= sl;
-        }
+        float all = (float)ug[r].v[e];
+        if (ANY && p.act) all *= act_slope_at(fmaf(xh[r][e], w[r][e], b[r][e]), p.act, p.slope);
+        const float du = in ? all : 0.f;
         aw[r][e] = fmaf(du, h, aw[r][e]);
         ab[r][e] += du;
         g[r][e] = all * w[r][e];
@@ -519,10 +517,7 @@ int ln_bwd_t(LnP p, void* dw, void* db, int acc, hipStream_t s) {
   else if (nv <= 512 * K) rc = ln_bwd_run<T, W, V, 512, K>(p, chunks, s);
   else if (nv <= 1024 * K) rc = ln_bwd_run<T, W, V, 1024, K>(p, chunks, s);
   else {
-    if (p.y) {
-      hipLaunchKernelGGL((ln_dx_any_kernel<T, W, V>), dim3(ln_grid(p.rows)), dim3(LN_ANY), 0, s, p);
-      ITG_CHECK_LAUNCH();
-    }
+    // (the shares read every row of dy and x, and dx may be written over either)
     if (shares) {
       // about 2048 workgroups in all, and no share of fewer than 8 rows
       const int cols = (nv + 255) / 256;
@@ -530,6 +525,10 @@ int ln_bwd_t(LnP p, void* dw, void* db, int acc, hipStream_t s) {
       const int64_t chunk = (p.rows + k - 1) / k;
       chunks = (int)((p.rows + chunk - 1) / chunk);
       hipLaunchKernelGGL((ln_dw_any_kernel<T, W, V>), dim3(cols, chunks), dim3(256), 0, s, p, chunk);
+      ITG_CHECK_LAUNCH();
+    }
+    if (p.y) {
+      hipLaunchKernelGGL((ln_dx_any_kernel<T, W, V>), dim3(ln_grid(p.rows)), dim3(LN_ANY), 0, s, p);
       ITG_CHECK_LAUNCH();
     }
   }
@@ -569,7 +568,7 @@ int itg_layer_norm_fwd(const void* x, int64_t ldx, const void* gamma, const void
                        int64_t rows, int c, int pad, int dtype, int param_dtype, float eps, int act, float slope, void* stream) {
   int rc;
   if ((rc = ln_check(rows, c, pad, ldx, dtype, param_dtype, act)) || (rc = ln_check(rows, c, pad, ldy, dtype, param_dtype, act))) return rc;
-  if (!x || !y || !(eps >= 0.f)) return ITG_ERR_ARG;
+  if (!x || !y || !(eps >= 0.f) || (rows > 1 && y == x && ldy != ldx)) return ITG_ERR_ARG;
   if (misaligned(x, dtype) || misaligned(y, dtype) || misaligned(gamma, param_dtype) || misaligned(beta, param_dtype) ||
       misaligned(mean_rstd, ITG_F32)) return ITG_ERR_ALIGN;
   LnP p{};
@@ -592,6 +591,7 @@ int itg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy,
   if ((rc = ln_check(rows, c, pad, ldx, dtype, param_dtype, act)) || (rc = ln_check(rows, c, pad, lddy, dtype, param_dtype, act)) ||
       (dx && (rc = ln_check(rows, c, pad, lddx, dtype, param_dtype, act)))) return rc;
   if (!x || !dy || !mean_rstd) return ITG_ERR_ARG;
+  if (rows > 1 && ((dx == x && lddx != ldx) || (dx == dy && lddx != lddy))) return ITG_ERR_ARG;
   if (misaligned(x, dtype) || misaligned(dy, dtype) || misaligned(dx, dtype) || misaligned(gamma, param_dtype) ||
       misaligned(beta, param_dtype) || misaligned(dgamma, param_dtype) || misaligned(dbeta, param_dtype) ||
       misaligned(mean_rstd, ITG_F32) || misaligned(workspace, ITG_F32)) return ITG_ERR_ALIGN;

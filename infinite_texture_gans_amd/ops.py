@@ -1224,6 +1224,8 @@ class _LayerNorm(torch.autograd.Function):
     # (the engine runs this on a thread of its own, where Python is twice as slow: addresses go to the library as they are)
     @staticmethod
     def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            raise _lib.ItgError("layer_norm: no second derivatives (create_graph=True)")
         x, gamma, beta, stat = ctx.saved_tensors
         c, width, ldx, dt, pdt, act, slope, sinks = ctx.meta
         need_x, need_g, need_b = ctx.needs_input_grad[:3]
@@ -1232,7 +1234,7 @@ class _LayerNorm(torch.autograd.Function):
         dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
         acc, dg, db = 0, None, None
         if sinks is not None and (need_g or need_b):
-            (dg, db), acc = sinks, ACC_DW
+            dg, db, acc = sinks[0] if need_g else None, sinks[1] if need_b else None, ACC_DW
         else:
             dg = torch.empty_like(gamma) if need_g else None
             db = torch.empty_like(beta) if need_b else None
@@ -1257,7 +1259,8 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, slope=0.0, sink
     ``gamma`` / ``beta``: one value per channel, contiguous, float32 or x's type, both alike; None = 1 / 0.  Statistics and sums are
     fp32.  No running statistics: training and evaluation are the same function.  ``sinks`` = (gamma.grad, beta.grad) buffers
     the backward accumulates into.  The activation's derivative at 0 is that of its negative side.  A NaN or an infinity in a
-    row makes that row NaN."""
+    row makes that row NaN.  No second derivatives.  A backward pass is captured into a graph only while no eager graph of the
+    same leaves lives (torch's rule for every function of its tape)."""
     grid = isinstance(x, GT)
     t, c = (x.t, x.c) if grid else (x, x.shape[-1] if x.dim() else 0)
     if grid:

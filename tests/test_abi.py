@@ -164,6 +164,7 @@ def test_training_operators_reject_bad_calls_on_the_host(lib):
     def bwd(stat=q, dx=q, dg=q, ws=q, n=1 << 20, rows=4, c=8, lddx=8):
         return so.itg_layer_norm_bwd(q, 8, q, 8, stat, None, None, dx, lddx, dg, None, 0, rows, c, 0, 0, 0, 0, f(0.0), ws, n, None)
 
+    assert fwd(ldx=9) == -1 and bwd(lddx=9) == -1           # in place at two strides
     assert bwd(stat=None) == -1 and bwd(ws=None) == -4 and bwd(n=7) == -4 and bwd(lddx=4) == -1 and bwd(ws=p(4097)) == -2
     assert bwd(dx=None, dg=None) == 0                       # nothing asked for: nothing launched
 
@@ -185,7 +186,9 @@ def test_training_operators_reject_bad_calls_on_the_host(lib):
 
     assert ns(g=None) == -1 and ns(out=None) == -1 and ns(steps=0) == -1 and ns(steps=17) == -1 and ns(co=None) == -1 and ns(eps=-1.0) == -1
     assert ns(co=(f * 3)(9.0, 0.0, 0.0)) == -1 and ns(co=(f * 3)(float("inf"), 0.0, 0.0)) == -1
-    assert ns(ws=None) == -4 and ns(size=16) == -4 and ns(ws=p(4100)) == -2 and ns(g=p(4098)) == -2
+    large = job(rows=256, cols=300, il=300, ol=300)
+    assert ns(size=size(job()) - 1) == -4 and ns(j=large, size=size(large) - 1) == -4 and size(large) > 4 * 256 * 300
+    assert ns(ws=None) == -4 and ns(ws=p(4100)) == -2 and ns(g=p(4098)) == -2
 
     def muon(j=job(ist=0, ost=0), p_=q, g=q, m=q, e=None, ws=q, size=1 << 30):
         return so.itg_muon_step(ctypes.byref(j), 1, p_, g, m, e, f(0.1), f(0.9), 1, f(0.0), f(0.9), 1, co, f(0.0), ws, size, None)

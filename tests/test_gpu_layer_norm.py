@@ -305,3 +305,95 @@ def test_refusals(ops):
                 lambda: ops.layer_norm(x.int())):
         with pytest.raises(ItgError):
             bad()
+
+
+def call(name, *args):
+    from infinite_texture_gans_amd import _lib
+    return _lib.fn(name)(*[a.data_ptr() if torch.is_tensor(a) else a for a in args], torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("c,pad", [(3, 0), (52, 0), (45, 3), (100, 19), (1021, 0), (4096, 0), (9001, 0), (9001, 5), (20003, 0)])
+@pytest.mark.parametrize("t,dt", [(torch.float32, 0), (torch.bfloat16, 1)])
+def test_written_over_the_inputs(ops, c, pad, t, dt):
+    """y over x, dx over x and dx over dy: the bits that separate buffers give, and in the padding zeros whatever it held"""
+    rows, ld = 37, c + pad
+    x, w, b, dy = make(rows, ld, t, torch.float32, seed=c)
+    w, b = w[:c].contiguous(), b[:c].contiguous()
+    if pad:
+        x[:, c:], dy[:, c:] = float("nan"), float("inf")
+    ws = torch.empty(ops._lib.fn("itg_layer_norm_bwd_workspace")(rows, c), device="cuda")
+    for act in (0, 1, 2):
+        def fwd(src, out, stat):
+            assert call("itg_layer_norm_fwd", src, ld, w, b, out, ld, stat, rows, c, pad, dt, 0, 1e-5, act, 0.1) == 0
+
+        def bwd(src, grad, stat, out, dw, db):
+            assert call("itg_layer_norm_bwd", src, ld, grad, ld, stat, w, b, out, ld, dw, db, 0, rows, c, pad, dt, 0, act, 0.1, ws, ws.numel()) == 0
+
+        y, stat, dx = torch.empty_like(x), torch.empty(2 * rows, device="cuda"), torch.empty_like(x)
+        dw, db = torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+        fwd(x, y, stat)
+        bwd(x, dy, stat, dx, dw, db)
+        assert torch.equal(y[:, :c], ops.layer_norm(x[:, :c].contiguous(), w, b, act=act, slope=0.1)) and torch.isfinite(dx).all()
+        assert not y[:, c:].any() and not dx[:, c:].any()
+        for over in ("x", "dy"):
+            a, g = x.clone(), dy.clone()
+            ew, eb = torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+            bwd(a, g, stat, a if over == "x" else g, ew, eb)
+            assert torch.equal(a if over == "x" else g, dx) and torch.equal(ew, dw) and torch.equal(eb, db), (over, act)
+        a, s = x.clone(), torch.empty_like(stat)
+        fwd(a, a, s)
+        assert torch.equal(a, y) and torch.equal(s, stat)
+    # one buffer at two strides is no buffer at all
+    assert call("itg_layer_norm_fwd", x, ld, w, b, x, ld + 1, None, rows - 2, c, pad, dt, 0, 1e-5, 0, 0.0) == -1
+    assert call("itg_layer_norm_bwd", x, ld, dy, ld, stat, w, b, dy, ld + 1, None, None, 0, rows - 2, c, pad, dt, 0, 0, 0.0, None, 0) == -1
+
+
+def test_sinks_of_a_frozen_parameter_stay(ops):
+    x, w, b, dy = make(200, 26, torch.float32, torch.float32)
+    for k in (0, 1):
+        ps = [w.clone().requires_grad_(k == 0), b.clone().requires_grad_(k == 1)]
+        plain, = torch.autograd.grad(ops.layer_norm(x, *ps), ps[k], dy)
+        sinks = (torch.full((26,), 2.0, device="cuda"), torch.full((26,), 2.0, device="cuda"))
+        xs = x.clone().requires_grad_()
+        ops.layer_norm(xs, *ps, sinks=sinks).backward(dy)
+        assert torch.equal(sinks[k], 2.0 + plain) and torch.equal(sinks[1 - k], torch.full((26,), 2.0, device="cuda"))
+
+
+def test_second_derivatives_are_refused(ops):
+    from infinite_texture_gans_amd._lib import ItgError
+    x = torch.randn(4, 8, device="cuda", requires_grad=True)
+    with pytest.raises(ItgError):
+        torch.autograd.grad(ops.layer_norm(x).sum(), x, create_graph=True)
+
+
+def test_two_captured_graphs_and_rows_far_apart(ops):
+    """two captured training passes replayed in turn keep to their own buffers; a row stride that puts rows past 2^31 elements"""
+    made, outs = [], []
+    for seed, (rows, c) in enumerate(((40, 9001), (300, 416))):
+        x, w, b, dy = make(rows, c, torch.float32, torch.float32, seed=seed)
+        x, w, b = x.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            y = ops.layer_norm(x, w, b)
+            outs.append([y.detach()] + list(torch.autograd.grad(y, [x, w, b], dy)))
+        made.append((graph, x, w, b, dy))
+    for turn in range(3):
+        for graph, *_ in made if turn % 2 else made[::-1]:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, x, w, b, dy), got in zip(made, outs):
+            xe, we, be = (v.detach().clone().requires_grad_() for v in (x, w, b))
+            y = ops.layer_norm(xe, we, be)
+            for p, q in zip(got, [y.detach()] + list(torch.autograd.grad(y, [xe, we, be], dy))):
+                assert torch.equal(p, q)
+            for p in got:
+                p.zero_()
+    ld = (1 << 31) + 24
+    big = torch.empty(2 * ld + 64, device="cuda", dtype=torch.bfloat16)          # (written only where the three rows lie)
+    x = torch.as_strided(big, (3, 52), (ld, 1))
+    x.copy_(torch.randn(3, 52))
+    xc, dy = x.contiguous().requires_grad_(), torch.randn(3, 52, device="cuda").bfloat16()
+    xs = x.detach().requires_grad_()
+    ys, yc = ops.layer_norm(xs), ops.layer_norm(xc)
+    assert torch.equal(ys, yc) and torch.equal(torch.autograd.grad(ys, xs, dy)[0], torch.autograd.grad(yc, xc, dy)[0])
