@@ -447,7 +447,8 @@ int itg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy,
  * coefficients: HOST array of 3 * steps floats (a, b, c of each step); they must keep the singular values below 3.9 (checked).
  * dtype: ITG_F32 / ITG_F16 = products as exact as fp32 ones, ITG_BF16 = as exact as the type.  out may be g (same layout).
  * A job is `count` matrices of one shape at a stride; offsets and strides count elements from g / out.  Matrices of one call
- * must not overlap in out.  A matrix that holds an infinity or a NaN comes out as NaN, the others of the call as they are.
+ * must not overlap in out, and out overlaps g not at all or is g.  At most 2^22 matrices a call (2^23 where none has more than 128
+ * rows or columns, 2^24 where none has more than 64).  A matrix that holds an infinity or a NaN comes out as NaN, the others of the call as they are.
  * workspace: itg_newton_schulz_workspace() bytes, 16-byte aligned (-1 .. -4: the jobs are rejected).                            */
 #define ITG_NS_MAX_JOBS 32
 #define ITG_NS_MAX_DIM 65536
@@ -460,7 +461,7 @@ int64_t itg_newton_schulz_workspace(const itg_ns_job* jobs, int n, int dtype);
 int itg_newton_schulz(const itg_ns_job* jobs, int n, int dtype, const void* g, void* out, int steps, const float* coefficients,
                       float eps, void* workspace, int64_t workspace_bytes, void* stream);
 /* One optimiser step over fp32 matrices that live in flat buffers (job: count 1, contiguous, in_offset == out_offset, the same
- * offset in param, g, momentum and ema):
+ * offset in param, g, momentum and ema, which are four buffers; no two jobs overlap):
  *   momentum <- mu momentum + g;  U = nesterov ? g + mu momentum : momentum;  O = Newton-Schulz(U);
  *   param <- (1 - lr weight_decay) param - lr sqrt(max(1, rows / cols)) O;  ema <- ema_decay ema + (1 - ema_decay) param (ema may be NULL)
  * workspace as itg_newton_schulz with ITG_F32.                                                                               */

@@ -722,7 +722,7 @@ int ns_tiles(NsArgs& p, NsPlan& pl, int q, int64_t& slab) {
     const int64_t nt = j.mp / T, nx = j.np / T;
     j.tile0[q] = (int)tiles;
     tiles += (q == 2 ? nt * nx : nt * (nt + 1) / 2) * j.count;
-    if (tiles > INT32_MAX / 64) return ITG_ERR_ARG;
+    if (tiles >= ((int64_t)1 << (T == 256 ? 23 : 24))) return ITG_ERR_ARG;
   }
   const int64_t slots = 256 * (T == 256 ? 1 : 2);
   int64_t direct = tiles / slots * slots, rest = tiles - direct, shares = 0;
@@ -793,6 +793,11 @@ int ns_plan(const itg_ns_job* jobs, int n, bool split, bool muon, NsArgs& p, NsP
     if (q.in_ld > most / q.rows || q.out_ld > most / q.rows || q.in_stride > most / q.count || q.out_stride > most / q.count ||
         q.in_offset > most || q.out_offset > most) return ITG_ERR_ARG;
     if (muon && (q.count != 1 || q.in_ld != q.cols || q.out_ld != q.cols || q.in_offset != q.out_offset)) return ITG_ERR_ARG;
+    if (muon)
+      for (int k = 0; k < i; ++k) {
+        const int64_t o = jobs[k].out_offset;
+        if (q.out_offset < o + (int64_t)jobs[k].rows * jobs[k].cols && o < q.out_offset + (int64_t)q.rows * q.cols) return ITG_ERR_ARG;
+      }
     if (q.count > 1 && q.out_stride < (int64_t)(q.rows - 1) * q.out_ld + q.cols) return ITG_ERR_ARG;      // results may not overlap
     NsMat& j = p.j[i];
     j.tall = q.rows > q.cols;
@@ -808,7 +813,8 @@ int ns_plan(const itg_ns_job* jobs, int n, bool split, bool muon, NsArgs& p, NsP
       j.norm0 = (int)pl.norm; j.block0 = (int)pl.blocks;
       pl.norm += (int64_t)j.nblk * j.count;
       pl.blocks += (int64_t)j.blocks * j.count;
-      if (pl.norm > INT32_MAX || pl.blocks > INT32_MAX) return ITG_ERR_ARG;
+      // a launch counts its threads in 32 bits
+      if ((!pl.one && pl.norm >= ((int64_t)1 << 22)) || pl.blocks * 4 * pl.thin >= ((int64_t)1 << 32)) return ITG_ERR_ARG;
       j.wst = pl.one ? 0 : up(thin_ws_bytes(pl.thin, j.np, j.blocks), 256);
       j.ws = pl.bytes;
       if (j.wst > ((int64_t)1 << 60) / j.count) return ITG_ERR_ARG;
@@ -827,7 +833,7 @@ int ns_plan(const itg_ns_job* jobs, int n, bool split, bool muon, NsArgs& p, NsP
     j.norm0 = (int)pl.norm; j.conv0 = (int)pl.conv;
     pl.norm += (int64_t)j.nblk * j.count;
     pl.conv += (int64_t)(j.mp / 64) * (j.np / 64) * j.count;
-    if (pl.norm > INT32_MAX || pl.conv > INT32_MAX) return ITG_ERR_ARG;
+    if (pl.norm >= ((int64_t)1 << 22) || pl.conv >= ((int64_t)1 << 24)) return ITG_ERR_ARG;      // a launch counts its threads in 32 bits
     j.wst = up(ns_ws_bytes(j.mp, j.np, split), 256);
     j.ws = pl.bytes;
     if (j.wst > ((int64_t)1 << 60) / j.count) return ITG_ERR_ARG;
@@ -972,6 +978,7 @@ int itg_muon_step(const itg_ns_job* jobs, int n, float* param, const float* g, f
                   int nesterov, float weight_decay, float ema_decay, int steps, const float* coefficients, float eps,
                   void* workspace, int64_t workspace_bytes, void* stream) {
   if (!param || !g || !momentum || !coefficients || steps < 1 || steps > ITG_NS_MAX_STEPS || !(eps >= 0.f)) return ITG_ERR_ARG;
+  if (param == g || param == momentum || g == momentum || ema == param || ema == g || ema == momentum) return ITG_ERR_ARG;
   if (((uintptr_t)param | (uintptr_t)g | (uintptr_t)momentum | (uintptr_t)ema) & 3) return ITG_ERR_ALIGN;
   NsArgs p; NsPlan pl;
   const int rc = ns_plan(jobs, n, true, true, p, pl);

@@ -1758,7 +1758,7 @@ def _ns_coefficients(coefficients, steps):
 def _ns_workspace(jobs, n, dtype, device):
     need = _lib.fn("itg_newton_schulz_workspace")(jobs, n, dtype)
     if need < 0:
-        raise _lib.ItgError("Newton-Schulz: matrices of 1 .. %d rows and columns expected" % _lib.NS_MAX_DIM)
+        raise _lib.ItgError("Newton-Schulz: matrices of 1 .. %d rows and columns, fewer than 2^22 of them, expected" % _lib.NS_MAX_DIM)
     return torch.empty(need, device=device, dtype=torch.uint8), need
 
 
@@ -1769,7 +1769,8 @@ def orthogonalize(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-12, out=None)
     float32 / float16: products as exact as fp32 ones; bfloat16: as exact as the type.  ``g`` may be strided (row- or column-major
     matrices at one batch stride are read in place).  ``coefficients``: (a, b, c) of X <- a X + (b A + c A A) X, or one triple per
     step.  A matrix with a norm of ``eps`` or less has no direction and gives zeros; one with a NaN or an infinity gives NaN.
-    ``out``: a contiguous tensor like ``g`` for the result; may be ``g`` itself where that is contiguous."""
+    ``out``: a contiguous tensor like ``g`` for the result, which may be ``g`` itself where that is contiguous and otherwise lies
+    outside the memory that ``g`` spans."""
     if not g.is_cuda or g.dtype not in _DTYPES:
         raise _lib.ItgError("orthogonalize: a float32, bfloat16 or float16 tensor on the GPU expected, got %s on %s" % (g.dtype, g.device))
     if g.dim() < 2:
@@ -1781,6 +1782,10 @@ def orthogonalize(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-12, out=None)
     if out is not None and (out.shape != g.shape or out.dtype != g.dtype or out.device != g.device or not out.is_contiguous()
                             or (out.data_ptr() == g.data_ptr() and not g.is_contiguous())):
         raise _lib.ItgError("orthogonalize: out must be a contiguous tensor of g's shape, type and device")
+    if out is not None and out.data_ptr() != g.data_ptr() and g.numel():
+        span = sum((s - 1) * st for s, st in zip(g.shape, g.stride())) + 1
+        if g.data_ptr() < out.data_ptr() + out.numel() * out.element_size() and out.data_ptr() < g.data_ptr() + span * g.element_size():
+            raise _lib.ItgError("orthogonalize: out overlaps g")
     g = g.detach()
     result = out if out is not None else torch.empty(g.shape, device=g.device, dtype=g.dtype)
     if not g.numel():
@@ -1819,7 +1824,8 @@ def _matrices(g):
 class MuonPlan:
     """The filter matrices of a flat fp32 parameter buffer: ``shapes`` = (rows, columns) of each, one behind the other from
     element ``offset`` on.  Holds the job table and the workspace of :func:`muon_step`; steps of one plan have to be ordered
-    (they share parameters, momentum and workspace)."""
+    (they share parameters, momentum and workspace), and the plan is kept until the last of them, or the last replay of a graph
+    with one in it, has run."""
 
     def __init__(self, shapes, device, offset=0):
         self.shapes = [(int(r), int(c)) for r, c in shapes]
@@ -1856,6 +1862,8 @@ def muon_step(plan, p, g, momentum_buf, ema=None, lr=0.02, momentum=0.95, nester
         _req_cuda(t, "muon_step: " + name)
         if not t.is_contiguous() or t.numel() < plan.end or t.device != p.device:
             raise _lib.ItgError("muon_step: %s must be a contiguous buffer of at least %d values on one device" % (name, plan.end))
+    if len({t.data_ptr() for t in (p, g, momentum_buf, ema) if t is not None}) != (3 if ema is None else 4):
+        raise _lib.ItgError("muon_step: p, g, momentum_buf and ema must be buffers of their own")
     if p.device != plan.workspace.device:
         raise _lib.ItgError("muon_step: the plan was made for %s, the parameters are on %s" % (plan.workspace.device, p.device))
     if not eps >= 0.0:

@@ -193,8 +193,18 @@ def test_training_operators_reject_bad_calls_on_the_host(lib):
     def muon(j=job(ist=0, ost=0), p_=q, g=q, m=q, e=None, ws=q, size=1 << 30):
         return so.itg_muon_step(ctypes.byref(j), 1, p_, g, m, e, f(0.1), f(0.9), 1, f(0.0), f(0.9), 1, co, f(0.0), ws, size, None)
 
-    assert muon(p_=None) == -1 and muon(g=None) == -1 and muon(m=None) == -1 and muon(e=p(4098)) == -2 and muon(ws=None) == -4
-    assert muon(j=job(count=2)) == -1 and muon(j=job(il=9)) == -1 and muon(j=job(io=1, oo=0)) == -1
+    assert size(job(rows=1, cols=1, il=1, ist=1, ol=1, ost=1, count=(1 << 24) - 1)) == 16 and size(job(rows=1, cols=1, il=1, ist=1, ol=1, ost=1, count=1 << 24)) == -1
+    assert size(job(rows=65, cols=70, il=70, ol=70, ost=4550, count=1 << 23)) == -1 and size(job(rows=65, cols=70, il=70, ol=70, ost=4550, count=(1 << 23) - 1)) == 16
+    assert size(job(rows=2, cols=200, il=200, ol=200, ost=400, count=1 << 22)) == -1 and size(job(rows=130, cols=130, il=130, ol=130, ost=16900, count=1 << 21)) == -1
+
+    assert muon(p_=q, g=q) == -1                            # one buffer for two
+    q2, q3, q4 = p(1 << 20), p(2 << 20), p(3 << 20)
+    assert muon(g=q2, m=q2) == -1 and muon(g=q2, m=q3, e=q3) == -1 and muon(g=q2, m=q3, e=q, ws=q4) == -1
+    two = (lib.NsJob * 2)(job(ist=0, ost=0), job(ist=0, ost=0, io=31, oo=31))
+    assert so.itg_muon_step(two, 2, q, q2, q3, None, f(0.1), f(0.9), 1, f(0.0), f(0.9), 1, co, f(0.0), q4, 1 << 30, None) == -1      # overlap
+    assert muon(p_=None) == -1 and muon(g=None) == -1 and muon(m=None) == -1 and muon(g=q2, m=q3, e=p(4098)) == -2 and muon(g=q2, m=q3, ws=None) == -4
+    for bad in (job(count=2), job(il=9), job(io=1, oo=0)):
+        assert muon(j=bad, g=q2, m=q3) == -1
 
 
 def test_training_operators_have_no_cpu_path():

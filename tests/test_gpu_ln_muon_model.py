@@ -186,3 +186,57 @@ def test_train_and_sample_command_lines(tmp_path, mode):
     S.main(["--model_path", str(out / "2__ema.pth"), "--output_resolution_height", "100", "--output_resolution_width", "170",
             "--output_name", "gen.png"])
     assert Image.open(out / "gen.png").size == (170, 100)
+
+
+def _steps(rank, world, port, out):
+    """two iterations of the whole model: plain (world 0), or its patch rows sharded over ``world`` ranks"""
+    import os
+    import sys
+    sys.path.insert(0, os.path.dirname(__file__))
+    import torch.distributed as dist
+    from infinite_texture_gans_amd.engine import BandTrainer, Trainer
+    from infinite_texture_gans_amd.dist import BandComm
+    if world > 1:
+        os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+        dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        G, D = build(BASE)
+        args = args_of("--smooth", "--optimizer", "muon")
+        tr = BandTrainer(G, D, args, cuda, BandComm(rank, world)) if world else Trainer(G, D, args, cuda)
+        losses = []
+        for s in range(2):
+            real, z = inputs(BASE, s)
+            k = real.shape[0] // max(1, world)
+            losses.append([float(v) for v in tr.step(real[rank * k:(rank + 1) * k].to(cuda), z.to(cuda))])
+        torch.save({"losses": losses, "G": {k: v.cpu() for k, v in G.state_dict().items()},
+                    "D": {k: v.cpu() for k, v in D.state_dict().items()}}, "%s.%d.%d" % (out, world, rank))
+    finally:
+        if world > 1:
+            dist.destroy_process_group()
+
+
+def test_row_sharded_steps_equal_the_plain_ones(tmp_path):
+    """the generator's 3 patch rows on one rank and on two (2 + 1): no statistics are exchanged, the halo rows and gradients are.
+    Other conv kernels run there: gradients differ by fp32 rounding (about 1e-5), which five Newton-Schulz steps amplify by
+    3.4^5 at most - 5e-3 of an update whose singular values are 0.01 beside weights' of about 1; Adam's first steps of a vector
+    are +-lr where rounding decides the sign."""
+    import torch.multiprocessing as mp
+    from test_gpu_model import free_port
+    out = str(tmp_path / "r")
+    _steps(0, 0, 0, out)
+    _steps(0, 1, 0, out)
+    mp.spawn(_steps, args=(2, free_port(), out), nprocs=2, join=True)
+    plain = torch.load(out + ".0.0")
+    runs = [[torch.load(out + ".1.0")], [torch.load(out + ".2.%d" % r) for r in range(2)]]
+    for res in runs:
+        for s in range(2):
+            mean = np.mean([r["losses"][s] for r in res], 0)
+            assert np.allclose(mean, plain["losses"][s], rtol=1e-3, atol=1e-5), (len(res), s, mean, plain["losses"][s])
+        for key in ("G", "D"):
+            for k, v in plain[key].items():
+                got = res[0][key][k]
+                assert all(torch.equal(got, r[key][k]) for r in res[1:]), k          # the replicas stay identical
+                if v.dim() < 2:
+                    assert float((got - v).abs().max()) <= 2 * 2e-4 * 2 + 1e-6, k
+                else:
+                    assert rel_l2(got, v) < 2e-3, (k, rel_l2(got, v))

@@ -266,3 +266,33 @@ def test_every_tile_size(ops, t, m, n, batch):
         off = rel(got[z], want)
         own = rel(own, want) if own is not None else 4e-6      # fp32 chains of this kind: 2e-6 .. 4e-6 off
         assert off <= (2.0 ** -8 if t == "bf16" else 3 * own + (2.0 ** -11 if t == "f16" else 0.0)), (z, off, own)
+
+
+def test_overlaps_are_refused(ops):
+    """out inside the memory g spans; one buffer in two of a step's places; what lies beside g is fine"""
+    from infinite_texture_gans_amd._lib import ItgError
+    buf = torch.randn(100 * 80 + 40, device="cuda")
+    g, shifted = buf[:8000].view(100, 80), buf[40:].view(100, 80)
+    for a, b in ((g, shifted), (shifted, g), (buf[:8000].view(50, 160)[:, :40], buf[4000:6000].view(50, 40))):
+        with pytest.raises(ItgError):
+            ops.orthogonalize(a, out=b)
+    halves = torch.randn(2, 30, 50, device="cuda")
+    want = ops.orthogonalize(halves[0])
+    assert ops.orthogonalize(halves[0], out=halves[1]) is not None and torch.equal(halves[1], want)
+    plan = ops.MuonPlan([(4, 8)], "cuda")
+    p, g, m = (torch.randn(32, device="cuda") for _ in range(3))
+    for args in ((p, p, m), (p, g, g), (p, g, p), (p, g, m, p), (p, g, m, g), (p, g, m, m)):
+        with pytest.raises(ItgError):
+            ops.muon_step(plan, *args)
+
+
+def test_long_batches_of_tiny_matrices(ops):
+    """a workgroup per matrix: 200 000 matrices of 1 x 1 (their signs under the iteration's gain) and of 2 x 3"""
+    g = torch.randn(200000, 1, 1, device="cuda")
+    o = ops.orthogonalize(g)
+    want = steps_of(torch.ones(1, 1, dtype=torch.float64)).item()
+    assert torch.equal(torch.sign(o), torch.sign(g)) and float((o.abs() - want).abs().max()) < 1e-5
+    g = torch.randn(200000, 2, 3, device="cuda")
+    o = ops.orthogonalize(g)
+    for k in (0, 1, 99999, 199999):
+        assert torch.equal(o[k], ops.orthogonalize(g[k]))
