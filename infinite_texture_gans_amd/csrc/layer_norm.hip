@@ -6,6 +6,7 @@
 // Statistics, sums and products are fp32 whatever the tensors' type; the variance is taken around the mean of the row (a second
 // sweep over values that are already on the chip), never as a difference of moments.  Every sum has a fixed order: results do
 // not change from call to call.
+#include <type_traits>
 #include "itg_common.h"
 
 namespace {
@@ -45,12 +46,45 @@ __host__ __device__ inline LnV ln_vectors(int c, int pad, int V) {
 
 template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[V]; };
 
-// the R vectors of a thread in row `q` (nothing is read past the row's end)
+// V values as they lie in memory, in 32-bit words (a Pack of 16-bit values takes a register each)
+template <typename T, int V> struct Held {
+  static constexpr int N = (V * (int)sizeof(T) + 3) / 4;
+  uint32_t w[N];
+  __device__ __forceinline__ float at(int e) const {
+    if (sizeof(T) == 4) return __builtin_bit_cast(float, w[e]);
+    return (float)__builtin_bit_cast(T, (typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type)(w[e / 2] >> (16 * (e & 1))));
+  }
+  __device__ __forceinline__ void load(const T* q) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Words { uint32_t w[N]; };
+    if (V * sizeof(T) % 4 == 0) {
+      const Words u = *reinterpret_cast<const Words*>(q);
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = u.w[i];
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(q);
+    }
+  }
+  // the compiler takes the values for changed: what is computed from them again is not carried over in registers instead
+  __device__ __forceinline__ void renew() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm("" : "+v"(w[i]));
+  }
+};
+
+// The R vectors of a thread in row `q`.  A thread that has none reads the row's last one, and ln_take makes zeros of it: a load behind
+// a branch is waited for at the branch's end.
 template <typename T, int V, int R>
-__device__ __forceinline__ void ln_fetch(const T* q, const int (&off)[R], const int (&hi)[R], Pack<T, V> (&u)[R]) {
+__device__ __forceinline__ void ln_fetch(const T* q, const int (&off)[R], Held<T, V> (&u)[R]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) u[r].load(q + off[r]);
+}
+
+template <typename T, int V, int R>
+__device__ __forceinline__ void ln_take(const Held<T, V> (&u)[R], const int (&hi)[R], Held<T, V> (&k)[R]) {
 #pragma unroll
   for (int r = 0; r < R; ++r)
-    if (hi[r] > 0) u[r] = *reinterpret_cast<const Pack<T, V>*>(q + off[r]);
+#pragma unroll
+    for (int i = 0; i < Held<T, V>::N; ++i) k[r].w[i] = hi[r] > 0 ? u[r].w[i] : 0u;
 }
 
 template <typename T, int V>
@@ -108,6 +142,12 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return s;
 }
 
+// a thread's row among those of its workgroup; from a wave per row on the same in every lane, and known to be: addresses then are a
+// scalar base and 32 bits a lane
+template <int TPR> __device__ __forceinline__ int ln_group() {
+  return TPR > 64 ? 0 : TPR == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : threadIdx.x / TPR;
+}
+
 // ANY: an activation, or rows that V does not divide; without it neither is looked at (a quarter of the instructions per value,
 // which at 2 bytes a value is time: 16384 x 4096 bf16 forward 61.6 us with the masks, 55.5 without)
 template <typename T, typename W, int V, int TPR, int R, bool ANY>
@@ -115,7 +155,7 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
   constexpr int NT = TPR > 64 ? TPR : 256, GROUPS = NT / TPR;
   __shared__ float red[4][TPR > 64 ? TPR / 64 : 1];      // two sums per row, two rows' worth: a row's sums outlive the next row's first barrier
   const LnV lv = ln_vectors(p.c, p.pad, V);
-  const int tid = threadIdx.x % TPR;
+  const int tid = TPR > 64 ? threadIdx.x : threadIdx.x % TPR;
   int off[R], lo[R], hi[R];
   float w[R][V], b[R][V];
 #pragma unroll
@@ -128,22 +168,24 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
   const float inv = 1.f / (float)p.c;
   int flip = 0;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
-  int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / TPR;
-  Pack<T, V> u[R] = {};
-  if (row < p.rows) ln_fetch<T, V, R>((const T*)p.x + row * p.ldx, off, hi, u);
+  int64_t row = (int64_t)blockIdx.x * GROUPS + ln_group<TPR>();
+  Held<T, V> u[R] = {};
+  if (row < p.rows) ln_fetch<T, V, R>((const T*)p.x + row * p.ldx, off, u);
 #pragma unroll
   for (int r = 0; r < R; ++r) { ln_param<W, V, ANY>(p.w, off[r], hi[r], 1.f, w[r]); ln_param<W, V, ANY>(p.b, off[r], hi[r], 0.f, b[r]); }
   for (; row < p.rows; row += step, flip ^= 2) {
     float f[R][V], s = 0.f;
+    Held<T, V> k[R];
+    ln_take<T, V, R>(u, hi, k);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        f[r][e] = (float)u[r].v[e];
+        f[r][e] = k[r].at(e);
         s += !ANY || (e >= lo[r] && e < hi[r]) ? f[r][e] : 0.f;      // a vector past the row's end holds zeros
       }
     // the next row is on its way while this one is reduced and written
-    if (row + step < p.rows) ln_fetch<T, V, R>((const T*)p.x + (row + step) * p.ldx, off, hi, u);
+    if (row + step < p.rows) ln_fetch<T, V, R>((const T*)p.x + (row + step) * p.ldx, off, u);
     const float mean = row_sum<TPR>(s, red[flip]) * inv;
     s = 0.f;
 #pragma unroll
@@ -175,60 +217,86 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
   }
 }
 
-// dx, and this workgroup's share of dw | db (`part`), which a thread sums over the rows it sees for the channels it holds
+// dx, and this workgroup's share of dw | db (`part`), which a thread sums over the rows it sees for the channels it holds.
+// From 16 channels a thread on (R V = 16, rows of 8193 .. 16384 16-bit values) the row stays in its own 16 bits between the two
+// sweeps and gamma in its own type, and the next row is fetched behind the last sweep: fp32 copies and a row under way do not fit
+// the 128 registers that 1024 threads have (4096 x 12288 bf16: 88 us, swept three times by the kernels for any length 142).
 template <typename T, typename W, int V, int TPR, int R, bool ANY>
 __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
   constexpr int NT = TPR > 64 ? TPR : 256, GROUPS = NT / TPR;
+  constexpr bool TIGHT = R * V >= 16;
   __shared__ float red[4][TPR > 64 ? TPR / 64 : 1];
   const LnV lv = ln_vectors(p.c, p.pad, V);
-  const int tid = threadIdx.x % TPR;
+  const int tid = TPR > 64 ? threadIdx.x : threadIdx.x % TPR;
   int off[R], lo[R], hi[R];
   float w[R][V], b[R][V], aw[R][V], ab[R][V];
+  Held<W, V> tw[R] = {}, tb[R] = {};
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int i = tid + r * TPR;
     off[r] = i < lv.nv - 1 ? i * V : lv.off_last;
     lo[r] = i < lv.nv - 1 ? 0 : lv.lo_last;
     hi[r] = i < lv.nv - 1 ? V : i < lv.nv ? lv.hi_last : 0;
-    ln_param<W, V, ANY>(p.w, off[r], hi[r], 1.f, w[r]);
-    ln_param<W, V, ANY>(ANY && p.act ? p.b : nullptr, off[r], hi[r], 0.f, b[r]);
+    if (TIGHT) {
+      if (hi[r] > 0 && p.w) tw[r].load((const W*)p.w + off[r]);
+      if (ANY && p.act && hi[r] > 0 && p.b) tb[r].load((const W*)p.b + off[r]);
+    } else {
+      ln_param<W, V, ANY>(p.w, off[r], hi[r], 1.f, w[r]);
+      ln_param<W, V, ANY>(ANY && p.act ? p.b : nullptr, off[r], hi[r], 0.f, b[r]);
+    }
 #pragma unroll
     for (int e = 0; e < V; ++e) aw[r][e] = ab[r][e] = 0.f;
   }
   const float inv = 1.f / (float)p.c;
   int flip = 0;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
-  int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / TPR;
-  Pack<T, V> ux[R] = {}, ug[R] = {};
+  int64_t row = (int64_t)blockIdx.x * GROUPS + ln_group<TPR>();
+  Held<T, V> ux[R] = {}, ug[R] = {};
   float mean = 0.f, rs = 0.f;
   auto fetch = [&](int64_t at) {
-    ln_fetch<T, V, R>((const T*)p.x + at * p.ldx, off, hi, ux);
-    ln_fetch<T, V, R>((const T*)p.dy + at * p.lddy, off, hi, ug);
+    ln_fetch<T, V, R>((const T*)p.x + at * p.ldx, off, ux);
+    ln_fetch<T, V, R>((const T*)p.dy + at * p.lddy, off, ug);
     mean = p.stat[2 * at]; rs = p.stat[2 * at + 1];
+  };
+  auto gain = [&](int r, int e) { return TIGHT ? p.w ? tw[r].at(e) : 1.f : w[r][e]; };
+  // xh, and the gradient in front of the activation
+  auto at_u = [&](int r, int e, const Held<T, V>& px, const Held<T, V>& pg, float m, float s, float& xh, float& du) {
+    xh = (px.at(e) - m) * s;
+    du = pg.at(e);
+    if (ANY && p.act) du *= act_slope_at(fmaf(xh, gain(r, e), TIGHT ? tb[r].at(e) : b[r][e]), p.act, p.slope);
   };
   if (row < p.rows) fetch(row);
   for (; row < p.rows; row += step, flip ^= 2) {
     float xh[R][V], g[R][V], s1 = 0.f, s2 = 0.f;
-    const float r_now = rs;
+    const float r_now = rs, m_now = mean;
+    Held<T, V> kx[R], kg[R];
+    ln_take<T, V, R>(ux, hi, kx);
+    ln_take<T, V, R>(ug, hi, kg);
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+      if (TIGHT) { kx[r].renew(); kg[r].renew(); tw[r].renew(); if (ANY) tb[r].renew(); }
 #pragma unroll
       for (int e = 0; e < V; ++e) {      // a vector past the row's end holds zeros in dy
         const bool in = !ANY || (e >= lo[r] && e < hi[r]);
-        const float h = in ? ((float)ux[r].v[e] - mean) * rs : 0.f;
-        xh[r][e] = ANY ? ((float)ux[r].v[e] - mean) * rs : h;
-        float all = (float)ug[r].v[e];
-        if (ANY && p.act) all *= act_slope_at(fmaf(xh[r][e], w[r][e], b[r][e]), p.act, p.slope);
-        const float du = in ? all : 0.f;
+        float h, all;
+        at_u(r, e, kx[r], kg[r], m_now, r_now, h, all);
+        xh[r][e] = h;
+        if (ANY && !in) h = 0.f;
+        const float du = in ? all : 0.f, wi = gain(r, e);
         aw[r][e] = fmaf(du, h, aw[r][e]);
         ab[r][e] += du;
-        g[r][e] = all * w[r][e];
-        const float gi = ANY ? du * w[r][e] : g[r][e];
+        g[r][e] = all * wi;
+        const float gi = ANY ? du * wi : g[r][e];
         s1 += gi;
         s2 = fmaf(gi, h, s2);
       }
+    }
+    if (TIGHT) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) { kx[r].renew(); kg[r].renew(); tw[r].renew(); if (ANY) tb[r].renew(); }
+    }
     // the next row is on its way while this one is reduced and written
-    if (row + step < p.rows) fetch(row + step);
+    if (!TIGHT && row + step < p.rows) fetch(row + step);
     if (p.y) {
       const float m1 = row_sum<TPR>(s1, red[flip]) * inv, m2 = row_sum<TPR>(s2, red[flip + 1]) * inv;
       T* dx = (T*)p.y + row * p.ldy;
@@ -236,12 +304,16 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
       for (int r = 0; r < R; ++r) {
         if (hi[r] <= 0) continue;
 #pragma unroll
-        for (int e = 0; e < V; ++e) g[r][e] = !ANY || e < hi[r] ? r_now * (g[r][e] - m1 - xh[r][e] * m2) : 0.f;
+        for (int e = 0; e < V; ++e) {
+          if (TIGHT) { at_u(r, e, kx[r], kg[r], m_now, r_now, xh[r][e], g[r][e]); g[r][e] *= gain(r, e); }
+          g[r][e] = !ANY || e < hi[r] ? r_now * (g[r][e] - m1 - xh[r][e] * m2) : 0.f;
+        }
         ln_store<T, V>(dx + off[r], g[r]);
       }
       if (ANY && p.pad && lv.hi_last == V)
         for (int i = tid; i < p.pad; i += TPR) dx[p.c + i] = (T)0.f;
     }
+    if (TIGHT && row + step < p.rows) fetch(row + step);
   }
   if (!p.part) return;
   // the row groups of this workgroup: lanes of a wave by shuffles, waves in order through LDS
@@ -461,8 +533,8 @@ int ln_fwd_run(const LnP& p, hipStream_t s) {
 }
 
 // Threads per row and vectors per thread: as few threads as hold the row at one vector each up to a wave; beyond, workgroups of
-// 128 .. 1024 threads at one vector of 8 or two of 4 (the backward pass keeps six values per channel it holds: at 16 channels a
-// thread it spills).
+// 128 .. 1024 threads at two vectors each (backward: at one vector of 8 or two of 4, as it keeps six values per channel it holds;
+// at two of 8 its row stays in 16 bits, see there).
 template <typename T, typename W>
 int ln_fwd_t(const LnP& p, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
@@ -503,6 +575,10 @@ int ln_bwd_t(LnP p, void* dw, void* db, int acc, hipStream_t s) {
   constexpr int V = 16 / sizeof(T), K = V == 8 ? 1 : 2;      // K: vectors per thread of the workgroup sizes
   const int nv = (p.c + V - 1) / V, padded = p.pad > 0 && p.pad < V && (p.c + p.pad) % V == 0;
   const bool shares = dw || db;
+  // A row in registers is read once, but every workgroup leaves a share of dw | db, 16 bytes a channel written and read, where the
+  // kernels for any length read the row three times and leave a share per 8 rows: those for few long rows (bf16, 8192 channels:
+  // 256 rows 24.4 us in registers, 16.0 swept; 768 rows 25.5, 30.5; 16384 channels: 512 rows 43, 33; 1536 rows 59, 81)
+  const bool few = p.c >= 8192 && p.rows * 16 < p.c;
   int chunks = 0, rc = ITG_OK;
   if (!shares) p.part = nullptr;
   if (p.c < V && !padded) rc = p.c <= 4 ? ln_bwd_run<T, W, 1, 4, 1>(p, chunks, s) : ln_bwd_run<T, W, 1, 8, 1>(p, chunks, s);
@@ -515,7 +591,8 @@ int ln_bwd_t(LnP p, void* dw, void* db, int acc, hipStream_t s) {
   else if (nv <= 128 * K) rc = ln_bwd_run<T, W, V, 128, K>(p, chunks, s);
   else if (nv <= 256 * K) rc = ln_bwd_run<T, W, V, 256, K>(p, chunks, s);
   else if (nv <= 512 * K) rc = ln_bwd_run<T, W, V, 512, K>(p, chunks, s);
-  else if (nv <= 1024 * K) rc = ln_bwd_run<T, W, V, 1024, K>(p, chunks, s);
+  else if (nv <= 1024 * K && !few) rc = ln_bwd_run<T, W, V, 1024, K>(p, chunks, s);
+  else if (nv <= 2048 && !few) rc = ln_bwd_run<T, W, V, 1024, 2>(p, chunks, s);
   else {
     // (the shares read every row of dy and x, and dx may be written over either)
     if (shares) {

@@ -397,3 +397,46 @@ def test_two_captured_graphs_and_rows_far_apart(ops):
     xs = x.detach().requires_grad_()
     ys, yc = ops.layer_norm(xs), ops.layer_norm(xc)
     assert torch.equal(ys, yc) and torch.equal(torch.autograd.grad(ys, xs, dy)[0], torch.autograd.grad(yc, xc, dy)[0])
+
+
+@pytest.mark.parametrize("rows,c", [(520, 8200), (600, 9001), (1030, 16384), (3, 8200), (511, 8192), (512, 8192)])
+@pytest.mark.parametrize("types", ["bf16/bf16", "f16/f32", "f32/f32"])
+def test_many_and_few_long_rows(ops, rows, c, types):
+    """rows of more than 8192 values: in registers where they are many, swept where they are few"""
+    t, tw = (TYPES[k] for k in types.split("/"))
+    x, w, b, dy = make(rows, c, t, tw, seed=rows)
+    for act, slope in ((0, 0.0), (1, 0.1)):
+        want, u = oracle(x.double(), w.double(), b.double(), dy.double(), 1e-5, act, slope, t, tw)
+        g = dy if act == 0 else torch.where(u.abs() < 1e-4, torch.zeros_like(dy), dy)
+        if act:
+            want, _ = oracle(x.double(), w.double(), b.double(), g.double(), 1e-5, act, slope, t, tw)
+        y, grads = run(ops, x, w, b, g, act=act, slope=slope)
+        for got, ref, what in zip((y,) + tuple(grads), want, ("y", "dx", "dw", "db")):
+            near(got, ref, what)
+
+
+@pytest.mark.parametrize("t,dt", [(torch.bfloat16, 1), (torch.float16, 2)])
+def test_many_long_rows_over_the_inputs(ops, t, dt):
+    """as test_written_over_the_inputs, for rows that stay in registers in 16 bits, with padding that holds anything"""
+    rows, c, pad = 600, 9001, 5
+    ld = c + pad
+    x, w, b, dy = make(rows, ld, t, torch.float32, seed=5)
+    w, b = w[:c].contiguous(), b[:c].contiguous()
+    x[:, c:], dy[:, c:] = float("inf"), float("nan")
+    ws = torch.empty(ops._lib.fn("itg_layer_norm_bwd_workspace")(rows, c), device="cuda")
+    y, stat, dx = torch.empty_like(x), torch.empty(2 * rows, device="cuda"), torch.empty_like(x)
+    dw, db = torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+    assert call("itg_layer_norm_fwd", x, ld, w, b, y, ld, stat, rows, c, pad, dt, 0, 1e-5, 1, 0.1) == 0
+
+    def bwd(src, grad, out, gw, gb):
+        assert call("itg_layer_norm_bwd", src, ld, grad, ld, stat, w, b, out, ld, gw, gb, 0, rows, c, pad, dt, 0, 1, 0.1, ws, ws.numel()) == 0
+
+    bwd(x, dy, dx, dw, db)
+    xs, ps = x[:, :c].contiguous().requires_grad_(), [w.requires_grad_(), b.requires_grad_()]
+    want = torch.autograd.grad(ops.layer_norm(xs, *ps, act=1, slope=0.1), [xs] + ps, dy[:, :c].contiguous())
+    assert torch.equal(dx[:, :c], want[0]) and not dx[:, c:].any() and torch.equal(dw, want[1]) and torch.equal(db, want[2])
+    for over in ("x", "dy"):
+        a, g = x.clone(), dy.clone()
+        ew, eb = torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+        bwd(a, g, a if over == "x" else g, ew, eb)
+        assert torch.equal(a if over == "x" else g, dx) and torch.equal(ew, dw) and torch.equal(eb, db), over
