@@ -79,19 +79,36 @@ __device__ __forceinline__ void ln_fetch(const T* q, const int (&off)[R], Held<T
   for (int r = 0; r < R; ++r) u[r].load(q + off[r]);
 }
 
-template <typename T, int V, int R>
-__device__ __forceinline__ void ln_take(const Held<T, V> (&u)[R], const int (&hi)[R], Held<T, V> (&k)[R]) {
+template <typename T, int V, int R, bool MASK>
+__device__ __forceinline__ void ln_take(const Held<T, V> (&u)[R], const int (&hi)[R], const Held<T, V> (&mine)[R], Held<T, V> (&k)[R]) {
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int i = 0; i < Held<T, V>::N; ++i) k[r].w[i] = hi[r] > 0 ? u[r].w[i] : 0u;
+    for (int i = 0; i < Held<T, V>::N; ++i) k[r].w[i] = MASK ? u[r].w[i] & mine[r].w[i] : hi[r] > 0 ? u[r].w[i] : 0u;
 }
 
+// the bits of a vector's values in front of `hi`
 template <typename T, int V>
-__device__ __forceinline__ void ln_store(T* q, const float (&f)[V]) {
+__device__ __forceinline__ void ln_bits(int hi, Held<T, V>& m) {
+#pragma unroll
+  for (int i = 0; i < Held<T, V>::N; ++i) m.w[i] = 0u;
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (e < hi) m.w[e * sizeof(T) / 4] |= sizeof(T) == 4 ? ~0u : 0xffffu << (16 * (e & 1));
+}
+
+template <typename T, int V, bool MASK>
+__device__ __forceinline__ void ln_store(T* q, const float (&f)[V], const Held<T, V>& mine) {
   Pack<T, V> u;
 #pragma unroll
   for (int e = 0; e < V; ++e) u.v[e] = (T)f[e];
+  if (MASK) {
+    Held<T, V> k = {};
+    __builtin_memcpy(&k, &u, sizeof(u));
+#pragma unroll
+    for (int i = 0; i < Held<T, V>::N; ++i) k.w[i] &= mine.w[i];
+    __builtin_memcpy(&u, &k, sizeof(u));
+  }
   *reinterpret_cast<Pack<T, V>*>(q) = u;
 }
 
@@ -148,22 +165,33 @@ template <int TPR> __device__ __forceinline__ int ln_group() {
   return TPR > 64 ? 0 : TPR == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : threadIdx.x / TPR;
 }
 
-// ANY: an activation, or rows that V does not divide; without it neither is looked at (a quarter of the instructions per value,
-// which at 2 bytes a value is time: 16384 x 4096 bf16 forward 61.6 us with the masks, 55.5 without)
-template <typename T, typename W, int V, int TPR, int R, bool ANY>
+// What a row needs beyond its values: nothing, masks (V does not divide it), or an activation too.  Each is a kernel of its own: at 2
+// bytes a value instructions are time (forward, bf16: 16384 x 4096 takes 43.0 us plain, 49.3 with the activation, 53.6 where masks and
+// the activation's kind are looked at for every value; 60000 x 333 19.7 us where a mask is a factor and an AND, 25.7 where it is two
+// comparisons a value).
+enum { LN_PLAIN = 0, LN_MASK = 1, LN_ACT = 2 };
+
+template <typename T, typename W, int V, int TPR, int R, int KIND>
 __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
   constexpr int NT = TPR > 64 ? TPR : 256, GROUPS = NT / TPR;
   __shared__ float red[4][TPR > 64 ? TPR / 64 : 1];      // two sums per row, two rows' worth: a row's sums outlive the next row's first barrier
   const LnV lv = ln_vectors(p.c, p.pad, V);
   const int tid = TPR > 64 ? threadIdx.x : threadIdx.x % TPR;
+  constexpr bool MASK = KIND != LN_PLAIN;
   int off[R], lo[R], hi[R];
-  float w[R][V], b[R][V];
+  float w[R][V], b[R][V], m[R][V];      // m: 1 for the values a thread counts, 0 for those it shares with a neighbour and padding
+  Held<T, V> mine[R];                   // the bits of the values it reads and writes
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int i = tid + r * TPR;
     off[r] = i < lv.nv - 1 ? i * V : lv.off_last;
     lo[r] = i < lv.nv - 1 ? 0 : lv.lo_last;
     hi[r] = i < lv.nv - 1 ? V : i < lv.nv ? lv.hi_last : 0;
+    if (MASK) {
+      ln_bits<T, V>(hi[r], mine[r]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) m[r][e] = e >= lo[r] && e < hi[r] ? 1.f : 0.f;
+    }
   }
   const float inv = 1.f / (float)p.c;
   int flip = 0;
@@ -172,17 +200,18 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
   Held<T, V> u[R] = {};
   if (row < p.rows) ln_fetch<T, V, R>((const T*)p.x + row * p.ldx, off, u);
 #pragma unroll
-  for (int r = 0; r < R; ++r) { ln_param<W, V, ANY>(p.w, off[r], hi[r], 1.f, w[r]); ln_param<W, V, ANY>(p.b, off[r], hi[r], 0.f, b[r]); }
+  for (int r = 0; r < R; ++r) { ln_param<W, V, MASK>(p.w, off[r], hi[r], 1.f, w[r]); ln_param<W, V, MASK>(p.b, off[r], hi[r], 0.f, b[r]); }
+  const float below = p.act == ITG_ACT_LRELU ? p.slope : 1.f;
   for (; row < p.rows; row += step, flip ^= 2) {
     float f[R][V], s = 0.f;
     Held<T, V> k[R];
-    ln_take<T, V, R>(u, hi, k);
+    ln_take<T, V, R, MASK>(u, hi, mine, k);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         f[r][e] = k[r].at(e);
-        s += !ANY || (e >= lo[r] && e < hi[r]) ? f[r][e] : 0.f;      // a vector past the row's end holds zeros
+        s = MASK ? fmaf(f[r][e], m[r][e], s) : s + f[r][e];      // a vector past the row's end holds zeros
       }
     // the next row is on its way while this one is reduced and written
     if (row + step < p.rows) ln_fetch<T, V, R>((const T*)p.x + (row + step) * p.ldx, off, u);
@@ -194,10 +223,9 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         f[r][e] -= mean;
-        const float d = !ANY || (e >= lo[r] && e < hi[r]) ? f[r][e] : 0.f;      // (padding may hold anything, a NaN too)
-        q = fmaf(d, d, q);
+        q = fmaf(MASK ? f[r][e] * m[r][e] : f[r][e], f[r][e], q);
       }
-      s += hi[r] > 0 ? q : 0.f;
+      s += MASK || hi[r] > 0 ? q : 0.f;
     }
     const float rs = 1.f / sqrtf(row_sum<TPR>(s, red[flip + 1]) * inv + p.eps);
     T* y = (T*)p.y + row * p.ldy;
@@ -207,11 +235,15 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         f[r][e] = fmaf(f[r][e] * rs, w[r][e], b[r][e]);
-        if (ANY) f[r][e] = e < hi[r] ? act_apply(f[r][e], p.act, p.slope) : 0.f;
+        if (KIND == LN_ACT) f[r][e] = f[r][e] > 0.f ? f[r][e] : f[r][e] * below;
       }
-      ln_store<T, V>(y + off[r], f[r]);
+      if (KIND == LN_ACT && p.act == ITG_ACT_TANH) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[r][e] = tanhf(f[r][e]);
+      }
+      ln_store<T, V, MASK>(y + off[r], f[r], mine[r]);
     }
-    if (ANY && p.pad && lv.hi_last == V)
+    if (MASK && p.pad && lv.hi_last == V)
       for (int i = tid; i < p.pad; i += TPR) y[p.c + i] = (T)0.f;
     if (p.stat && tid == 0) { p.stat[2 * row] = mean; p.stat[2 * row + 1] = rs; }
   }
@@ -221,15 +253,16 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
 // From 16 channels a thread on (R V = 16, rows of 8193 .. 16384 16-bit values) the row stays in its own 16 bits between the two
 // sweeps and gamma in its own type, and the next row is fetched behind the last sweep: fp32 copies and a row under way do not fit
 // the 128 registers that 1024 threads have (4096 x 12288 bf16: 88 us, swept three times by the kernels for any length 142).
-template <typename T, typename W, int V, int TPR, int R, bool ANY>
+template <typename T, typename W, int V, int TPR, int R, int KIND>
 __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
   constexpr int NT = TPR > 64 ? TPR : 256, GROUPS = NT / TPR;
-  constexpr bool TIGHT = R * V >= 16;
+  constexpr bool TIGHT = R * V >= 16, MASK = KIND != LN_PLAIN, ACT = KIND == LN_ACT;
   __shared__ float red[4][TPR > 64 ? TPR / 64 : 1];
   const LnV lv = ln_vectors(p.c, p.pad, V);
   const int tid = TPR > 64 ? threadIdx.x : threadIdx.x % TPR;
   int off[R], lo[R], hi[R];
-  float w[R][V], b[R][V], aw[R][V], ab[R][V];
+  float w[R][V], b[R][V], aw[R][V], ab[R][V], m[R][V];
+  Held<T, V> mine[R];
   Held<W, V> tw[R] = {}, tb[R] = {};
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -237,12 +270,17 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
     off[r] = i < lv.nv - 1 ? i * V : lv.off_last;
     lo[r] = i < lv.nv - 1 ? 0 : lv.lo_last;
     hi[r] = i < lv.nv - 1 ? V : i < lv.nv ? lv.hi_last : 0;
+    if (MASK) {
+      ln_bits<T, V>(hi[r], mine[r]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) m[r][e] = e >= lo[r] && e < hi[r] ? 1.f : 0.f;
+    }
     if (TIGHT) {
       if (hi[r] > 0 && p.w) tw[r].load((const W*)p.w + off[r]);
-      if (ANY && p.act && hi[r] > 0 && p.b) tb[r].load((const W*)p.b + off[r]);
+      if (ACT && hi[r] > 0 && p.b) tb[r].load((const W*)p.b + off[r]);
     } else {
-      ln_param<W, V, ANY>(p.w, off[r], hi[r], 1.f, w[r]);
-      ln_param<W, V, ANY>(ANY && p.act ? p.b : nullptr, off[r], hi[r], 0.f, b[r]);
+      ln_param<W, V, MASK>(p.w, off[r], hi[r], 1.f, w[r]);
+      ln_param<W, V, MASK>(ACT ? p.b : nullptr, off[r], hi[r], 0.f, b[r]);
     }
 #pragma unroll
     for (int e = 0; e < V; ++e) aw[r][e] = ab[r][e] = 0.f;
@@ -263,37 +301,38 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
   auto at_u = [&](int r, int e, const Held<T, V>& px, const Held<T, V>& pg, float m, float s, float& xh, float& du) {
     xh = (px.at(e) - m) * s;
     du = pg.at(e);
-    if (ANY && p.act) du *= act_slope_at(fmaf(xh, gain(r, e), TIGHT ? tb[r].at(e) : b[r][e]), p.act, p.slope);
+    if (ACT) {
+      const float u = fmaf(xh, gain(r, e), TIGHT ? tb[r].at(e) : b[r][e]);
+      if (p.act == ITG_ACT_TANH) { const float t = tanhf(u); du *= 1.f - t * t; }
+      else du *= u > 0.f ? 1.f : p.slope;
+    }
   };
   if (row < p.rows) fetch(row);
   for (; row < p.rows; row += step, flip ^= 2) {
     float xh[R][V], g[R][V], s1 = 0.f, s2 = 0.f;
     const float r_now = rs, m_now = mean;
     Held<T, V> kx[R], kg[R];
-    ln_take<T, V, R>(ux, hi, kx);
-    ln_take<T, V, R>(ug, hi, kg);
+    ln_take<T, V, R, MASK>(ux, hi, mine, kx);
+    ln_take<T, V, R, MASK>(ug, hi, mine, kg);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (TIGHT) { kx[r].renew(); kg[r].renew(); tw[r].renew(); if (ANY) tb[r].renew(); }
+      if (TIGHT) { kx[r].renew(); kg[r].renew(); tw[r].renew(); if (ACT) tb[r].renew(); }
 #pragma unroll
       for (int e = 0; e < V; ++e) {      // a vector past the row's end holds zeros in dy
-        const bool in = !ANY || (e >= lo[r] && e < hi[r]);
-        float h, all;
-        at_u(r, e, kx[r], kg[r], m_now, r_now, h, all);
+        float h, du;
+        at_u(r, e, kx[r], kg[r], m_now, r_now, h, du);
         xh[r][e] = h;
-        if (ANY && !in) h = 0.f;
-        const float du = in ? all : 0.f, wi = gain(r, e);
-        aw[r][e] = fmaf(du, h, aw[r][e]);
+        aw[r][e] = fmaf(du, h, aw[r][e]);      // (of a value that a neighbour counts, too: left out at the end)
         ab[r][e] += du;
-        g[r][e] = all * wi;
-        const float gi = ANY ? du * wi : g[r][e];
+        g[r][e] = du * gain(r, e);
+        const float gi = !MASK ? g[r][e] : TIGHT ? (e >= lo[r] && e < hi[r] ? g[r][e] : 0.f) : g[r][e] * m[r][e];
         s1 += gi;
         s2 = fmaf(gi, h, s2);
       }
     }
     if (TIGHT) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) { kx[r].renew(); kg[r].renew(); tw[r].renew(); if (ANY) tb[r].renew(); }
+      for (int r = 0; r < R; ++r) { kx[r].renew(); kg[r].renew(); tw[r].renew(); if (ACT) tb[r].renew(); }
     }
     // the next row is on its way while this one is reduced and written
     if (!TIGHT && row + step < p.rows) fetch(row + step);
@@ -306,11 +345,11 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           if (TIGHT) { at_u(r, e, kx[r], kg[r], m_now, r_now, xh[r][e], g[r][e]); g[r][e] *= gain(r, e); }
-          g[r][e] = !ANY || e < hi[r] ? r_now * (g[r][e] - m1 - xh[r][e] * m2) : 0.f;
+          g[r][e] = r_now * (g[r][e] - m1 - xh[r][e] * m2);
         }
-        ln_store<T, V>(dx + off[r], g[r]);
+        ln_store<T, V, MASK>(dx + off[r], g[r], mine[r]);
       }
-      if (ANY && p.pad && lv.hi_last == V)
+      if (MASK && p.pad && lv.hi_last == V)
         for (int i = tid; i < p.pad; i += TPR) dx[p.c + i] = (T)0.f;
     }
     if (TIGHT && row + step < p.rows) fetch(row + step);
@@ -518,16 +557,17 @@ constexpr int LN_CHUNKS = 1024;      // at most this many shares of dw | db
 inline int ln_chunks(int64_t rows) { return (int)(rows < LN_CHUNKS ? rows : LN_CHUNKS); }
 inline unsigned ln_grid(int64_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); }
 
-// ANY of the kernels: an activation, a row that V does not divide (padding included)
-template <int V> inline bool ln_any(const LnP& p) { return p.act != ITG_ACT_NONE || p.c % V != 0 || p.pad != 0; }
+template <int V> inline int ln_kind(const LnP& p) { return p.act != ITG_ACT_NONE ? LN_ACT : p.c % V != 0 || p.pad != 0 ? LN_MASK : LN_PLAIN; }
 
 template <typename T, typename W, int V, int TPR, int R>
 int ln_fwd_run(const LnP& p, hipStream_t s) {
   constexpr int NT = TPR > 64 ? TPR : 256, GROUPS = NT / TPR;
   const int64_t need = (p.rows + GROUPS - 1) / GROUPS, most = 256 * (2048 / NT);
   const dim3 grid((unsigned)(need < most ? need : most));
-  if (ln_any<V>(p)) hipLaunchKernelGGL((ln_fwd_kernel<T, W, V, TPR, R, true>), grid, dim3(NT), 0, s, p);
-  else hipLaunchKernelGGL((ln_fwd_kernel<T, W, V, TPR, R, false>), grid, dim3(NT), 0, s, p);
+  const int kind = ln_kind<V>(p);
+  if (kind == LN_ACT) hipLaunchKernelGGL((ln_fwd_kernel<T, W, V, TPR, R, LN_ACT>), grid, dim3(NT), 0, s, p);
+  else if (kind == LN_MASK) hipLaunchKernelGGL((ln_fwd_kernel<T, W, V, TPR, R, LN_MASK>), grid, dim3(NT), 0, s, p);
+  else hipLaunchKernelGGL((ln_fwd_kernel<T, W, V, TPR, R, LN_PLAIN>), grid, dim3(NT), 0, s, p);
   ITG_CHECK_LAUNCH();
   return ITG_OK;
 }
@@ -564,8 +604,10 @@ int ln_bwd_run(const LnP& p, int& chunks, hipStream_t s) {
   // every CU has a workgroup before one gets fewer than four turns: a share costs a write and a read of 2 c floats
   const int64_t most = 256 * (1024 / NT) < LN_CHUNKS ? (256 * (1024 / NT) < few ? 256 * (1024 / NT) : few) : (LN_CHUNKS < few ? LN_CHUNKS : few);
   chunks = (int)(need < most ? need : most);
-  if (ln_any<V>(p)) hipLaunchKernelGGL((ln_bwd_kernel<T, W, V, TPR, R, true>), dim3(chunks), dim3(NT), 0, s, p);
-  else hipLaunchKernelGGL((ln_bwd_kernel<T, W, V, TPR, R, false>), dim3(chunks), dim3(NT), 0, s, p);
+  const int kind = ln_kind<V>(p);
+  if (kind == LN_ACT) hipLaunchKernelGGL((ln_bwd_kernel<T, W, V, TPR, R, LN_ACT>), dim3(chunks), dim3(NT), 0, s, p);
+  else if (kind == LN_MASK) hipLaunchKernelGGL((ln_bwd_kernel<T, W, V, TPR, R, LN_MASK>), dim3(chunks), dim3(NT), 0, s, p);
+  else hipLaunchKernelGGL((ln_bwd_kernel<T, W, V, TPR, R, LN_PLAIN>), dim3(chunks), dim3(NT), 0, s, p);
   ITG_CHECK_LAUNCH();
   return ITG_OK;
 }
