@@ -1190,6 +1190,18 @@ def _rows(t):
     return (t, ld) if ld is not None else (t.contiguous(), t.shape[-1])
 
 
+def _call_on(index, name, *args):
+    """``_lib.call`` with the current stream of device ``index`` as the last argument, that device being the current one."""
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _lib.call(name, *args, _stream())
+    return _lib.call(name, *args, _raw_stream(index) if _raw_stream is not None else _stream())
+
+
+def _dense_like(x):
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+
+
 def _ln_forward(x, ldx, gamma, beta, c, eps, act, slope, stats):
     """-> (y, mean and 1 / deviation of every row or None, ITG_* type of x, of gamma and beta); x's rows at a stride of ``ldx``."""
     dt = _DTYPES[x.dtype]
@@ -1197,27 +1209,27 @@ def _ln_forward(x, ldx, gamma, beta, c, eps, act, slope, stats):
     pdt = _DTYPES[p.dtype] if p is not None else dt
     width = x.shape[-1]
     rows = x.numel() // width
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = _dense_like(x)
     stat = torch.empty(2 * rows, device=x.device, dtype=torch.float32) if stats else None
     if rows:
-        with _on(x):
-            _lib.call("itg_layer_norm_fwd", x.data_ptr(), ldx, gamma.data_ptr() if gamma is not None else None,
-                      beta.data_ptr() if beta is not None else None, y.data_ptr(), width, stat.data_ptr() if stats else None, rows, c,
-                      width - c, dt, pdt, eps, act, slope, _stream())
+        _call_on(x.get_device(), "itg_layer_norm_fwd", x.data_ptr(), ldx, gamma.data_ptr() if gamma is not None else None,
+                 beta.data_ptr() if beta is not None else None, y.data_ptr(), width, stat.data_ptr() if stats else None, rows, c,
+                 width - c, dt, pdt, eps, act, slope)
     if act == ACT_LRELU and dt == _lib.DT_F32:
         _sink_act(y, c, act, "ln")
     return y, stat, dt, pdt
 
 
 class _LayerNorm(torch.autograd.Function):
-    """y = act(gamma * xhat + beta), xhat = the row's values normalised with their own mean and variance; ``c`` of the
-    x.shape[-1] values of a row are channels, the rest (patch-grid padding) is written as zeros."""
+    """y = act(gamma * xhat + beta), xhat = the row's values normalised with their own mean and variance; ``how`` = (c, eps, act,
+    slope, sinks): c of the x.shape[-1] values of a row are channels, the rest (patch-grid padding) is written as zeros."""
 
     @staticmethod
-    def forward(ctx, x, gamma, beta, c, eps, act, slope, sinks):
+    def forward(ctx, x, gamma, beta, how):
+        c, eps, act, slope, sinks = how
         x, ldx = _rows(x)
         y, stat, dt, pdt = _ln_forward(x, ldx, gamma, beta, c, eps, act, slope, True)
-        ctx.meta = (c, x.shape[-1], ldx, dt, pdt, act, slope, sinks)
+        ctx.meta = (stat.numel() // 2, c, x.shape[-1], ldx, dt, pdt, act, slope, sinks)
         ctx.save_for_backward(x, gamma, beta, stat)
         return y
 
@@ -1227,11 +1239,10 @@ class _LayerNorm(torch.autograd.Function):
         if torch.is_grad_enabled():
             raise _lib.ItgError("layer_norm: no second derivatives (create_graph=True)")
         x, gamma, beta, stat = ctx.saved_tensors
-        c, width, ldx, dt, pdt, act, slope, sinks = ctx.meta
-        need_x, need_g, need_b = ctx.needs_input_grad[:3]
+        rows, c, width, ldx, dt, pdt, act, slope, sinks = ctx.meta
+        need_x, need_g, need_b, _ = ctx.needs_input_grad
         dy, ldy = _rows(dy)
-        rows = stat.numel() // 2
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
+        dx = _dense_like(x) if need_x else None
         acc, dg, db = 0, None, None
         if sinks is not None and (need_g or need_b):
             dg, db, acc = sinks[0] if need_g else None, sinks[1] if need_b else None, ACC_DW
@@ -1244,12 +1255,11 @@ class _LayerNorm(torch.autograd.Function):
                 n = _lib.fn("itg_layer_norm_bwd_workspace")(rows, c)
                 ws = torch.empty(n, device=x.device, dtype=torch.float32)
             at = [t.data_ptr() if t is not None else None for t in (x, dy, stat, gamma, beta, dx, dg, db, ws)]
-            with _on(x):
-                _lib.call("itg_layer_norm_bwd", at[0], ldx, at[1], ldy, at[2], at[3], at[4], at[5], width, at[6], at[7], acc, rows, c,
-                          width - c, dt, pdt, act, slope, at[8], n, _stream())
+            _call_on(x.get_device(), "itg_layer_norm_bwd", at[0], ldx, at[1], ldy, at[2], at[3], at[4], at[5], width, at[6], at[7], acc,
+                     rows, c, width - c, dt, pdt, act, slope, at[8], n)
         elif not acc:
             dg, db = (t.zero_() if t is not None else None for t in (dg, db))
-        return (dx, None, None, None, None, None, None, None) if acc else (dx, dg, db, None, None, None, None, None)
+        return (dx, None, None, None) if acc else (dx, dg, db, None)
 
 
 def layer_norm(x, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, slope=0.0, sinks=None):
@@ -1281,7 +1291,7 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, slope=0.0, sink
                                                                    or not s.is_contiguous() or s.device != t.device for s in sinks)):
         raise _lib.ItgError("layer_norm: sinks are two contiguous buffers like gamma and beta")
     if torch.is_grad_enabled() and (t.requires_grad or (gamma is not None and gamma.requires_grad) or (beta is not None and beta.requires_grad)):
-        y = _LayerNorm.apply(t, gamma, beta, c, float(eps), int(act), float(slope), sinks)
+        y = _LayerNorm.apply(t, gamma, beta, (c, float(eps), int(act), float(slope), sinks))
     else:      # no tape: a quarter of the host's time for a call
         y = _ln_forward(*_rows(t), gamma, beta, c, float(eps), int(act), float(slope), False)[0]
     return GT(y, c) if grid else y
