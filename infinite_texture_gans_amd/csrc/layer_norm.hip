@@ -159,6 +159,19 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return s;
 }
 
+// two sums at once, `red` = 2 TPR / 64 floats, one barrier
+template <int TPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* red) {
+  a = group_sum<(TPR < 64 ? TPR : 64)>(a);
+  b = group_sum<(TPR < 64 ? TPR : 64)>(b);
+  if (TPR <= 64) return;
+  if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = a; red[TPR / 64 + (threadIdx.x >> 6)] = b; }
+  __syncthreads();
+  a = b = 0.f;
+#pragma unroll
+  for (int k = 0; k < (TPR > 64 ? TPR / 64 : 1); ++k) { a += red[k]; b += red[TPR / 64 + k]; }
+}
+
 // a thread's row among those of its workgroup; from a wave per row on the same in every lane, and known to be: addresses then are a
 // scalar base and 32 bits a lane
 template <int TPR> __device__ __forceinline__ int ln_group() {
@@ -337,7 +350,9 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
     // the next row is on its way while this one is reduced and written
     if (!TIGHT && row + step < p.rows) fetch(row + step);
     if (p.y) {
-      const float m1 = row_sum<TPR>(s1, red[flip]) * inv, m2 = row_sum<TPR>(s2, red[flip + 1]) * inv;
+      if (TIGHT) { s1 = row_sum<TPR>(s1, red[flip]); s2 = row_sum<TPR>(s2, red[flip + 1]); }      // (both at once spill there)
+      else row_sum2<TPR>(s1, s2, red[flip]);
+      const float m1 = s1 * inv, m2 = s2 * inv;
       T* dx = (T*)p.y + row * p.ldy;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -474,7 +489,8 @@ __global__ __launch_bounds__(LN_ANY) void ln_dx_any_kernel(LnP p) {
         s1 += g; s2 = fmaf(g, xh, s2);
       }
     });
-    const float m1 = row_sum<LN_ANY>(s1, red[flip]) * inv, m2 = row_sum<LN_ANY>(s2, red[flip + 1]) * inv;
+    row_sum2<LN_ANY>(s1, s2, red[flip]);
+    const float m1 = s1 * inv, m2 = s2 * inv;
     T* dx = (T*)p.y + row * p.ldy;
     ln_sweep<V>(p.c, [&](int at, auto width) {
       constexpr int N = decltype(width)::value;
