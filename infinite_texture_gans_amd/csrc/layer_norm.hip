@@ -263,13 +263,13 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
 }
 
 // dx, and this workgroup's share of dw | db (`part`), which a thread sums over the rows it sees for the channels it holds.
-// From 16 channels a thread on (R V = 16, rows of 8193 .. 16384 16-bit values) the row stays in its own 16 bits between the two
+// At 16 channels in each of 1024 threads (rows of 8193 .. 16384 16-bit values) the row stays in its own 16 bits between the two
 // sweeps and gamma in its own type, and the next row is fetched behind the last sweep: fp32 copies and a row under way do not fit
 // the 128 registers that 1024 threads have (4096 x 12288 bf16: 88 us, swept three times by the kernels for any length 142).
 template <typename T, typename W, int V, int TPR, int R, int KIND>
 __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
   constexpr int NT = TPR > 64 ? TPR : 256, GROUPS = NT / TPR;
-  constexpr bool TIGHT = R * V >= 16, MASK = KIND != LN_PLAIN, ACT = KIND == LN_ACT;
+  constexpr bool TIGHT = R * V >= 16 && TPR == 1024, MASK = KIND != LN_PLAIN, ACT = KIND == LN_ACT;
   __shared__ float red[4][TPR > 64 ? TPR / 64 : 1];
   const LnV lv = ln_vectors(p.c, p.pad, V);
   const int tid = TPR > 64 ? threadIdx.x : threadIdx.x % TPR;
@@ -589,8 +589,9 @@ int ln_fwd_run(const LnP& p, hipStream_t s) {
 }
 
 // Threads per row and vectors per thread: as few threads as hold the row at one vector each up to a wave; beyond, workgroups of
-// 128 .. 1024 threads at two vectors each (backward: at one vector of 8 or two of 4, as it keeps six values per channel it holds;
-// at two of 8 its row stays in 16 bits, see there).
+// 128 .. 1024 threads at two vectors each.  Backward: up to two vectors in a wave (65536 x 1023 bf16 96 us, in two waves of one each
+// 120, where 1024 shares of dw | db are 8 waves a CU), then one of 8 or two of 4, as it keeps six values per channel it holds; at
+// two of 8 its row stays in 16 bits, see there.
 template <typename T, typename W>
 int ln_fwd_t(const LnP& p, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
@@ -645,8 +646,8 @@ int ln_bwd_t(LnP p, void* dw, void* db, int acc, hipStream_t s) {
   else if (nv <= 16) rc = ln_bwd_run<T, W, V, 16, 1>(p, chunks, s);
   else if (nv <= 32) rc = ln_bwd_run<T, W, V, 32, 1>(p, chunks, s);
   else if (nv <= 64) rc = ln_bwd_run<T, W, V, 64, 1>(p, chunks, s);
-  else if (nv <= 64 * K) rc = ln_bwd_run<T, W, V, 64, K>(p, chunks, s);
-  else if (nv <= 128 * K) rc = ln_bwd_run<T, W, V, 128, K>(p, chunks, s);
+  else if (nv <= 128) rc = ln_bwd_run<T, W, V, 64, 2>(p, chunks, s);
+  else if (K == 2 && nv <= 256) rc = ln_bwd_run<T, W, V, K == 2 ? 128 : 256, K>(p, chunks, s);
   else if (nv <= 256 * K) rc = ln_bwd_run<T, W, V, 256, K>(p, chunks, s);
   else if (nv <= 512 * K) rc = ln_bwd_run<T, W, V, 512, K>(p, chunks, s);
   else if (nv <= 1024 * K && !few) rc = ln_bwd_run<T, W, V, 1024, K>(p, chunks, s);
