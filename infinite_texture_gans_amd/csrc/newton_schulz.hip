@@ -297,13 +297,13 @@ template <int T> __device__ __forceinline__ f16x8 frag_t(const _Float16* at) {
   return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// T: tile; WR x WC waves share it, each with FR x FC fragments of 16 x 16
-template <int T_, bool SPLIT> struct Tile {
-  static constexpr int T = T_, WR = 2, WC = T_ == 256 ? 4 : 2, WAVES = WR * WC, NT = WAVES * 64;
-  static constexpr int FR = T / WR / 16, FC = T / WC / 16;
+// T: tile, TR x T where TALL; WR x WC waves share it, each with FR x FC fragments of 16 x 16
+template <int T_, bool SPLIT, bool TALL = false> struct Tile {
+  static constexpr int T = T_, TR = TALL ? 2 * T_ : T_, WR = 2, WC = T_ == 256 ? 4 : 2, WAVES = WR * WC, NT = WAVES * 64;
+  static constexpr int FR = TR / WR / 16, FC = T / WC / 16;
   static constexpr int NP = SPLIT ? 2 : 1, BK = SPLIT ? 32 : 64;
-  static constexpr int PLANE = T * BK, BUF = 2 * NP * PLANE;            // halves: one operand plane, one buffer
-  static constexpr int LP = PLANE * 2 / 1024 / WAVES;                    // loads of a wave per plane
+  static constexpr int PP = TR * BK, PQ = T * BK, BUF = NP * (PP + PQ);      // halves: a plane of each operand, one buffer
+  static constexpr int LP = PP * 2 / 1024 / WAVES, LQ = PQ * 2 / 1024 / WAVES;      // loads of a wave per plane
 };
 
 template <typename C>
@@ -322,29 +322,33 @@ __device__ __forceinline__ void acc_zero(Acc<C>& a) {
 // TURN: P[plane] holds the operand by column (row k of it at k * ldp)
 template <typename C, bool SPLIT, int DEPTH, bool TURN>
 __device__ __forceinline__ void ns_product(Acc<C>& acc, const _Float16* const* P, int ldp, const _Float16* const* Q, int ldq, int k0, int k1, _Float16* lds) {
-  constexpr int BK = C::BK, NP = C::NP, T = C::T, CH = BK / 8, ROWS = 64 / CH, CHT = T / 8, ROWST = 64 / CHT;
+  constexpr int BK = C::BK, NP = C::NP, T = C::T, TR = C::TR, CH = BK / 8, ROWS = 64 / CH, CHT = TR / 8, ROWST = 64 / CHT;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l15 = lane & 15, lk = lane >> 4;
-  uint32_t from_p[C::LP], from_q[C::LP];                   // bytes from a slice's first value to what this lane fetches
+  uint32_t from_p[C::LP], from_q[C::LQ];                   // bytes from a slice's first value to what this lane fetches
 #pragma unroll
   for (int u = 0; u < C::LP; ++u) {
     const int r = (wave * C::LP + u) * ROWS + lane / CH, rt = (wave * C::LP + u) * ROWST + lane / CHT;
+    from_p[u] = TURN ? (uint32_t)(rt * ldp + slot_t<TR>(rt, lane % CHT) * 8) * 2u : (uint32_t)(r * ldp + slot<BK>(r, lane % CH) * 8) * 2u;
+  }
+#pragma unroll
+  for (int u = 0; u < C::LQ; ++u) {
+    const int r = (wave * C::LQ + u) * ROWS + lane / CH;
     from_q[u] = (uint32_t)(r * ldq + slot<BK>(r, lane % CH) * 8) * 2u;
-    from_p[u] = TURN ? (uint32_t)(rt * ldp + slot_t<T>(rt, lane % CHT) * 8) * 2u : (uint32_t)(r * ldp + slot<BK>(r, lane % CH) * 8) * 2u;
   }
   auto stage = [&](int buf, int k) {
+    auto fetch = [&](const _Float16* from, const uint32_t* off, int n, _Float16* to) {
 #pragma unroll
-    for (int o = 0; o < 2; ++o)
+      for (int u = 0; u < n; ++u)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((const char*)from + off[u]),
+                                         (__attribute__((address_space(3))) void*)(to + u * 512), 16, 0, 0);
+    };
 #pragma unroll
-      for (int q = 0; q < NP; ++q) {
-        const char* base = (const char*)(o ? Q[q] + k : TURN ? P[q] + (int64_t)k * ldp : P[q] + k);
-        _Float16* to = lds + buf * C::BUF + (o * NP + q) * C::PLANE + wave * C::LP * 512;
+    for (int q = 0; q < NP; ++q)
+      fetch(TURN ? P[q] + (int64_t)k * ldp : P[q] + k, from_p, C::LP, lds + buf * C::BUF + q * C::PP + wave * C::LP * 512);
 #pragma unroll
-        for (int u = 0; u < C::LP; ++u)
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + (o ? from_q[u] : from_p[u])),
-                                           (__attribute__((address_space(3))) void*)(to + u * 512), 16, 0, 0);
-      }
+    for (int q = 0; q < NP; ++q) fetch(Q[q] + k, from_q, C::LQ, lds + buf * C::BUF + NP * C::PP + q * C::PQ + wave * C::LQ * 512);
   };
-  const int wr = (wave / C::WC) * (T / C::WR), wc = (wave % C::WC) * (T / C::WC);
+  const int wr = (wave / C::WC) * (TR / C::WR), wc = (wave % C::WC) * (T / C::WC);
   const int row_q = (wc + l15) * BK;
   int at_p[C::FR], ch[BK / 32];
 #pragma unroll
@@ -352,7 +356,7 @@ __device__ __forceinline__ void ns_product(Acc<C>& acc, const _Float16* const* P
 #pragma unroll
   for (int i = 0; i < C::FR; ++i) {
     const int r = lk * 8 + (l15 >> 2);
-    at_p[i] = TURN ? r * T + slot_t<T>(r, wr / 8 + 2 * i + ((l15 >> 1) & 1)) * 8 + (l15 & 1) * 4 : (wr + i * 16 + l15) * BK;
+    at_p[i] = TURN ? r * TR + slot_t<TR>(r, wr / 8 + 2 * i + ((l15 >> 1) & 1)) * 8 + (l15 & 1) * 4 : (wr + i * 16 + l15) * BK;
   }
   // split: sums in two levels, a fresh accumulator every 256 of K.  One accumulator over all of K drifts: each MFMA adds to it
   // with an error of one step of the sum, and on the diagonal of X X^T, a sum of squares, these do not cancel (a 1 x 4099 matrix:
@@ -363,7 +367,7 @@ __device__ __forceinline__ void ns_product(Acc<C>& acc, const _Float16* const* P
   if (SPLIT) acc_zero(part);
   Acc<C>& run = SPLIT ? part : acc;
   const int nk = (k1 - k0) / BK;
-  constexpr int LOADS = 2 * NP * C::LP;                    // of a wave per buffer
+  constexpr int LOADS = NP * (C::LP + C::LQ);              // of a wave per buffer
   struct Frags { f16x8 p[NP][C::FR], q[NP][C::FC]; };
   auto read = [&](int buf, int ks, Frags& f) {
     const _Float16* at = lds + buf * C::BUF;
@@ -371,9 +375,9 @@ __device__ __forceinline__ void ns_product(Acc<C>& acc, const _Float16* const* P
     for (int q = 0; q < NP; ++q) {
 #pragma unroll
       for (int i = 0; i < C::FR; ++i)
-        f.p[q][i] = TURN ? frag_t<T>(at + q * C::PLANE + at_p[i] + ks * 32 * T) : *reinterpret_cast<const f16x8*>(at + q * C::PLANE + at_p[i] + ch[ks]);
+        f.p[q][i] = TURN ? frag_t<TR>(at + q * C::PP + at_p[i] + ks * 32 * TR) : *reinterpret_cast<const f16x8*>(at + q * C::PP + at_p[i] + ch[ks]);
 #pragma unroll
-      for (int k = 0; k < C::FC; ++k) f.q[q][k] = *reinterpret_cast<const f16x8*>(at + (NP + q) * C::PLANE + row_q + ch[ks] + k * 16 * BK);
+      for (int k = 0; k < C::FC; ++k) f.q[q][k] = *reinterpret_cast<const f16x8*>(at + NP * C::PP + q * C::PQ + row_q + ch[ks] + k * 16 * BK);
     }
   };
   // lo hi, hi lo, hi hi: each over all fragments, so that no product waits for the one before it
@@ -475,7 +479,7 @@ struct Addend {
   __device__ __forceinline__ void load(const NsMat& j, const NsWs& w, int ti, int tj, int gen, int i0) {
     if (PH == PH_A) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int rbase = ti * C::T + (wave / C::WC) * (C::T / C::WR) + i0 * 16 + (lane >> 4) * 4, cbase = tj * C::T + (wave % C::WC) * (C::T / C::WC) + (lane & 15);
+    const int rbase = ti * C::TR + (wave / C::WC) * (C::TR / C::WR) + i0 * 16 + (lane >> 4) * 4, cbase = tj * C::T + (wave % C::WC) * (C::T / C::WC) + (lane & 15);
     const _Float16* hi = PH == PH_B ? w.a[0] : w.x[gen][0];
     const _Float16* lo = PH == PH_B ? w.a[1] : w.x[gen][1];
     const int64_t ld = PH == PH_B ? j.mp : j.np;
@@ -504,7 +508,7 @@ template <typename C, bool SPLIT, int PH, typename OUT, bool MUON, int N>
 __device__ __forceinline__ void ns_write_rows(const f32x4 (*acc)[C::FC], int i0, const Addend<C, SPLIT, PH, N>& ad, _Float16* lds, const NsArgs& p,
                                               const NsMat& j, const NsWs& w, int z, int ti, int tj, int gen, float ca, float cb, float cc) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, lk = lane >> 4;
-  const int r0 = ti * C::T + (wave / C::WC) * (C::T / C::WR) + i0 * 16, c0 = tj * C::T + (wave % C::WC) * (C::T / C::WC);
+  const int r0 = ti * C::TR + (wave / C::WC) * (C::TR / C::WR) + i0 * 16, c0 = tj * C::T + (wave % C::WC) * (C::T / C::WC);
   f16x4 hi[N][C::FC], lo[N][C::FC];
 #pragma unroll
   for (int i = 0; i < N; ++i)
@@ -566,15 +570,15 @@ __device__ __forceinline__ void ns_write_rows(const f32x4 (*acc)[C::FC], int i0,
 }
 
 // matrix z and tile (ti, tj) of tile `local` of a job
-template <int T, int PH>
+template <int T, int TR, int PH>
 __device__ __forceinline__ void ns_tile(const NsMat& j, int local, int& z, int& ti, int& tj) {
   const int nt = j.mp / T;
   if (PH >= PH_X) {
-    const int per = nt * (j.np / T);
+    const int per = nt * (j.np / TR);
     z = local / per; local -= z * per;
     // rows: X's columns, columns: X's rows.  Bands of 8 tile rows: the tiles a die works on at a time form a square, which reads
     // the fewest operand rows
-    const int nr = j.np / T, band = local / (8 * nt), in = local - band * 8 * nt, high = nr - band * 8 < 8 ? nr - band * 8 : 8;
+    const int nr = j.np / TR, band = local / (8 * nt), in = local - band * 8 * nt, high = nr - band * 8 < 8 ? nr - band * 8 : 8;
     tj = in / high; ti = band * 8 + (in - tj * high);
   } else {
     const int per = nt * (nt + 1) / 2;
@@ -587,9 +591,9 @@ __device__ __forceinline__ void ns_tile(const NsMat& j, int local, int& z, int& 
 
 // One workgroup per tile, or, of the tiles behind direct[], per share of a tile's K, which goes to the slab: the tiles of a small
 // call do not fill the chip, and neither do those that are left over from its last full round.
-template <int T, bool SPLIT, int DEPTH, int PH, typename OUT, bool MUON>
+template <int T, bool SPLIT, bool TALL, int DEPTH, int PH, typename OUT, bool MUON>
 __global__ __launch_bounds__((Tile<T, SPLIT>::NT), 2) void ns_gemm_kernel(NsArgs p, int gen, float ca, float cb, float cc) {
-  typedef Tile<T, SPLIT> C;
+  typedef Tile<T, SPLIT, TALL> C;
   constexpr int Q3 = PH < PH_X ? PH : 2;
   extern __shared__ __attribute__((aligned(16))) _Float16 lds[];
   const int direct = p.direct[Q3], bid = blockIdx.x;
@@ -614,13 +618,13 @@ __global__ __launch_bounds__((Tile<T, SPLIT>::NT), 2) void ns_gemm_kernel(NsArgs
   }
   const NsMat& j = p.j[job];
   int z, ti, tj;
-  ns_tile<T, PH>(j, tile, z, ti, tj);
+  ns_tile<T, C::TR, PH>(j, tile, z, ti, tj);
   const NsWs w = ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np, SPLIT);
   const int ld = PH == PH_A ? j.np : j.mp;                 // of the second operand, and K
   const _Float16* P[2]; const _Float16* Q[2];
 #pragma unroll
   for (int q = 0; q < C::NP; ++q) {
-    P[q] = PH >= PH_X ? w.x[gen][q] + ti * T : (PH == PH_A ? w.x[gen][q] : w.a[q]) + (int64_t)ti * T * ld;
+    P[q] = PH >= PH_X ? w.x[gen][q] + ti * C::TR : (PH == PH_A ? w.x[gen][q] : w.a[q]) + (int64_t)ti * T * ld;
     Q[q] = (PH == PH_A ? w.x[gen][q] : PH == PH_B ? w.a[q] : w.b[q]) + (int64_t)tj * T * ld;
   }
   int k0 = 0, k1 = ld;
@@ -633,10 +637,10 @@ __global__ __launch_bounds__((Tile<T, SPLIT>::NT), 2) void ns_gemm_kernel(NsArgs
   constexpr int N = T == 256 ? 4 : 2;
   Acc<C> acc;
   Addend<C, SPLIT, PH, N> ad;
-  if (T == 64 && whole) ad.load(j, w, ti, tj, gen, 0);
+  if (C::FR == N && whole) ad.load(j, w, ti, tj, gen, 0);
   ns_product<C, SPLIT, DEPTH, (PH >= PH_X)>(acc, P, PH >= PH_X ? j.np : ld, Q, ld, k0, k1, lds);
   if (whole) {
-    if (T != 64) ad.load(j, w, ti, tj, gen, 0);
+    if (C::FR != N) ad.load(j, w, ti, tj, gen, 0);
     __syncthreads();                                       // the slices in LDS have been read: it turns the results now
     ns_write_rows<C, SPLIT, PH, OUT, MUON, N>(acc.v, 0, ad, lds, p, j, w, z, ti, tj, gen, ca, cb, cc);
     if (C::FR > N) {
@@ -644,7 +648,7 @@ __global__ __launch_bounds__((Tile<T, SPLIT>::NT), 2) void ns_gemm_kernel(NsArgs
       ns_write_rows<C, SPLIT, PH, OUT, MUON, N>(acc.v + C::FR - N, N, ad, lds, p, j, w, z, ti, tj, gen, ca, cb, cc);
     }
   } else {
-    f32x4* to = reinterpret_cast<f32x4*>(p.slab) + (int64_t)slot_at * (T * T / 4) + threadIdx.x;
+    f32x4* to = reinterpret_cast<f32x4*>(p.slab) + (int64_t)slot_at * (C::TR * T / 4) + threadIdx.x;
 #pragma unroll
     for (int i = 0; i < C::FR; ++i)
 #pragma unroll
@@ -653,18 +657,18 @@ __global__ __launch_bounds__((Tile<T, SPLIT>::NT), 2) void ns_gemm_kernel(NsArgs
 }
 
 // the split tiles: their shares added in order, then as any other tile; a workgroup per row of fragments
-template <int T, bool SPLIT, int PH, typename OUT, bool MUON>
+template <int T, bool SPLIT, bool TALL, int PH, typename OUT, bool MUON>
 __global__ __launch_bounds__((Tile<T, SPLIT>::NT)) void ns_join_kernel(NsArgs p, int gen, float ca, float cb, float cc) {
-  typedef Tile<T, SPLIT> C;
+  typedef Tile<T, SPLIT, TALL> C;
   constexpr int Q3 = PH < PH_X ? PH : 2;
   const int direct = p.direct[Q3], t = direct + blockIdx.x / C::FR, i = blockIdx.x % C::FR;
   const NsMat& j = p.j[ns_job(p, t, [](const NsMat& q) { return q.tile0[Q3]; })];
   const int first = j.tile0[Q3] > direct ? j.tile0[Q3] : direct, n = j.shares[Q3];
-  const f32x4* from = reinterpret_cast<const f32x4*>(p.slab) + (int64_t)(j.share0[Q3] + t - first) * (T * T / 4) + i * C::FC * C::NT + threadIdx.x;
-  const int64_t next = (int64_t)j.cut[Q3] * (T * T / 4);
+  const f32x4* from = reinterpret_cast<const f32x4*>(p.slab) + (int64_t)(j.share0[Q3] + t - first) * (C::TR * T / 4) + i * C::FC * C::NT + threadIdx.x;
+  const int64_t next = (int64_t)j.cut[Q3] * (C::TR * T / 4);
   __shared__ __attribute__((aligned(16))) _Float16 lds[C::WAVES * ns_turn<1, C::FC>()];
   int z, ti, tj;
-  ns_tile<T, PH>(j, t - j.tile0[Q3], z, ti, tj);
+  ns_tile<T, C::TR, PH>(j, t - j.tile0[Q3], z, ti, tj);
   const NsWs w = ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np, SPLIT);
   Addend<C, SPLIT, PH, 1> ad;
   ad.load(j, w, ti, tj, gen, i);
@@ -681,9 +685,9 @@ __global__ __launch_bounds__((Tile<T, SPLIT>::NT)) void ns_join_kernel(NsArgs p,
 #include "newton_schulz_thin.h"
 
 // ---- host side
-// launches of a call: workgroups of norm and conversion; per product its tile size, workgroups (whole tiles and shares) and split tiles
+// launches of a call: workgroups of norm and conversion; per product its tile size (TR: columns of X in a tile of product X), workgroups (whole tiles and shares) and split tiles
 // thin: 0, or the short side that newton_schulz_thin.h holds; blocks: its workgroups; one: a matrix is one block
-struct NsPlan { int64_t bytes, norm, conv; int T[3]; int64_t grid[3], join[3]; int thin; int64_t blocks; bool one; };
+struct NsPlan { int64_t bytes, norm, conv; int T[3], TR; int64_t grid[3], join[3]; int thin; int64_t blocks; bool one; };
 
 inline int64_t up(int64_t v, int64_t k) { return (v + k - 1) / k * k; }
 
@@ -692,16 +696,20 @@ inline int64_t up(int64_t v, int64_t k) { return (v + k - 1) / k * k; }
 //   only: split has no registers for it) from a full round of 256 tiles on (4096 x 8192 bf16: 3207 -> 3056 us).
 // A and B, whose leftover tiles are split along K, go by tiles x K: split 128 from 192 K on (1024 x 8192, A 288 K: 712 -> 673 us;
 //   4 x 1024 x 1024, 144 K: 634 -> 642), single from 400 K on (1536 x 6144, A 468 K: 626 -> 598 us; 1024 x 8192, 288 K: 406 -> 413).
+//   Split at 64 takes tiles of 128 columns of X by 64 rows where they make 512 or more: a third less of LDS and cache traffic for a
+//   product (the default generator's matrices, a Muon step: 417 -> 392 us; 2048 x 2048 835 -> 811; 512 x 4096, 256 such tiles:
+//   217 -> 246; single, 2048 x 2048: 441 -> 450).
 // A size whose padding adds more than an eighth to the planes is not taken (the default generator's matrices of 3 to 416 rows: 448 us
 // a Muon step with X at 128, 430 without).
 void ns_tile_sizes(const NsArgs& p, bool split, NsPlan& pl) {
-  int64_t a = 0, b = 0, x = 0, x64 = 0, x256 = 0;
+  int64_t a = 0, b = 0, x = 0, x64 = 0, x256 = 0, tall = 0;
   for (int i = 0; i < p.n; ++i) {
     const NsMat& j = p.j[i];
     const int64_t m = up(j.m, 128) / 128, n = up(j.n, 128) / 128, sym = m * (m + 1) / 2 * j.count;
     a += sym * n * 128;
     b += sym * m * 128;
     x += m * n * j.count;
+    tall += up(j.m, 64) / 64 * n * j.count;
     x64 += up(j.m, 64) / 64 * (up(j.n, 64) / 64) * j.count;
     x256 += ((m + 1) / 2) * ((n + 1) / 2) * j.count;
   }
@@ -710,6 +718,7 @@ void ns_tile_sizes(const NsArgs& p, bool split, NsPlan& pl) {
   pl.T[0] = fits && a >= least ? 128 : 64;
   pl.T[1] = fits && b >= least ? 128 : 64;
   pl.T[2] = !split && fits256 && x256 >= 256 ? 256 : fits && x >= 384 ? 128 : 64;
+  pl.TR = split && pl.T[2] == 64 && 16 * tall <= 9 * x64 && tall >= 512 ? 128 : pl.T[2];
 }
 
 // Tiles and shares of product q (A, B, X).  `slots` workgroups run at a time; whole rounds of them take a tile each, and what is
@@ -719,7 +728,7 @@ int ns_tiles(NsArgs& p, NsPlan& pl, int q, int64_t& slab) {
   int64_t tiles = 0;
   for (int i = 0; i < p.n; ++i) {
     NsMat& j = p.j[i];
-    const int64_t nt = j.mp / T, nx = j.np / T;
+    const int64_t nt = j.mp / T, nx = j.np / pl.TR;
     j.tile0[q] = (int)tiles;
     tiles += (q == 2 ? nt * nx : nt * (nt + 1) / 2) * j.count;
     if (tiles >= ((int64_t)1 << (T == 256 ? 23 : 24))) return ITG_ERR_ARG;
@@ -748,7 +757,8 @@ int ns_tiles(NsArgs& p, NsPlan& pl, int q, int64_t& slab) {
   p.direct[q] = (int)direct;
   pl.grid[q] = direct + shares;
   pl.join[q] = rest;
-  if (shares * T * T * 4 > slab) slab = shares * T * T * 4;
+  const int64_t each = (int64_t)(q == 2 ? pl.TR : T) * T * 4;
+  if (shares * each > slab) slab = shares * each;
   return ITG_OK;
 }
 
@@ -828,7 +838,7 @@ int ns_plan(const itg_ns_job* jobs, int n, bool split, bool muon, NsArgs& p, NsP
   for (int i = 0; i < n; ++i) {
     const itg_ns_job& q = jobs[i];
     NsMat& j = p.j[i];
-    j.mp = (int)up(j.m, T); j.np = (int)up(j.n, T);
+    j.mp = (int)up(j.m, T); j.np = (int)up(j.n, T > pl.TR ? T : pl.TR);
     ns_job_fields(q, j);
     j.norm0 = (int)pl.norm; j.conv0 = (int)pl.conv;
     pl.norm += (int64_t)j.nblk * j.count;
@@ -873,15 +883,15 @@ int ns_lds(K kernel, int bytes) {
              ? ITG_OK : ITG_ERR_LAUNCH;
 }
 
-template <int T, bool SPLIT, int DEPTH, int PH, typename OUT, bool MUON>
+template <int T, bool SPLIT, int DEPTH, int PH, typename OUT, bool MUON, bool TALL = false>
 int ns_launch(const NsArgs& p, const NsPlan& pl, int gen, const float* abc, hipStream_t s) {
-  typedef Tile<T, SPLIT> C;
+  typedef Tile<T, SPLIT, TALL> C;
   constexpr int Q3 = PH < PH_X ? PH : 2, LDS = DEPTH * C::BUF * 2;
-  if (ns_lds(&ns_gemm_kernel<T, SPLIT, DEPTH, PH, OUT, MUON>, LDS)) return ITG_ERR_LAUNCH;
-  hipLaunchKernelGGL((ns_gemm_kernel<T, SPLIT, DEPTH, PH, OUT, MUON>), dim3((unsigned)pl.grid[Q3]), dim3(C::NT), LDS, s, p, gen, abc[0], abc[1], abc[2]);
+  if (ns_lds(&ns_gemm_kernel<T, SPLIT, TALL, DEPTH, PH, OUT, MUON>, LDS)) return ITG_ERR_LAUNCH;
+  hipLaunchKernelGGL((ns_gemm_kernel<T, SPLIT, TALL, DEPTH, PH, OUT, MUON>), dim3((unsigned)pl.grid[Q3]), dim3(C::NT), LDS, s, p, gen, abc[0], abc[1], abc[2]);
   ITG_CHECK_LAUNCH();
   if (pl.join[Q3]) {
-    hipLaunchKernelGGL((ns_join_kernel<T, SPLIT, PH, OUT, MUON>), dim3((unsigned)(pl.join[Q3] * C::FR)), dim3(C::NT), 0, s, p, gen, abc[0], abc[1], abc[2]);
+    hipLaunchKernelGGL((ns_join_kernel<T, SPLIT, TALL, PH, OUT, MUON>), dim3((unsigned)(pl.join[Q3] * C::FR)), dim3(C::NT), 0, s, p, gen, abc[0], abc[1], abc[2]);
     ITG_CHECK_LAUNCH();
   }
   return ITG_OK;
@@ -893,6 +903,7 @@ int ns_phase(const NsArgs& p, const NsPlan& pl, int gen, const float* abc, hipSt
   const int64_t grid = pl.grid[PH < PH_X ? PH : 2];
   // 64: four buffers while two workgroups a CU take the whole launch (2 x 333 x 1501 bf16: 156 us against 162 with two), two buffers
   // and up to five workgroups a CU beyond
+  if (PH >= PH_X && T == 64 && pl.TR == 128) return ns_launch<64, SPLIT, 2, PH, OUT, MUON, SPLIT && PH >= PH_X>(p, pl, gen, abc, s);
   if (T == 64 && grid <= 512) return ns_launch<64, SPLIT, 4, PH, OUT, MUON>(p, pl, gen, abc, s);
   if (T == 64) return ns_launch<64, SPLIT, 2, PH, OUT, MUON>(p, pl, gen, abc, s);
   if (SPLIT || T == 128) return ns_launch<128, SPLIT, 2, PH, OUT, MUON>(p, pl, gen, abc, s);

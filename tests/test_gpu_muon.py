@@ -296,3 +296,14 @@ def test_long_batches_of_tiny_matrices(ops):
     o = ops.orthogonalize(g)
     for k in (0, 1, 99999, 199999):
         assert torch.equal(o[k], ops.orthogonalize(g[k]))
+
+
+@pytest.mark.parametrize("t,m,n,batch", [("f32", 200, 5000, 6), ("f32", 1000, 4100, 1), ("f16", 130, 1400, 33), ("f32", 1900, 450, 5), ("f32", 1930, 1930, 1)])
+def test_tall_tiles(ops, t, m, n, batch):
+    """calls of 512 and more tiles of 128 columns by 64 rows, with columns behind the last whole tile, alone and split along K"""
+    g = torch.stack([matrix(m, n, seed=s) for s in range(batch)]).cuda().to(TYPES[t])
+    got = ops.orthogonalize(g)
+    for z in range(batch):
+        want, own = steps_of(g[z].double()), steps_of(g[z].float().cpu()).cuda()
+        off, own = rel(got[z], want), rel(own, want)
+        assert off <= 3 * own + (2.0 ** -11 if t == "f16" else 0.0), (z, off, own)
