@@ -440,3 +440,33 @@ def test_many_long_rows_over_the_inputs(ops, t, dt):
         ew, eb = torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
         bwd(a, g, a if over == "x" else g, ew, eb)
         assert torch.equal(a if over == "x" else g, dx) and torch.equal(ew, dw) and torch.equal(eb, db), over
+
+
+def test_more_than_2_31_values(ops):
+    """a contiguous tensor whose later rows lie past 2^31 values: each row as it is alone, the weights' gradients as from its halves"""
+    rows, c = (1 << 20) + 5, 2056
+    x = torch.empty(rows, c, device="cuda", dtype=torch.bfloat16)
+    block = torch.randn(1 << 12, c, device="cuda").bfloat16()
+    for k in range(0, rows, 1 << 12):
+        x[k:k + (1 << 12)] = block[:min(1 << 12, rows - k)]
+    x[-5:] = torch.randn(5, c, device="cuda").bfloat16()
+    w, b = torch.randn(c, device="cuda", requires_grad=True), torch.randn(c, device="cuda", requires_grad=True)
+    xs = x.requires_grad_()
+    y = ops.layer_norm(xs, w, b)
+    dx, dw, db = torch.autograd.grad(y, [xs, w, b], x.detach())
+    tail = x.detach()[-4101:].clone().requires_grad_()
+    yt = ops.layer_norm(tail, w, b)
+    dt, = torch.autograd.grad(yt, tail, tail.detach())
+    assert torch.equal(y[-4101:], yt) and torch.equal(dx[-4101:], dt)
+    first = x.detach()[:1 << 12].clone().requires_grad_()
+    yf = ops.layer_norm(first, w, b)
+    df, fw, fb = torch.autograd.grad(yf, [first, w, b], first.detach())
+    assert torch.equal(y[:1 << 12], yf) and torch.equal(dx[:1 << 12], df)
+    last = x.detach()[-5:].clone().requires_grad_()
+    _, lw, lb = torch.autograd.grad(ops.layer_norm(last, w, b), [last, w, b], last.detach())
+    # 256 blocks of the same rows, and five.  A channel's fp32 sum of 2^20 terms passes through at most 600 additions in a row (4096
+    # rows a workgroup's share in four groups, 1024 shares in 64 lanes), the block's through fewer: 600 half steps of the sum of
+    # the terms' sizes each, which is below 1.2 a row for normal values over 4096 different rows
+    for whole, f, l in ((dw, fw, lw), (db, fb, lb)):
+        want = 256 * f.double() + l.double()
+        assert float((whole.double() - want).abs().max()) <= 2 * 600 * 2.0 ** -24 * 1.2 * rows

@@ -307,3 +307,28 @@ def test_tall_tiles(ops, t, m, n, batch):
         want, own = steps_of(g[z].double()), steps_of(g[z].float().cpu()).cuda()
         off, own = rel(got[z], want), rel(own, want)
         assert off <= 3 * own + (2.0 ** -11 if t == "f16" else 0.0), (z, off, own)
+
+
+def test_offsets_past_2_31(ops):
+    """matrices more than 2^31 values apart, rows more than 2^31 / 64 apart, and filters behind 2^31 values of a flat buffer"""
+    big = torch.empty((1 << 32) + (1 << 28), device="cuda", dtype=torch.bfloat16)          # (written only where the matrices lie)
+    far = torch.as_strided(big, (2, 70, 130), ((1 << 32) + 7, 130, 1))
+    near = torch.randn(2, 70, 130, device="cuda").bfloat16()
+    far.copy_(near)
+    assert torch.equal(ops.orthogonalize(far), ops.orthogonalize(near))
+    wide = torch.as_strided(big, (66, 200), ((1 << 26) + 3, 1))
+    flat = torch.randn(66, 200, device="cuda").bfloat16()
+    wide.copy_(flat)
+    assert torch.equal(ops.orthogonalize(wide), ops.orthogonalize(flat))
+    del big, far, wide
+    shapes, at = [(64, 48), (130, 300)], (1 << 31) + 5
+    total = sum(r * c for r, c in shapes)
+    bufs = [torch.empty(at + total, device="cuda") for _ in range(3)]
+    small = [torch.randn(total, device="cuda") for _ in range(3)]
+    for v, s in zip(bufs, small):
+        v[at:].copy_(s)
+        v[at - 3:at] = 5.0
+    ops.muon_step(ops.MuonPlan(shapes, "cuda", offset=at), *bufs)
+    ops.muon_step(ops.MuonPlan(shapes, "cuda"), *small)
+    for v, s in zip(bufs, small):
+        assert torch.equal(v[at:], s) and torch.equal(v[at - 3:at], torch.full((3,), 5.0, device="cuda"))
