@@ -470,3 +470,19 @@ def test_more_than_2_31_values(ops):
     for whole, f, l in ((dw, fw, lw), (db, fb, lb)):
         want = 256 * f.double() + l.double()
         assert float((whole.double() - want).abs().max()) <= 2 * 600 * 2.0 ** -24 * 1.2 * rows
+
+
+@pytest.mark.parametrize("rows,c", [(40, 7), (40, 52), (70, 1021), (9, 4096), (600, 9001), (5, 20003)])
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_vectors_at_odd_addresses(ops, rows, c, t):
+    """x, dy, gamma and beta one value behind an aligned address: the bits that aligned tensors give"""
+    x, w, b, dy = make(rows, c, TYPES[t], TYPES[t], seed=c)
+    y, grads = run(ops, x, w, b, dy, act=1, slope=0.1)
+
+    def shift(v):
+        return torch.cat([v.new_zeros(1), v.flatten()])[1:].view(v.shape)
+
+    y1, g1 = run(ops, shift(x), shift(w), shift(b), shift(dy), act=1, slope=0.1)
+    assert shift(x).data_ptr() % 16 and torch.equal(y, y1)
+    for p, q in zip(grads, g1):
+        assert torch.equal(p, q)

@@ -332,3 +332,21 @@ def test_offsets_past_2_31(ops):
     ops.muon_step(ops.MuonPlan(shapes, "cuda"), *small)
     for v, s in zip(bufs, small):
         assert torch.equal(v[at:], s) and torch.equal(v[at - 3:at], torch.full((3,), 5.0, device="cuda"))
+
+
+@pytest.mark.parametrize("t,m,n,batch", [("f32", 100, 100, 3), ("bf16", 700, 100, 1), ("f32", 128, 128, 1), ("bf16", 4096, 4100, 1), ("f32", 1000, 4100, 1),
+                                         ("f16", 60, 5000, 2)])
+def test_captured_calls_of_every_path(ops, t, m, n, batch):
+    """calls whose kernels ask for more shared memory than the default, split tiles and one-launch matrices, captured and replayed"""
+    g = torch.stack([matrix(m, n, seed=s) for s in range(batch)]).cuda().to(TYPES[t])
+    static = g.clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        o = ops.orthogonalize(static)
+    for k in range(3):
+        static.copy_(g.roll(k, -1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, ops.orthogonalize(static)), k
+        o.zero_()
