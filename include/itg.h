@@ -445,7 +445,7 @@ int itg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy,
  * For every matrix G (rows x cols, row-major with a row stride) of a call:  X = G / |G|_F  (zeros where |G|_F <= eps), then
  * `steps` times  A = X X^T, X <- a X + (b A + c A A) X  (on the transpose where rows > cols), out = X in G's type.
  * coefficients: HOST array of 3 * steps floats (a, b, c of each step); they must keep the singular values below 3.9 (checked).
- * dtype: ITG_F32 / ITG_F16 = products as exact as fp32 ones, ITG_BF16 = as exact as the type.  out may be g (same layout).
+ * dtype: ITG_F32 | ITG_BF16 | ITG_F16; products as exact as fp32 ones for each, the result rounded once.  out may be g (same layout).
  * A job is `count` matrices of one shape at a stride; offsets and strides count elements from g / out.  Matrices of one call
  * must not overlap in out, and out overlaps g not at all or is g.  At most 2^22 matrices a call (2^23 where none has more than 128
  * rows or columns, 2^24 where none has more than 64).  A matrix that holds an infinity or a NaN comes out as NaN, the others of the call as they are.

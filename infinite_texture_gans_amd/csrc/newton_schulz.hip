@@ -6,11 +6,10 @@
 // Arithmetic.  The products run on the fp16 matrix cores with fp32 accumulation.  X is carried as two fp16 planes hi + lo (22 bits):
 // what a step rounds off X reappears in directions G does not have, and every later step multiplies it by a = 3.4 (X in fp16 alone:
 // 8e-2 off for an update of rank 1), while what the products round off stays inside G's own row and column space.
-//   split (fp32 and fp16 matrices): A and B are hi + lo as well and every product is hi hi + hi lo + lo hi: as near to 64 bits as
-//     fp32 products are, at three of the 16 MFMA issues an fp32 product of the same shape costs;
-//   single (bf16 matrices): one product of the hi planes.  The diagonals of A and B, which are the large entries and whose rounding
-//     would scale a whole row, stay fp32 (the planes hold zero there) and join in the epilogues: the error beside the result's own
-//     rounding to bf16 stays at 0.6 of it or less.
+// A and B are hi + lo as well and every product is hi hi + hi lo + lo hi: as near to 64 bits as fp32 products are, at three of the
+// 16 MFMA issues an fp32 product of the same shape costs.  What is dropped is lo lo, 2^-22 of a product.  That holds for every type:
+// a bf16 matrix is rounded once, at the end (one product of the hi planes would be off by 0.5 .. 1.5 of that rounding beside it, most
+// where the matrix is small).
 // The planes hold X * 2^12, A * 2^12 and B * 2^10, so that lo is a normal number wherever it matters; the spectral bound of X under
 // the coefficients (checked on the host) keeps hi finite.
 //
@@ -51,20 +50,19 @@ struct NsArgs {
   float eps, mu, lr, wd, ema_decay;
 };
 
-// a matrix's workspace: double norm2[NORM_BLOCKS] | X planes (two generations) | A | B planes | their diagonals
+// a matrix's workspace: double norm2[NORM_BLOCKS] | X planes (two generations) | A | B planes
 struct NsWs {
   double* part;
   _Float16* x[2][2];                  // [generation][hi, lo]: [mp][np]
   _Float16 *a[2], *b[2];              // [hi, lo]: [mp][mp]
-  float *da, *db;                     // diagonals of A and B (single)
 };
 
-__host__ __device__ inline int64_t ns_ws_bytes(int mp, int np, bool split) {
+__host__ __device__ inline int64_t ns_ws_bytes(int mp, int np) {
   const int64_t x = (int64_t)mp * np * 2, a = (int64_t)mp * mp * 2;
-  return (int64_t)NORM_BLOCKS * 8 + 4 * x + a * (split ? 4 : 2) + (int64_t)mp * 8;
+  return (int64_t)NORM_BLOCKS * 8 + 4 * x + 4 * a;
 }
 
-__device__ inline NsWs ns_ws(char* base, int mp, int np, bool split) {
+__device__ inline NsWs ns_ws(char* base, int mp, int np) {
   NsWs w;
   const int64_t x = (int64_t)mp * np, a = (int64_t)mp * mp;
   w.part = (double*)base;
@@ -74,10 +72,9 @@ __device__ inline NsWs ns_ws(char* base, int mp, int np, bool split) {
     w.x[g][1] = q; q += x;
   }
   w.a[0] = q; q += a;
-  w.a[1] = q; q += split ? a : 0;
+  w.a[1] = q; q += a;
   w.b[0] = q; q += a;
-  w.b[1] = q; q += split ? a : 0;
-  w.da = (float*)q; w.db = w.da + mp;
+  w.b[1] = q;
   return w;
 }
 
@@ -199,7 +196,7 @@ __global__ __launch_bounds__(1024) void ns_norm_kernel(NsArgs p) {
 
 // ---- X = G / |G| as planes: 64 x 64 tiles of the padded matrix in G's own orientation, turned in LDS where G is tall
 template <typename T, bool MUON>
-__global__ __launch_bounds__(256) void ns_convert_kernel(NsArgs p, bool split) {
+__global__ __launch_bounds__(256) void ns_convert_kernel(NsArgs p) {
   const NsMat& j = p.j[ns_job(p, blockIdx.x, [](const NsMat& q) { return q.conv0; })];
   const int rp = j.tall ? j.np : j.mp, cp = j.tall ? j.mp : j.np;        // padded extents in G's orientation
   const int tc = cp / 64, per = tc * (rp / 64);
@@ -208,7 +205,7 @@ __global__ __launch_bounds__(256) void ns_convert_kernel(NsArgs p, bool split) {
   local -= z * per;
   const int r0 = local / tc * 64, c0 = local % tc * 64;
   const int rows = j.tall ? j.n : j.m, cols = j.tall ? j.m : j.n;
-  const NsWs w = ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np, split);
+  const NsWs w = ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np);
   __shared__ double lds[4];
   __shared__ float tile[64][65];
   const int c = (threadIdx.x & 15) * 4, rt = threadIdx.x >> 4;
@@ -276,8 +273,9 @@ __global__ __launch_bounds__(256) void ns_convert_kernel(NsArgs p, bool split) {
 //
 // Staging: 16-byte chunks go from global memory straight into LDS.  A wave's 64 lanes fill 1 KiB in lane order, so the chunk a
 // lane FETCHES is permuted instead: chunk c of row r sits in slot c ^ f(r), which spreads the 16 rows an MFMA operand read
-// touches over all banks (BK 64: 8 chunks a row, f = r; BK 32: 4 chunks a row, f = r / 2).
-template <int BK> __device__ __forceinline__ int slot(int r, int c) { return BK == 64 ? c ^ (r & 7) : c ^ ((r >> 1) & 3); }
+// touches over all banks (4 chunks a row, f = r / 2).
+constexpr int BK = 32;                 // K of a slice: that of one MFMA
+__device__ __forceinline__ int slot(int r, int c) { return c ^ ((r >> 1) & 3); }
 
 // Product X takes its first operand, whose rows are X's COLUMNS, from X itself: slices of BK rows of X, T columns wide, read by the
 // transposing LDS read (16 lanes give four rows of 16 columns, lane l gets column l).  A copy of X^T instead would be half of all
@@ -298,11 +296,10 @@ template <int T> __device__ __forceinline__ f16x8 frag_t(const _Float16* at) {
 }
 
 // T: tile, TR x T where TALL; WR x WC waves share it, each with FR x FC fragments of 16 x 16
-template <int T_, bool SPLIT, bool TALL = false> struct Tile {
-  static constexpr int T = T_, TR = TALL ? 2 * T_ : T_, WR = 2, WC = T_ == 256 ? 4 : 2, WAVES = WR * WC, NT = WAVES * 64;
+template <int T_, bool TALL = false> struct Tile {
+  static constexpr int T = T_, TR = TALL ? 2 * T_ : T_, WR = 2, WC = 2, WAVES = WR * WC, NT = WAVES * 64;
   static constexpr int FR = TR / WR / 16, FC = T / WC / 16;
-  static constexpr int NP = SPLIT ? 2 : 1, BK = SPLIT ? 32 : 64;
-  static constexpr int PP = TR * BK, PQ = T * BK, BUF = NP * (PP + PQ);      // halves: a plane of each operand, one buffer
+  static constexpr int PP = TR * BK, PQ = T * BK, BUF = 2 * (PP + PQ);      // halves: a plane of each operand, one buffer
   static constexpr int LP = PP * 2 / 1024 / WAVES, LQ = PQ * 2 / 1024 / WAVES;      // loads of a wave per plane
 };
 
@@ -320,20 +317,20 @@ __device__ __forceinline__ void acc_zero(Acc<C>& a) {
 // DEPTH LDS buffers: DEPTH - 1 slices of K are on their way while one is multiplied
 // acc = the product over k0 .. k1 (multiples of BK) of the T rows from P[plane] and Q[plane] on
 // TURN: P[plane] holds the operand by column (row k of it at k * ldp)
-template <typename C, bool SPLIT, int DEPTH, bool TURN>
+template <typename C, int DEPTH, bool TURN>
 __device__ __forceinline__ void ns_product(Acc<C>& acc, const _Float16* const* P, int ldp, const _Float16* const* Q, int ldq, int k0, int k1, _Float16* lds) {
-  constexpr int BK = C::BK, NP = C::NP, T = C::T, TR = C::TR, CH = BK / 8, ROWS = 64 / CH, CHT = TR / 8, ROWST = 64 / CHT;
+  constexpr int T = C::T, TR = C::TR, CH = BK / 8, ROWS = 64 / CH, CHT = TR / 8, ROWST = 64 / CHT;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l15 = lane & 15, lk = lane >> 4;
   uint32_t from_p[C::LP], from_q[C::LQ];                   // bytes from a slice's first value to what this lane fetches
 #pragma unroll
   for (int u = 0; u < C::LP; ++u) {
     const int r = (wave * C::LP + u) * ROWS + lane / CH, rt = (wave * C::LP + u) * ROWST + lane / CHT;
-    from_p[u] = TURN ? (uint32_t)(rt * ldp + slot_t<TR>(rt, lane % CHT) * 8) * 2u : (uint32_t)(r * ldp + slot<BK>(r, lane % CH) * 8) * 2u;
+    from_p[u] = TURN ? (uint32_t)(rt * ldp + slot_t<TR>(rt, lane % CHT) * 8) * 2u : (uint32_t)(r * ldp + slot(r, lane % CH) * 8) * 2u;
   }
 #pragma unroll
   for (int u = 0; u < C::LQ; ++u) {
     const int r = (wave * C::LQ + u) * ROWS + lane / CH;
-    from_q[u] = (uint32_t)(r * ldq + slot<BK>(r, lane % CH) * 8) * 2u;
+    from_q[u] = (uint32_t)(r * ldq + slot(r, lane % CH) * 8) * 2u;
   }
   auto stage = [&](int buf, int k) {
     auto fetch = [&](const _Float16* from, const uint32_t* off, int n, _Float16* to) {
@@ -343,55 +340,53 @@ __device__ __forceinline__ void ns_product(Acc<C>& acc, const _Float16* const* P
                                          (__attribute__((address_space(3))) void*)(to + u * 512), 16, 0, 0);
     };
 #pragma unroll
-    for (int q = 0; q < NP; ++q)
+    for (int q = 0; q < 2; ++q)
       fetch(TURN ? P[q] + (int64_t)k * ldp : P[q] + k, from_p, C::LP, lds + buf * C::BUF + q * C::PP + wave * C::LP * 512);
 #pragma unroll
-    for (int q = 0; q < NP; ++q) fetch(Q[q] + k, from_q, C::LQ, lds + buf * C::BUF + NP * C::PP + q * C::PQ + wave * C::LQ * 512);
+    for (int q = 0; q < 2; ++q) fetch(Q[q] + k, from_q, C::LQ, lds + buf * C::BUF + 2 * C::PP + q * C::PQ + wave * C::LQ * 512);
   };
   const int wr = (wave / C::WC) * (TR / C::WR), wc = (wave % C::WC) * (T / C::WC);
   const int row_q = (wc + l15) * BK;
-  int at_p[C::FR], ch[BK / 32];
-#pragma unroll
-  for (int ks = 0; ks < BK / 32; ++ks) ch[ks] = slot<BK>(l15, ks * 4 + lk) * 8;
+  const int ch = slot(l15, lk) * 8;
+  int at_p[C::FR];
 #pragma unroll
   for (int i = 0; i < C::FR; ++i) {
     const int r = lk * 8 + (l15 >> 2);
     at_p[i] = TURN ? r * TR + slot_t<TR>(r, wr / 8 + 2 * i + ((l15 >> 1) & 1)) * 8 + (l15 & 1) * 4 : (wr + i * 16 + l15) * BK;
   }
-  // split: sums in two levels, a fresh accumulator every 256 of K.  One accumulator over all of K drifts: each MFMA adds to it
+  // sums in two levels, a fresh accumulator every 256 of K.  One accumulator over all of K drifts: each MFMA adds to it
   // with an error of one step of the sum, and on the diagonal of X X^T, a sum of squares, these do not cancel (a 1 x 4099 matrix:
   // 2.9e-6 off with one level, fp32 products in torch 6e-7)
   constexpr int FLUSH = KSHARE / BK;
   Acc<C> part;
   acc_zero(acc);
-  if (SPLIT) acc_zero(part);
-  Acc<C>& run = SPLIT ? part : acc;
+  acc_zero(part);
   const int nk = (k1 - k0) / BK;
-  constexpr int LOADS = NP * (C::LP + C::LQ);              // of a wave per buffer
-  struct Frags { f16x8 p[NP][C::FR], q[NP][C::FC]; };
-  auto read = [&](int buf, int ks, Frags& f) {
+  constexpr int LOADS = 2 * (C::LP + C::LQ);               // of a wave per buffer
+  struct Frags { f16x8 p[2][C::FR], q[2][C::FC]; };
+  auto read = [&](int buf, Frags& f) {
     const _Float16* at = lds + buf * C::BUF;
 #pragma unroll
-    for (int q = 0; q < NP; ++q) {
+    for (int q = 0; q < 2; ++q) {
 #pragma unroll
       for (int i = 0; i < C::FR; ++i)
-        f.p[q][i] = TURN ? frag_t<TR>(at + q * C::PP + at_p[i] + ks * 32 * TR) : *reinterpret_cast<const f16x8*>(at + q * C::PP + at_p[i] + ch[ks]);
+        f.p[q][i] = TURN ? frag_t<TR>(at + q * C::PP + at_p[i]) : *reinterpret_cast<const f16x8*>(at + q * C::PP + at_p[i] + ch);
 #pragma unroll
-      for (int k = 0; k < C::FC; ++k) f.q[q][k] = *reinterpret_cast<const f16x8*>(at + NP * C::PP + q * C::PQ + row_q + ch[ks] + k * 16 * BK);
+      for (int k = 0; k < C::FC; ++k) f.q[q][k] = *reinterpret_cast<const f16x8*>(at + 2 * C::PP + q * C::PQ + row_q + ch + k * 16 * BK);
     }
   };
   // lo hi, hi lo, hi hi: each over all fragments, so that no product waits for the one before it
   auto multiply = [&](const Frags& f) {
 #pragma unroll
-    for (int q = SPLIT ? 0 : 2; q < 3; ++q)
+    for (int q = 0; q < 3; ++q)
 #pragma unroll
       for (int i = 0; i < C::FR; ++i)
 #pragma unroll
         for (int k = 0; k < C::FC; ++k)
-          run.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[q == 0 ? NP - 1 : 0][i], f.q[q == 1 ? NP - 1 : 0][k], run.v[i][k], 0, 0, 0);
+          part.v[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[q == 0][i], f.q[q == 1][k], part.v[i][k], 0, 0, 0);
   };
   auto flush = [&](int kk) {
-    if (!SPLIT || ((kk + 1) % FLUSH != 0 && kk + 1 != nk)) return;
+    if ((kk + 1) % FLUSH != 0 && kk + 1 != nk) return;
 #pragma unroll
     for (int i = 0; i < C::FR; ++i)
 #pragma unroll
@@ -402,22 +397,16 @@ __device__ __forceinline__ void ns_product(Acc<C>& acc, const _Float16* const* P
   // barrier, the other waves'.  The barrier also tells that the buffer before has been read and may be filled again.
   if (DEPTH == 4) {
     // few workgroups: nothing else hides the LDS reads, so a slice is read while the one before is multiplied
-    constexpr int KS = BK / 32;
-    Frags f[2][KS];
-    auto all = [&](int buf, Frags (&g)[KS]) {
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) read(buf, ks, g[ks]);
-    };
+    Frags f[2];
 #pragma unroll
     for (int b = 0; b < DEPTH; ++b) stage(b, slice(b));
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((DEPTH - 1) * LOADS) : "memory");
-    all(0, f[0]);
-    auto turn = [&](int kk, Frags (&now)[KS], Frags (&next)[KS]) {
+    read(0, f[0]);
+    auto turn = [&](int kk, const Frags& now, Frags& next) {
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((DEPTH - 2) * LOADS) : "memory");
       stage(kk & 3, slice(kk + DEPTH));
-      all((kk + 1) & 3, next);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) multiply(now[ks]);
+      read((kk + 1) & 3, next);
+      multiply(now);
       flush(kk);
     };
     int kk = 0;
@@ -430,8 +419,9 @@ __device__ __forceinline__ void ns_product(Acc<C>& acc, const _Float16* const* P
     for (int kk = 0; kk < nk; ++kk) {
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((DEPTH - 2) * LOADS) : "memory");
       stage(into, slice(kk + DEPTH - 1));
-#pragma unroll
-      for (int ks = 0; ks < BK / 32; ++ks) { Frags f; read(buf, ks, f); multiply(f); }
+      Frags f;
+      read(buf, f);
+      multiply(f);
       flush(kk);
       buf = buf + 1 == DEPTH ? 0 : buf + 1;
       into = into + 1 == DEPTH ? 0 : into + 1;
@@ -470,12 +460,10 @@ __device__ __forceinline__ void ns_store(_Float16* turn, const f16x4 (&v)[N][FC]
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read before the next call writes
 }
 
-// The operand whose tile a product's result is added to: A (product B) or X (product X), hi and lo, and the diagonals (single).
-template <typename C, bool SPLIT, int PH, int N>
+// The operand whose tile a product's result is added to: A (product B) or X (product X), hi and lo.
+template <typename C, int PH, int N>
 struct Addend {
   f16x4 h[N][C::FC], l[N][C::FC];
-  f32x4 drow[N];
-  float dcol[C::FC];
   __device__ __forceinline__ void load(const NsMat& j, const NsWs& w, int ti, int tj, int gen, int i0) {
     if (PH == PH_A) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -489,23 +477,16 @@ struct Addend {
       for (int k = 0; k < C::FC; ++k) {
         const int64_t at = (cbase + k * 16) * ld + rbase + i * 16;
         h[i][k] = *reinterpret_cast<const f16x4*>(hi + at);
-        if (SPLIT || PH != PH_B) l[i][k] = *reinterpret_cast<const f16x4*>(lo + at);
+        l[i][k] = *reinterpret_cast<const f16x4*>(lo + at);
       }
-    if (!SPLIT) {
-#pragma unroll
-      for (int k = 0; k < C::FC; ++k) dcol[k] = PH == PH_B ? w.da[cbase + k * 16] : w.db[cbase + k * 16];
-      if (PH == PH_B)
-#pragma unroll
-        for (int i = 0; i < N; ++i) drow[i] = *reinterpret_cast<const f32x4*>(w.da + rbase + i * 16);
-    }
   }
 };
 
 // What a product's tile (ti, tj) of a matrix becomes; N fragment rows of it, from i0 on.  A lane holds rows row0 .. row0 + 3 of
 // column col of each fragment.  The addend is read before the first store: loads and stores share one counter, so a load behind a
 // store waits for it (reading fragment by fragment cost 15 us a tile).
-template <typename C, bool SPLIT, int PH, typename OUT, bool MUON, int N>
-__device__ __forceinline__ void ns_write_rows(const f32x4 (*acc)[C::FC], int i0, const Addend<C, SPLIT, PH, N>& ad, _Float16* lds, const NsArgs& p,
+template <typename C, int PH, typename OUT, bool MUON, int N>
+__device__ __forceinline__ void ns_write_rows(const f32x4 (*acc)[C::FC], int i0, const Addend<C, PH, N>& ad, _Float16* lds, const NsArgs& p,
                                               const NsMat& j, const NsWs& w, int z, int ti, int tj, int gen, float ca, float cb, float cc) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, lk = lane >> 4;
   const int r0 = ti * C::TR + (wave / C::WC) * (C::TR / C::WR) + i0 * 16, c0 = tj * C::T + (wave % C::WC) * (C::T / C::WC);
@@ -522,30 +503,16 @@ __device__ __forceinline__ void ns_write_rows(const f32x4 (*acc)[C::FC], int i0,
       } else if (PH == PH_B) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float a1 = (float)ad.h[i][k][e] * (1.f / SA), a2 = sum[e] * (1.f / (SA * SA));
-          if (SPLIT) a1 += (float)ad.l[i][k][e] * (1.f / SA);
-          else if (row0 + e == col) { a1 = ad.drow[i][e]; a2 = fmaf(a1, a1, a2); }
-          else a2 = fmaf(ad.drow[i][e] + ad.dcol[k], a1, a2);
+          const float a1 = (float)ad.h[i][k][e] * (1.f / SA) + (float)ad.l[i][k][e] * (1.f / SA), a2 = sum[e] * (1.f / (SA * SA));
           v[e] = (cb * a1 + cc * a2) * SB;
         }
       } else {      // row: column of X, col: row of X
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = fmaf(ca, (float)ad.h[i][k][e] + (float)ad.l[i][k][e], sum[e] * (1.f / SB));
-          if (!SPLIT) v[e] = fmaf(ad.dcol[k], (float)ad.h[i][k][e], v[e]);
-        }
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(ca, (float)ad.h[i][k][e] + (float)ad.l[i][k][e], sum[e] * (1.f / SB));
       }
       if (PH == PH_LAST) {
         ns_result<OUT, MUON>(p, j, z, row0, col, v);
         continue;
-      }
-      if (PH < PH_X && !SPLIT) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (row0 + e == col) {
-            if (PH == PH_A) w.da[col] = v[e] * (1.f / SA); else w.db[col] = v[e] * (1.f / SB);
-            v[e] = 0.f;
-          }
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) { _Float16 h, l; split_f16(v[e], h, l); hi[i][k][e] = h; lo[i][k][e] = l; }
@@ -557,10 +524,10 @@ __device__ __forceinline__ void ns_write_rows(const f32x4 (*acc)[C::FC], int i0,
     _Float16* tl = PH == PH_A ? w.a[1] : w.b[1];
     const int64_t down = (int64_t)c0 * j.mp + r0, across = (int64_t)r0 * j.mp + c0;
     ns_store<N, C::FC, true>(turn, hi, th + down, j.mp);
-    if (SPLIT) ns_store<N, C::FC, true>(turn, lo, tl + down, j.mp);
+    ns_store<N, C::FC, true>(turn, lo, tl + down, j.mp);
     if (ti != tj) {
       ns_store<N, C::FC, false>(turn, hi, th + across, j.mp);
-      if (SPLIT) ns_store<N, C::FC, false>(turn, lo, tl + across, j.mp);
+      ns_store<N, C::FC, false>(turn, lo, tl + across, j.mp);
     }
   } else {
     const int64_t at = (int64_t)c0 * j.np + r0;
@@ -591,9 +558,9 @@ __device__ __forceinline__ void ns_tile(const NsMat& j, int local, int& z, int& 
 
 // One workgroup per tile, or, of the tiles behind direct[], per share of a tile's K, which goes to the slab: the tiles of a small
 // call do not fill the chip, and neither do those that are left over from its last full round.
-template <int T, bool SPLIT, bool TALL, int DEPTH, int PH, typename OUT, bool MUON>
-__global__ __launch_bounds__((Tile<T, SPLIT>::NT), 2) void ns_gemm_kernel(NsArgs p, int gen, float ca, float cb, float cc) {
-  typedef Tile<T, SPLIT, TALL> C;
+template <int T, bool TALL, int DEPTH, int PH, typename OUT, bool MUON>
+__global__ __launch_bounds__((Tile<T>::NT), 2) void ns_gemm_kernel(NsArgs p, int gen, float ca, float cb, float cc) {
+  typedef Tile<T, TALL> C;
   constexpr int Q3 = PH < PH_X ? PH : 2;
   extern __shared__ __attribute__((aligned(16))) _Float16 lds[];
   const int direct = p.direct[Q3], bid = blockIdx.x;
@@ -619,11 +586,11 @@ __global__ __launch_bounds__((Tile<T, SPLIT>::NT), 2) void ns_gemm_kernel(NsArgs
   const NsMat& j = p.j[job];
   int z, ti, tj;
   ns_tile<T, C::TR, PH>(j, tile, z, ti, tj);
-  const NsWs w = ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np, SPLIT);
+  const NsWs w = ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np);
   const int ld = PH == PH_A ? j.np : j.mp;                 // of the second operand, and K
   const _Float16* P[2]; const _Float16* Q[2];
 #pragma unroll
-  for (int q = 0; q < C::NP; ++q) {
+  for (int q = 0; q < 2; ++q) {
     P[q] = PH >= PH_X ? w.x[gen][q] + ti * C::TR : (PH == PH_A ? w.x[gen][q] : w.a[q]) + (int64_t)ti * T * ld;
     Q[q] = (PH == PH_A ? w.x[gen][q] : PH == PH_B ? w.a[q] : w.b[q]) + (int64_t)tj * T * ld;
   }
@@ -634,18 +601,18 @@ __global__ __launch_bounds__((Tile<T, SPLIT>::NT), 2) void ns_gemm_kernel(NsArgs
     k1 = k0 + per < ld ? k0 + per : ld;
   }
   // 64: the addend waits in registers through the product; larger tiles read it behind it, in halves
-  constexpr int N = T == 256 ? 4 : 2;
+  constexpr int N = 2;
   Acc<C> acc;
-  Addend<C, SPLIT, PH, N> ad;
+  Addend<C, PH, N> ad;
   if (C::FR == N && whole) ad.load(j, w, ti, tj, gen, 0);
-  ns_product<C, SPLIT, DEPTH, (PH >= PH_X)>(acc, P, PH >= PH_X ? j.np : ld, Q, ld, k0, k1, lds);
+  ns_product<C, DEPTH, (PH >= PH_X)>(acc, P, PH >= PH_X ? j.np : ld, Q, ld, k0, k1, lds);
   if (whole) {
     if (C::FR != N) ad.load(j, w, ti, tj, gen, 0);
     __syncthreads();                                       // the slices in LDS have been read: it turns the results now
-    ns_write_rows<C, SPLIT, PH, OUT, MUON, N>(acc.v, 0, ad, lds, p, j, w, z, ti, tj, gen, ca, cb, cc);
+    ns_write_rows<C, PH, OUT, MUON, N>(acc.v, 0, ad, lds, p, j, w, z, ti, tj, gen, ca, cb, cc);
     if (C::FR > N) {
       ad.load(j, w, ti, tj, gen, N);
-      ns_write_rows<C, SPLIT, PH, OUT, MUON, N>(acc.v + C::FR - N, N, ad, lds, p, j, w, z, ti, tj, gen, ca, cb, cc);
+      ns_write_rows<C, PH, OUT, MUON, N>(acc.v + C::FR - N, N, ad, lds, p, j, w, z, ti, tj, gen, ca, cb, cc);
     }
   } else {
     f32x4* to = reinterpret_cast<f32x4*>(p.slab) + (int64_t)slot_at * (C::TR * T / 4) + threadIdx.x;
@@ -657,9 +624,9 @@ __global__ __launch_bounds__((Tile<T, SPLIT>::NT), 2) void ns_gemm_kernel(NsArgs
 }
 
 // the split tiles: their shares added in order, then as any other tile; a workgroup per row of fragments
-template <int T, bool SPLIT, bool TALL, int PH, typename OUT, bool MUON>
-__global__ __launch_bounds__((Tile<T, SPLIT>::NT)) void ns_join_kernel(NsArgs p, int gen, float ca, float cb, float cc) {
-  typedef Tile<T, SPLIT, TALL> C;
+template <int T, bool TALL, int PH, typename OUT, bool MUON>
+__global__ __launch_bounds__((Tile<T>::NT)) void ns_join_kernel(NsArgs p, int gen, float ca, float cb, float cc) {
+  typedef Tile<T, TALL> C;
   constexpr int Q3 = PH < PH_X ? PH : 2;
   const int direct = p.direct[Q3], t = direct + blockIdx.x / C::FR, i = blockIdx.x % C::FR;
   const NsMat& j = p.j[ns_job(p, t, [](const NsMat& q) { return q.tile0[Q3]; })];
@@ -669,8 +636,8 @@ __global__ __launch_bounds__((Tile<T, SPLIT>::NT)) void ns_join_kernel(NsArgs p,
   __shared__ __attribute__((aligned(16))) _Float16 lds[C::WAVES * ns_turn<1, C::FC>()];
   int z, ti, tj;
   ns_tile<T, C::TR, PH>(j, t - j.tile0[Q3], z, ti, tj);
-  const NsWs w = ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np, SPLIT);
-  Addend<C, SPLIT, PH, 1> ad;
+  const NsWs w = ns_ws(p.ws + j.ws + z * j.wst, j.mp, j.np);
+  Addend<C, PH, 1> ad;
   ad.load(j, w, ti, tj, gen, i);
   f32x4 v[1][C::FC];
 #pragma unroll
@@ -679,7 +646,7 @@ __global__ __launch_bounds__((Tile<T, SPLIT>::NT)) void ns_join_kernel(NsArgs p,
   for (int s = 0; s < n; ++s)
 #pragma unroll
     for (int k = 0; k < C::FC; ++k) v[0][k] += from[s * next + k * C::NT];
-  ns_write_rows<C, SPLIT, PH, OUT, MUON, 1>(v, i, ad, lds, p, j, w, z, ti, tj, gen, ca, cb, cc);
+  ns_write_rows<C, PH, OUT, MUON, 1>(v, i, ad, lds, p, j, w, z, ti, tj, gen, ca, cb, cc);
 }
 
 #include "newton_schulz_thin.h"
@@ -692,17 +659,15 @@ struct NsPlan { int64_t bytes, norm, conv; int T[3], TR; int64_t grid[3], join[3
 inline int64_t up(int64_t v, int64_t k) { return (v + k - 1) / k * k; }
 
 // Tile sizes of the products, from the number of tiles that each size would make.
-// X: 128 from 384 tiles on (1024 x 8192 fp32, 512 tiles: 820 -> 712 us a call; 1024 x 4096, 256 tiles: 508 -> 566), and 256 (single
-//   only: split has no registers for it) from a full round of 256 tiles on (4096 x 8192 bf16: 3207 -> 3056 us).
-// A and B, whose leftover tiles are split along K, go by tiles x K: split 128 from 192 K on (1024 x 8192, A 288 K: 712 -> 673 us;
-//   4 x 1024 x 1024, 144 K: 634 -> 642), single from 400 K on (1536 x 6144, A 468 K: 626 -> 598 us; 1024 x 8192, 288 K: 406 -> 413).
-//   Split at 64 takes tiles of 128 columns of X by 64 rows where they make 512 or more: a third less of LDS and cache traffic for a
-//   product (the default generator's matrices, a Muon step: 417 -> 392 us; 2048 x 2048 835 -> 811; 512 x 4096, 256 such tiles:
-//   217 -> 246; single, 2048 x 2048: 441 -> 450).
+// X: 128 from 384 tiles on (1024 x 8192 fp32, 512 tiles: 820 -> 712 us a call; 1024 x 4096, 256 tiles: 508 -> 566).  Below, 64, as
+//   tiles of 128 columns of X by 64 rows where they make 512 or more: a third less of LDS and cache traffic for a product (the default
+//   generator's matrices, a Muon step: 417 -> 392 us; 2048 x 2048 835 -> 811; 512 x 4096, 256 such tiles: 217 -> 246).
+// A and B, whose leftover tiles are split along K, go by tiles x K: 128 from 192 K on (1024 x 8192, A 288 K: 712 -> 673 us;
+//   4 x 1024 x 1024, 144 K: 634 -> 642).
 // A size whose padding adds more than an eighth to the planes is not taken (the default generator's matrices of 3 to 416 rows: 448 us
 // a Muon step with X at 128, 430 without).
-void ns_tile_sizes(const NsArgs& p, bool split, NsPlan& pl) {
-  int64_t a = 0, b = 0, x = 0, x64 = 0, x256 = 0, tall = 0;
+void ns_tile_sizes(const NsArgs& p, NsPlan& pl) {
+  int64_t a = 0, b = 0, x = 0, x64 = 0, tall = 0;
   for (int i = 0; i < p.n; ++i) {
     const NsMat& j = p.j[i];
     const int64_t m = up(j.m, 128) / 128, n = up(j.n, 128) / 128, sym = m * (m + 1) / 2 * j.count;
@@ -711,14 +676,13 @@ void ns_tile_sizes(const NsArgs& p, bool split, NsPlan& pl) {
     x += m * n * j.count;
     tall += up(j.m, 64) / 64 * n * j.count;
     x64 += up(j.m, 64) / 64 * (up(j.n, 64) / 64) * j.count;
-    x256 += ((m + 1) / 2) * ((n + 1) / 2) * j.count;
   }
-  const int64_t least = (split ? 192 : 400) * 1024;
-  const bool fits = 32 * x <= 9 * x64, fits256 = 128 * x256 <= 9 * x64;
+  const int64_t least = 192 * 1024;
+  const bool fits = 32 * x <= 9 * x64;
   pl.T[0] = fits && a >= least ? 128 : 64;
   pl.T[1] = fits && b >= least ? 128 : 64;
-  pl.T[2] = !split && fits256 && x256 >= 256 ? 256 : fits && x >= 384 ? 128 : 64;
-  pl.TR = split && pl.T[2] == 64 && 16 * tall <= 9 * x64 && tall >= 512 ? 128 : pl.T[2];
+  pl.T[2] = fits && x >= 384 ? 128 : 64;
+  pl.TR = pl.T[2] == 64 && 16 * tall <= 9 * x64 && tall >= 512 ? 128 : pl.T[2];
 }
 
 // Tiles and shares of product q (A, B, X).  `slots` workgroups run at a time; whole rounds of them take a tile each, and what is
@@ -731,9 +695,9 @@ int ns_tiles(NsArgs& p, NsPlan& pl, int q, int64_t& slab) {
     const int64_t nt = j.mp / T, nx = j.np / pl.TR;
     j.tile0[q] = (int)tiles;
     tiles += (q == 2 ? nt * nx : nt * (nt + 1) / 2) * j.count;
-    if (tiles >= ((int64_t)1 << (T == 256 ? 23 : 24))) return ITG_ERR_ARG;
+    if (tiles >= ((int64_t)1 << 24)) return ITG_ERR_ARG;
   }
-  const int64_t slots = 256 * (T == 256 ? 1 : 2);
+  const int64_t slots = 512;
   int64_t direct = tiles / slots * slots, rest = tiles - direct, shares = 0;
   // more than half a round left, or nothing to split: the last round stays as it is
   bool splits = false;
@@ -791,7 +755,7 @@ bool ns_thin(NsArgs& p, NsPlan& pl) {
 }
 
 // fills p.j[] from the jobs; returns a status
-int ns_plan(const itg_ns_job* jobs, int n, bool split, bool muon, NsArgs& p, NsPlan& pl) {
+int ns_plan(const itg_ns_job* jobs, int n, bool muon, NsArgs& p, NsPlan& pl) {
   if (!jobs || n < 1 || n > ITG_NS_MAX_JOBS) return ITG_ERR_ARG;
   p.n = n;
   pl = NsPlan{};
@@ -833,7 +797,7 @@ int ns_plan(const itg_ns_job* jobs, int n, bool split, bool muon, NsArgs& p, NsP
     if (pl.one) pl.bytes = 16;
     return ITG_OK;
   }
-  ns_tile_sizes(p, split, pl);
+  ns_tile_sizes(p, pl);
   const int T = pl.T[2] > pl.T[0] ? pl.T[2] : pl.T[0] > pl.T[1] ? pl.T[0] : pl.T[1];
   for (int i = 0; i < n; ++i) {
     const itg_ns_job& q = jobs[i];
@@ -844,7 +808,7 @@ int ns_plan(const itg_ns_job* jobs, int n, bool split, bool muon, NsArgs& p, NsP
     pl.norm += (int64_t)j.nblk * j.count;
     pl.conv += (int64_t)(j.mp / 64) * (j.np / 64) * j.count;
     if (pl.norm >= ((int64_t)1 << 22) || pl.conv >= ((int64_t)1 << 24)) return ITG_ERR_ARG;      // a launch counts its threads in 32 bits
-    j.wst = up(ns_ws_bytes(j.mp, j.np, split), 256);
+    j.wst = up(ns_ws_bytes(j.mp, j.np), 256);
     j.ws = pl.bytes;
     if (j.wst > ((int64_t)1 << 60) / j.count) return ITG_ERR_ARG;
     pl.bytes += j.wst * j.count;
@@ -883,74 +847,72 @@ int ns_lds(K kernel, int bytes) {
              ? ITG_OK : ITG_ERR_LAUNCH;
 }
 
-template <int T, bool SPLIT, int DEPTH, int PH, typename OUT, bool MUON, bool TALL = false>
+template <int T, int DEPTH, int PH, typename OUT, bool MUON, bool TALL = false>
 int ns_launch(const NsArgs& p, const NsPlan& pl, int gen, const float* abc, hipStream_t s) {
-  typedef Tile<T, SPLIT, TALL> C;
+  typedef Tile<T, TALL> C;
   constexpr int Q3 = PH < PH_X ? PH : 2, LDS = DEPTH * C::BUF * 2;
-  if (ns_lds(&ns_gemm_kernel<T, SPLIT, TALL, DEPTH, PH, OUT, MUON>, LDS)) return ITG_ERR_LAUNCH;
-  hipLaunchKernelGGL((ns_gemm_kernel<T, SPLIT, TALL, DEPTH, PH, OUT, MUON>), dim3((unsigned)pl.grid[Q3]), dim3(C::NT), LDS, s, p, gen, abc[0], abc[1], abc[2]);
+  if (ns_lds(&ns_gemm_kernel<T, TALL, DEPTH, PH, OUT, MUON>, LDS)) return ITG_ERR_LAUNCH;
+  hipLaunchKernelGGL((ns_gemm_kernel<T, TALL, DEPTH, PH, OUT, MUON>), dim3((unsigned)pl.grid[Q3]), dim3(C::NT), LDS, s, p, gen, abc[0], abc[1], abc[2]);
   ITG_CHECK_LAUNCH();
   if (pl.join[Q3]) {
-    hipLaunchKernelGGL((ns_join_kernel<T, SPLIT, TALL, PH, OUT, MUON>), dim3((unsigned)(pl.join[Q3] * C::FR)), dim3(C::NT), 0, s, p, gen, abc[0], abc[1], abc[2]);
+    hipLaunchKernelGGL((ns_join_kernel<T, TALL, PH, OUT, MUON>), dim3((unsigned)(pl.join[Q3] * C::FR)), dim3(C::NT), 0, s, p, gen, abc[0], abc[1], abc[2]);
     ITG_CHECK_LAUNCH();
   }
   return ITG_OK;
 }
 
-template <bool SPLIT, int PH, typename OUT, bool MUON>
+template <int PH, typename OUT, bool MUON>
 int ns_phase(const NsArgs& p, const NsPlan& pl, int gen, const float* abc, hipStream_t s) {
   const int T = pl.T[PH < PH_X ? PH : 2];
   const int64_t grid = pl.grid[PH < PH_X ? PH : 2];
-  // 64: four buffers while two workgroups a CU take the whole launch (2 x 333 x 1501 bf16: 156 us against 162 with two), two buffers
-  // and up to five workgroups a CU beyond
-  if (PH >= PH_X && T == 64 && pl.TR == 128) return ns_launch<64, SPLIT, 2, PH, OUT, MUON, SPLIT && PH >= PH_X>(p, pl, gen, abc, s);
-  if (T == 64 && grid <= 512) return ns_launch<64, SPLIT, 4, PH, OUT, MUON>(p, pl, gen, abc, s);
-  if (T == 64) return ns_launch<64, SPLIT, 2, PH, OUT, MUON>(p, pl, gen, abc, s);
-  if (SPLIT || T == 128) return ns_launch<128, SPLIT, 2, PH, OUT, MUON>(p, pl, gen, abc, s);
-  constexpr int BIG = !SPLIT && PH >= PH_X ? 256 : 128;
-  return ns_launch<BIG, SPLIT, 2, PH, OUT, MUON>(p, pl, gen, abc, s);
+  // 64: four buffers while two workgroups a CU take the whole launch (512 x 512: 156 us against 182 with two,
+  // 2 x 1501 x 333: 185 against 196), two buffers and up to five workgroups a CU beyond
+  if (PH >= PH_X && T == 64 && pl.TR == 128) return ns_launch<64, 2, PH, OUT, MUON, (PH >= PH_X)>(p, pl, gen, abc, s);
+  if (T == 64 && grid <= 512) return ns_launch<64, 4, PH, OUT, MUON>(p, pl, gen, abc, s);
+  if (T == 64) return ns_launch<64, 2, PH, OUT, MUON>(p, pl, gen, abc, s);
+  return ns_launch<128, 2, PH, OUT, MUON>(p, pl, gen, abc, s);
 }
 
-template <int M, typename T, bool SPLIT, bool MUON>
+template <int M, typename T, bool MUON>
 int ns_thin_run(const NsArgs& p, const NsPlan& pl, const float* abc, int steps, hipStream_t s) {
-  typedef Thin<M, SPLIT> C;
+  typedef Thin<M> C;
   const dim3 grid((unsigned)pl.blocks), nt(C::NT);
   if (pl.one) {
     NsSteps st;
     for (int i = 0; i < 3 * steps; ++i) st.abc[i] = abc[i];
     st.n = steps;
-    if (ns_lds(&ns_thin_all_kernel<M, SPLIT, T, MUON>, C::LDS)) return ITG_ERR_LAUNCH;
-    hipLaunchKernelGGL((ns_thin_all_kernel<M, SPLIT, T, MUON>), grid, nt, C::LDS, s, p, st);
+    if (ns_lds(&ns_thin_all_kernel<M, T, MUON>, C::LDS)) return ITG_ERR_LAUNCH;
+    hipLaunchKernelGGL((ns_thin_all_kernel<M, T, MUON>), grid, nt, C::LDS, s, p, st);
     ITG_CHECK_LAUNCH();
     return ITG_OK;
   }
-  if (ns_lds(&ns_thin_first_kernel<M, SPLIT, T, MUON>, C::LDS) || ns_lds(&ns_thin_step_kernel<M, SPLIT, false, T, MUON>, C::LDS) ||
-      ns_lds(&ns_thin_step_kernel<M, SPLIT, true, T, MUON>, C::LDS)) return ITG_ERR_LAUNCH;
+  if (ns_lds(&ns_thin_first_kernel<M, T, MUON>, C::LDS) || ns_lds(&ns_thin_step_kernel<M, false, T, MUON>, C::LDS) ||
+      ns_lds(&ns_thin_step_kernel<M, true, T, MUON>, C::LDS)) return ITG_ERR_LAUNCH;
   hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)pl.norm), dim3(1024), 0, s, p);
   ITG_CHECK_LAUNCH();
-  hipLaunchKernelGGL((ns_thin_first_kernel<M, SPLIT, T, MUON>), grid, nt, C::LDS, s, p);
+  hipLaunchKernelGGL((ns_thin_first_kernel<M, T, MUON>), grid, nt, C::LDS, s, p);
   ITG_CHECK_LAUNCH();
   for (int k = 0; k < steps; ++k, abc += 3) {
-    if (k + 1 < steps) hipLaunchKernelGGL((ns_thin_step_kernel<M, SPLIT, false, T, MUON>), grid, nt, C::LDS, s, p, k & 1, abc[0], abc[1], abc[2]);
-    else hipLaunchKernelGGL((ns_thin_step_kernel<M, SPLIT, true, T, MUON>), grid, nt, C::LDS, s, p, k & 1, abc[0], abc[1], abc[2]);
+    if (k + 1 < steps) hipLaunchKernelGGL((ns_thin_step_kernel<M, false, T, MUON>), grid, nt, C::LDS, s, p, k & 1, abc[0], abc[1], abc[2]);
+    else hipLaunchKernelGGL((ns_thin_step_kernel<M, true, T, MUON>), grid, nt, C::LDS, s, p, k & 1, abc[0], abc[1], abc[2]);
     ITG_CHECK_LAUNCH();
   }
   return ITG_OK;
 }
 
-template <typename T, bool SPLIT, bool MUON>
+template <typename T, bool MUON>
 int ns_run(NsArgs& p, const NsPlan& pl, const float* abc, int steps, hipStream_t s) {
-  if (pl.thin) return pl.thin == 64 ? ns_thin_run<64, T, SPLIT, MUON>(p, pl, abc, steps, s) : ns_thin_run<128, T, SPLIT, MUON>(p, pl, abc, steps, s);
+  if (pl.thin) return pl.thin == 64 ? ns_thin_run<64, T, MUON>(p, pl, abc, steps, s) : ns_thin_run<128, T, MUON>(p, pl, abc, steps, s);
   p.slab = (float*)(p.ws + (int64_t)p.slab);
   hipLaunchKernelGGL((ns_norm_kernel<T, MUON>), dim3((unsigned)pl.norm), dim3(1024), 0, s, p);
   ITG_CHECK_LAUNCH();
-  hipLaunchKernelGGL((ns_convert_kernel<T, MUON>), dim3((unsigned)pl.conv), dim3(256), 0, s, p, SPLIT);
+  hipLaunchKernelGGL((ns_convert_kernel<T, MUON>), dim3((unsigned)pl.conv), dim3(256), 0, s, p);
   ITG_CHECK_LAUNCH();
   for (int k = 0; k < steps; ++k, abc += 3) {
     const int gen = k & 1;
-    int rc = ns_phase<SPLIT, PH_A, T, MUON>(p, pl, gen, abc, s);
-    if (!rc) rc = ns_phase<SPLIT, PH_B, T, MUON>(p, pl, gen, abc, s);
-    if (!rc) rc = k + 1 < steps ? ns_phase<SPLIT, PH_X, T, MUON>(p, pl, gen, abc, s) : ns_phase<SPLIT, PH_LAST, T, MUON>(p, pl, gen, abc, s);
+    int rc = ns_phase<PH_A, T, MUON>(p, pl, gen, abc, s);
+    if (!rc) rc = ns_phase<PH_B, T, MUON>(p, pl, gen, abc, s);
+    if (!rc) rc = k + 1 < steps ? ns_phase<PH_X, T, MUON>(p, pl, gen, abc, s) : ns_phase<PH_LAST, T, MUON>(p, pl, gen, abc, s);
     if (rc) return rc;
   }
   return ITG_OK;
@@ -963,7 +925,7 @@ extern "C" {
 int64_t itg_newton_schulz_workspace(const itg_ns_job* jobs, int n, int dtype) {
   if (dtype < ITG_F32 || dtype > ITG_F16) return ITG_ERR_ARG;
   NsArgs p; NsPlan pl;
-  const int rc = ns_plan(jobs, n, dtype != ITG_BF16, false, p, pl);
+  const int rc = ns_plan(jobs, n, false, p, pl);
   return rc ? rc : pl.bytes;
 }
 
@@ -972,7 +934,7 @@ int itg_newton_schulz(const itg_ns_job* jobs, int n, int dtype, const void* g, v
   if (dtype < ITG_F32 || dtype > ITG_F16 || !g || !out || !coefficients || steps < 1 || steps > ITG_NS_MAX_STEPS || !(eps >= 0.f)) return ITG_ERR_ARG;
   if (((uintptr_t)g | (uintptr_t)out) & (dtype == ITG_F32 ? 3 : 1)) return ITG_ERR_ALIGN;
   NsArgs p; NsPlan pl;
-  const int rc = ns_plan(jobs, n, dtype != ITG_BF16, false, p, pl);
+  const int rc = ns_plan(jobs, n, false, p, pl);
   if (rc) return rc;
   if (!ns_coefficients_ok(coefficients, steps)) return ITG_ERR_ARG;
   if (!workspace || workspace_bytes < pl.bytes) return ITG_ERR_WORKSPACE;
@@ -980,9 +942,9 @@ int itg_newton_schulz(const itg_ns_job* jobs, int n, int dtype, const void* g, v
   p.ws = (char*)workspace; p.g = g; p.out = out; p.mom = nullptr; p.ema = nullptr; p.eps = eps; p.nesterov = 0;
   p.mu = p.lr = p.wd = p.ema_decay = 0.f;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == ITG_F32) return ns_run<float, true, false>(p, pl, coefficients, steps, s);
-  if (dtype == ITG_BF16) return ns_run<__bf16, false, false>(p, pl, coefficients, steps, s);
-  return ns_run<_Float16, true, false>(p, pl, coefficients, steps, s);
+  if (dtype == ITG_F32) return ns_run<float, false>(p, pl, coefficients, steps, s);
+  if (dtype == ITG_BF16) return ns_run<__bf16, false>(p, pl, coefficients, steps, s);
+  return ns_run<_Float16, false>(p, pl, coefficients, steps, s);
 }
 
 int itg_muon_step(const itg_ns_job* jobs, int n, float* param, const float* g, float* momentum, float* ema, float lr, float mu,
@@ -992,14 +954,14 @@ int itg_muon_step(const itg_ns_job* jobs, int n, float* param, const float* g, f
   if (param == g || param == momentum || g == momentum || ema == param || ema == g || ema == momentum) return ITG_ERR_ARG;
   if (((uintptr_t)param | (uintptr_t)g | (uintptr_t)momentum | (uintptr_t)ema) & 3) return ITG_ERR_ALIGN;
   NsArgs p; NsPlan pl;
-  const int rc = ns_plan(jobs, n, true, true, p, pl);
+  const int rc = ns_plan(jobs, n, true, p, pl);
   if (rc) return rc;
   if (!ns_coefficients_ok(coefficients, steps)) return ITG_ERR_ARG;
   if (!workspace || workspace_bytes < pl.bytes) return ITG_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return ITG_ERR_ALIGN;
   p.ws = (char*)workspace; p.g = g; p.out = param; p.mom = momentum; p.ema = ema; p.eps = eps; p.nesterov = nesterov ? 1 : 0;
   p.mu = mu; p.lr = lr; p.wd = weight_decay; p.ema_decay = ema_decay;
-  return ns_run<float, true, true>(p, pl, coefficients, steps, (hipStream_t)stream);
+  return ns_run<float, true>(p, pl, coefficients, steps, (hipStream_t)stream);
 }
 
 }  // extern "C"

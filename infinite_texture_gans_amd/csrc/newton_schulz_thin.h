@@ -9,25 +9,23 @@
 // What bounds it is latency: 16 matrices of 64 x 64 take 22 us in one launch, where the
 // general path's 17 launches take 80.
 
-template <int M, bool SPLIT> struct Thin {
-  static constexpr int NW = M / 16, NT = NW * 64, W = 128, PX = W + 8, PA = M + 8, NP = SPLIT ? 2 : 1;
+template <int M> struct Thin {
+  static constexpr int NW = M / 16, NT = NW * 64, W = 128, PX = W + 8, PA = M + 8;
   static constexpr int AR = 2, AC = M / 32, WAC = 2;               // A: fragments of a wave, waves side by side
   static constexpr int XR = W / NW / 16, XC = M / 16;              // X: a wave has XR * 16 columns of X and all rows
-  static constexpr int LDS_X = 2 * M * PX, LDS_A = NP * M * PA;    // halves
-  static constexpr int LDS = (LDS_X + LDS_A) * 2 + 2 * M * 4 + 16 * 8;
+  static constexpr int LDS_X = 2 * M * PX, LDS_A = 2 * M * PA;    // halves
+  static constexpr int LDS = (LDS_X + LDS_A) * 2 + 16 * 8;
   static constexpr int VEC = 8;                                    // vectors of 4 values of a block that a thread loads
 };
 
-template <int M, bool SPLIT> struct ThinLds {
-  typedef Thin<M, SPLIT> C;
+template <int M> struct ThinLds {
+  typedef Thin<M> C;
   _Float16 *x[2], *a[2];
-  float *da, *db;
   double* red;
   __device__ __forceinline__ explicit ThinLds(_Float16* lds) {
     x[0] = lds; x[1] = lds + M * C::PX;
-    a[0] = lds + C::LDS_X; a[1] = a[0] + (SPLIT ? M * C::PA : 0);
-    da = (float*)(lds + C::LDS_X + C::LDS_A); db = da + M;
-    red = (double*)(db + M);
+    a[0] = lds + C::LDS_X; a[1] = a[0] + M * C::PA;
+    red = (double*)(lds + C::LDS_X + C::LDS_A);
   }
 };
 
@@ -73,8 +71,8 @@ __device__ __forceinline__ void thin_load(const NsArgs& p, const NsMat& j, int z
   }
 }
 
-template <typename C, int M, bool SPLIT>
-__device__ __forceinline__ void thin_put(const ThinLds<M, SPLIT>& s, bool tall, const f32x4 (&v)[C::VEC], double inv) {
+template <typename C, int M>
+__device__ __forceinline__ void thin_put(const ThinLds<M>& s, bool tall, const f32x4 (&v)[C::VEC], double inv) {
 #pragma unroll
   for (int q = 0; q < C::VEC; ++q) {
     const int id = q * C::NT + threadIdx.x;
@@ -92,20 +90,19 @@ __device__ __forceinline__ void thin_put(const ThinLds<M, SPLIT>& s, bool tall, 
   }
 }
 
-// acc += hi hi (+ hi lo + lo hi) of fragments P[NP][R] and Q[NP][N]
-template <bool SPLIT, int R, int N>
-__device__ __forceinline__ void thin_mfma(f32x4 (&acc)[R][N], const f16x8 (&P)[SPLIT ? 2 : 1][R], const f16x8 (&Q)[SPLIT ? 2 : 1][N]) {
-  constexpr int L = SPLIT ? 1 : 0;
+// acc += lo hi + hi lo + hi hi of fragments P[hi, lo][R] and Q[hi, lo][N]
+template <int R, int N>
+__device__ __forceinline__ void thin_mfma(f32x4 (&acc)[R][N], const f16x8 (&P)[2][R], const f16x8 (&Q)[2][N]) {
 #pragma unroll
-  for (int q = SPLIT ? 0 : 2; q < 3; ++q)
+  for (int q = 0; q < 3; ++q)
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
-      for (int k = 0; k < N; ++k) acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[q == 0 ? L : 0][i], Q[q == 1 ? L : 0][k], acc[i][k], 0, 0, 0);
+      for (int k = 0; k < N; ++k) acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[q == 0][i], Q[q == 1][k], acc[i][k], 0, 0, 0);
 }
 
 // this wave's part of S S^T over `slices` x 32 of the planes' columns (pitch PITCH), added to acc
-template <typename C, int M, bool SPLIT, int PITCH>
+template <typename C, int M, int PITCH>
 __device__ __forceinline__ void thin_square(f32x4 (&acc)[C::AR][C::AC], _Float16* const* S, int slices) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, lk = lane >> 4;
   const int wr = wave / C::WAC * (C::AR * 16), wc = wave % C::WAC * (C::AC * 16);
@@ -115,15 +112,15 @@ __device__ __forceinline__ void thin_square(f32x4 (&acc)[C::AR][C::AC], _Float16
 #pragma unroll
     for (int k = 0; k < C::AC; ++k) part[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int ks = 0; ks < slices; ++ks) {
-    f16x8 P[C::NP][C::AR], Q[C::NP][C::AC];
+    f16x8 P[2][C::AR], Q[2][C::AC];
 #pragma unroll
-    for (int q = 0; q < C::NP; ++q) {
+    for (int q = 0; q < 2; ++q) {
 #pragma unroll
       for (int i = 0; i < C::AR; ++i) P[q][i] = *reinterpret_cast<const f16x8*>(S[q] + (wr + i * 16 + l15) * PITCH + ks * 32 + lk * 8);
 #pragma unroll
       for (int k = 0; k < C::AC; ++k) Q[q][k] = *reinterpret_cast<const f16x8*>(S[q] + (wc + k * 16 + l15) * PITCH + ks * 32 + lk * 8);
     }
-    thin_mfma<SPLIT, C::AR, C::AC>(part, P, Q);
+    thin_mfma<C::AR, C::AC>(part, P, Q);
   }
 #pragma unroll
   for (int i = 0; i < C::AR; ++i)
@@ -132,29 +129,23 @@ __device__ __forceinline__ void thin_square(f32x4 (&acc)[C::AR][C::AC], _Float16
 }
 
 // A from its sum, then B in its place.  The caller has a barrier before (what lay there has been read), one is behind.
-template <typename C, int M, bool SPLIT>
-__device__ __forceinline__ void thin_poly(const ThinLds<M, SPLIT>& s, f32x4 (&acc)[C::AR][C::AC], float cb, float cc) {
+template <typename C, int M>
+__device__ __forceinline__ void thin_poly(const ThinLds<M>& s, f32x4 (&acc)[C::AR][C::AC], float cb, float cc) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, lk = lane >> 4;
   const int wr = wave / C::WAC * (C::AR * 16) + lk * 4, wc = wave % C::WAC * (C::AC * 16) + l15;
-  auto put = [&](const f32x4& v0, int row0, int col, float* diag, float unit) {      // symmetric: four rows of a column are four of a row
-    f32x4 v = v0;
+  auto put = [&](const f32x4& v, int row0, int col) {      // symmetric: four rows of a column are four of a row
     f16x4 hi, lo;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (!SPLIT && row0 + e == col) { diag[col] = v[e] * unit; v[e] = 0.f; }
-      _Float16 h, l;
-      split_f16(v[e], h, l);
-      hi[e] = h; lo[e] = l;
-    }
+    for (int e = 0; e < 4; ++e) { _Float16 h, l; split_f16(v[e], h, l); hi[e] = h; lo[e] = l; }
     *reinterpret_cast<f16x4*>(s.a[0] + col * C::PA + row0) = hi;
-    if (SPLIT) *reinterpret_cast<f16x4*>(s.a[1] + col * C::PA + row0) = lo;
+    *reinterpret_cast<f16x4*>(s.a[1] + col * C::PA + row0) = lo;
   };
 #pragma unroll
   for (int i = 0; i < C::AR; ++i)
 #pragma unroll
-    for (int k = 0; k < C::AC; ++k) { put(acc[i][k] * (SA / (SX * SX)), wr + i * 16, wc + k * 16, s.da, 1.f / SA); acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+    for (int k = 0; k < C::AC; ++k) { put(acc[i][k] * (SA / (SX * SX)), wr + i * 16, wc + k * 16); acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f}; }
   __syncthreads();
-  thin_square<C, M, SPLIT, C::PA>(acc, s.a, M / 32);
+  thin_square<C, M, C::PA>(acc, s.a, M / 32);
 #pragma unroll
   for (int i = 0; i < C::AR; ++i)
 #pragma unroll
@@ -163,10 +154,7 @@ __device__ __forceinline__ void thin_poly(const ThinLds<M, SPLIT>& s, f32x4 (&ac
       const f16x4 ah = *reinterpret_cast<const f16x4*>(s.a[0] + col * C::PA + row0), al = *reinterpret_cast<const f16x4*>(s.a[1] + col * C::PA + row0);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float a1 = (float)ah[e] * (1.f / SA), a2 = acc[i][k][e] * (1.f / (SA * SA));
-        if (SPLIT) a1 += (float)al[e] * (1.f / SA);
-        else if (row0 + e == col) { a1 = s.da[col]; a2 = fmaf(a1, a1, a2); }
-        else a2 = fmaf(s.da[row0 + e] + s.da[col], a1, a2);
+        const float a1 = (float)ah[e] * (1.f / SA) + (float)al[e] * (1.f / SA), a2 = acc[i][k][e] * (1.f / (SA * SA));
         acc[i][k][e] = (cb * a1 + cc * a2) * SB;
       }
     }
@@ -174,13 +162,13 @@ __device__ __forceinline__ void thin_poly(const ThinLds<M, SPLIT>& s, f32x4 (&ac
 #pragma unroll
   for (int i = 0; i < C::AR; ++i)
 #pragma unroll
-    for (int k = 0; k < C::AC; ++k) put(acc[i][k], wr + i * 16, wc + k * 16, s.db, 1.f / SB);
+    for (int k = 0; k < C::AC; ++k) put(acc[i][k], wr + i * 16, wc + k * 16);
   __syncthreads();
 }
 
 // this wave's columns of the block: X <- a X + B X, in place, or the result
-template <typename C, int M, bool SPLIT, bool LAST, typename OUT, bool MUON>
-__device__ __forceinline__ void thin_update(const ThinLds<M, SPLIT>& s, const NsArgs& p, const NsMat& j, int z, int j0, float ca) {
+template <typename C, int M, bool LAST, typename OUT, bool MUON>
+__device__ __forceinline__ void thin_update(const ThinLds<M>& s, const NsArgs& p, const NsMat& j, int z, int j0, float ca) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, lk = lane >> 4, c0 = wave * C::XR * 16;
   if (j0 + c0 >= j.n) return;                              // zeros behind the matrix stay
   f32x4 acc[C::XR][C::XC];
@@ -190,15 +178,15 @@ __device__ __forceinline__ void thin_update(const ThinLds<M, SPLIT>& s, const Ns
     for (int k = 0; k < C::XC; ++k) acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int ks = 0; ks < M / 32; ++ks) {
-    f16x8 P[C::NP][C::XR], Q[C::NP][C::XC];
+    f16x8 P[2][C::XR], Q[2][C::XC];
 #pragma unroll
-    for (int q = 0; q < C::NP; ++q) {
+    for (int q = 0; q < 2; ++q) {
 #pragma unroll
       for (int i = 0; i < C::XR; ++i) P[q][i] = frag_t<C::PX>(s.x[q] + (ks * 32 + lk * 8 + (l15 >> 2)) * C::PX + c0 + i * 16 + (l15 & 3) * 4);
 #pragma unroll
       for (int k = 0; k < C::XC; ++k) Q[q][k] = *reinterpret_cast<const f16x8*>(s.a[q] + (k * 16 + l15) * C::PA + ks * 32 + lk * 8);
     }
-    thin_mfma<SPLIT, C::XR, C::XC>(acc, P, Q);
+    thin_mfma<C::XR, C::XC>(acc, P, Q);
   }
 #pragma unroll
   for (int i = 0; i < C::XR; ++i)
@@ -207,13 +195,11 @@ __device__ __forceinline__ void thin_update(const ThinLds<M, SPLIT>& s, const Ns
       const int row0 = c0 + i * 16 + lk * 4, col = k * 16 + l15;
       _Float16 *xh = s.x[0] + col * C::PX + row0, *xl = s.x[1] + col * C::PX + row0;
       const f16x4 oh = *reinterpret_cast<const f16x4*>(xh), ol = *reinterpret_cast<const f16x4*>(xl);
-      const float d = SPLIT ? 0.f : s.db[col];
       f32x4 v;
       f16x4 hi, lo;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         v[e] = fmaf(ca, (float)oh[e] + (float)ol[e], acc[i][k][e] * (1.f / SB));
-        if (!SPLIT) v[e] = fmaf(d, (float)oh[e], v[e]);
         _Float16 h, l;
         split_f16(v[e], h, l);
         hi[e] = h; lo[e] = l;
@@ -230,11 +216,11 @@ __device__ __forceinline__ void thin_update(const ThinLds<M, SPLIT>& s, const Ns
 // ---- one launch: 1 / |G|, all steps, the result
 struct NsSteps { float abc[3 * ITG_NS_MAX_STEPS]; int n; };
 
-template <int M, bool SPLIT, typename T, bool MUON>
-__global__ __launch_bounds__((Thin<M, SPLIT>::NT)) void ns_thin_all_kernel(NsArgs p, NsSteps st) {
-  typedef Thin<M, SPLIT> C;
+template <int M, typename T, bool MUON>
+__global__ __launch_bounds__((Thin<M>::NT)) void ns_thin_all_kernel(NsArgs p, NsSteps st) {
+  typedef Thin<M> C;
   extern __shared__ __attribute__((aligned(16))) _Float16 lds[];
-  const ThinLds<M, SPLIT> s(lds);
+  const ThinLds<M> s(lds);
   const NsMat& j = p.j[ns_job(p, blockIdx.x, [](const NsMat& q) { return q.block0; })];
   const int z = blockIdx.x - j.block0;
   f32x4 v[C::VEC];
@@ -250,14 +236,14 @@ __global__ __launch_bounds__((Thin<M, SPLIT>::NT)) void ns_thin_all_kernel(NsArg
   sum = 0.0;
 #pragma unroll
   for (int q = 0; q < C::NW; ++q) sum += s.red[q];
-  thin_put<C, M, SPLIT>(s, j.tall, v, ns_scale(sum, p.eps));
+  thin_put<C, M>(s, j.tall, v, ns_scale(sum, p.eps));
   for (int k = 0; k < st.n; ++k) {
     __syncthreads();                                       // X is whole, B has been read
     f32x4 acc[C::AR][C::AC] = {};
-    thin_square<C, M, SPLIT, C::PX>(acc, s.x, (j.n + 31) / 32);      // n <= 128: no more of the block than the matrix fills
-    thin_poly<C, M, SPLIT>(s, acc, st.abc[3 * k + 1], st.abc[3 * k + 2]);
-    if (k + 1 < st.n) thin_update<C, M, SPLIT, false, T, MUON>(s, p, j, z, 0, st.abc[3 * k]);
-    else thin_update<C, M, SPLIT, true, T, MUON>(s, p, j, z, 0, st.abc[3 * k]);
+    thin_square<C, M, C::PX>(acc, s.x, (j.n + 31) / 32);      // n <= 128: no more of the block than the matrix fills
+    thin_poly<C, M>(s, acc, st.abc[3 * k + 1], st.abc[3 * k + 2]);
+    if (k + 1 < st.n) thin_update<C, M, false, T, MUON>(s, p, j, z, 0, st.abc[3 * k]);
+    else thin_update<C, M, true, T, MUON>(s, p, j, z, 0, st.abc[3 * k]);
   }
 }
 
@@ -279,8 +265,8 @@ __device__ __forceinline__ ThinWs thin_ws(char* base, int M, int np, int blocks)
 }
 
 // this wave's columns of the block from LDS to the planes
-template <typename C, int M, bool SPLIT>
-__device__ __forceinline__ void thin_keep(const ThinLds<M, SPLIT>& s, const ThinWs& w, int np, int j0) {
+template <typename C, int M>
+__device__ __forceinline__ void thin_keep(const ThinLds<M>& s, const ThinWs& w, int np, int j0) {
   constexpr int CH = C::XR * 2;                            // 16-byte chunks of a row
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the wave's own writes, read by its other lanes
@@ -303,11 +289,11 @@ __device__ __forceinline__ void thin_share(const f32x4 (&acc)[C::AR][C::AC], flo
 }
 
 // the planes of X and the shares of the first A
-template <int M, bool SPLIT, typename T, bool MUON>
-__global__ __launch_bounds__((Thin<M, SPLIT>::NT)) void ns_thin_first_kernel(NsArgs p) {
-  typedef Thin<M, SPLIT> C;
+template <int M, typename T, bool MUON>
+__global__ __launch_bounds__((Thin<M>::NT)) void ns_thin_first_kernel(NsArgs p) {
+  typedef Thin<M> C;
   extern __shared__ __attribute__((aligned(16))) _Float16 lds[];
-  const ThinLds<M, SPLIT> s(lds);
+  const ThinLds<M> s(lds);
   const NsMat& j = p.j[ns_job(p, blockIdx.x, [](const NsMat& q) { return q.block0; })];
   const int local = blockIdx.x - j.block0, z = local / j.blocks, b = local - z * j.blocks;
   const ThinWs w = thin_ws(p.ws + j.ws + z * j.wst, M, j.np, j.blocks);
@@ -326,19 +312,19 @@ __global__ __launch_bounds__((Thin<M, SPLIT>::NT)) void ns_thin_first_kernel(NsA
   f32x4 acc[C::AR][C::AC] = {};
   for (int j0 = first; j0 < end; j0 += C::W) {
     if (j0 != first) { thin_load<C, M, T, MUON, false>(p, j, z, j0, v); __syncthreads(); }      // the block before has been read
-    thin_put<C, M, SPLIT>(s, j.tall, v, inv);
+    thin_put<C, M>(s, j.tall, v, inv);
     __syncthreads();
-    thin_keep<C, M, SPLIT>(s, w, j.np, j0);
-    thin_square<C, M, SPLIT, C::PX>(acc, s.x, C::W / 32);
+    thin_keep<C, M>(s, w, j.np, j0);
+    thin_square<C, M, C::PX>(acc, s.x, C::W / 32);
   }
   thin_share<C>(acc, w.slab[0] + (int64_t)b * M * M);
 }
 
-template <int M, bool SPLIT, bool LAST, typename T, bool MUON>
-__global__ __launch_bounds__((Thin<M, SPLIT>::NT)) void ns_thin_step_kernel(NsArgs p, int gen, float ca, float cb, float cc) {
-  typedef Thin<M, SPLIT> C;
+template <int M, bool LAST, typename T, bool MUON>
+__global__ __launch_bounds__((Thin<M>::NT)) void ns_thin_step_kernel(NsArgs p, int gen, float ca, float cb, float cc) {
+  typedef Thin<M> C;
   extern __shared__ __attribute__((aligned(16))) _Float16 lds[];
-  const ThinLds<M, SPLIT> s(lds);
+  const ThinLds<M> s(lds);
   const NsMat& j = p.j[ns_job(p, blockIdx.x, [](const NsMat& q) { return q.block0; })];
   const int local = blockIdx.x - j.block0, z = local / j.blocks, b = local - z * j.blocks;
   const ThinWs w = thin_ws(p.ws + j.ws + z * j.wst, M, j.np, j.blocks);
@@ -359,7 +345,7 @@ __global__ __launch_bounds__((Thin<M, SPLIT>::NT)) void ns_thin_step_kernel(NsAr
     for (int i = 0; i < C::AR; ++i)
 #pragma unroll
       for (int k = 0; k < C::AC; ++k) acc[i][k] += from[(int64_t)q * (M * M / 4) + (i * C::AC + k) * C::NT];
-  thin_poly<C, M, SPLIT>(s, acc, cb, cc);
+  thin_poly<C, M>(s, acc, cb, cc);
 #pragma unroll
   for (int i = 0; i < C::AR; ++i)
 #pragma unroll
@@ -371,11 +357,11 @@ __global__ __launch_bounds__((Thin<M, SPLIT>::NT)) void ns_thin_step_kernel(NsAr
 #pragma unroll
       for (int k = 0; k < 4; ++k) { const int id = k * C::NT + threadIdx.x; *reinterpret_cast<f16x8*>(s.x[q] + (id >> 4) * C::PX + (id & 15) * 8) = u[q][k]; }
     __syncthreads();
-    thin_update<C, M, SPLIT, LAST, T, MUON>(s, p, j, z, j0, ca);
+    thin_update<C, M, LAST, T, MUON>(s, p, j, z, j0, ca);
     if (!LAST) {
-      thin_keep<C, M, SPLIT>(s, w, j.np, j0);
+      thin_keep<C, M>(s, w, j.np, j0);
       __syncthreads();
-      thin_square<C, M, SPLIT, C::PX>(acc, s.x, C::W / 32);
+      thin_square<C, M, C::PX>(acc, s.x, C::W / 32);
     }
   }
   if (!LAST) thin_share<C>(acc, w.slab[gen ^ 1] + (int64_t)b * M * M);

@@ -1776,7 +1776,7 @@ def orthogonalize(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-12, out=None)
     """The matrices (..., rows, columns) of ``g`` with their singular values driven towards 1 by ``steps`` Newton-Schulz products
     (the direction of a Muon update; no gradient flows through it).
 
-    float32 / float16: products as exact as fp32 ones; bfloat16: as exact as the type.  ``g`` may be strided (row- or column-major
+    Products are as exact as fp32 ones for every type, and the result is rounded once.  ``g`` may be strided (row- or column-major
     matrices at one batch stride are read in place).  ``coefficients``: (a, b, c) of X <- a X + (b A + c A A) X, or one triple per
     step.  A matrix with a norm of ``eps`` or less has no direction and gives zeros; one with a NaN or an infinity gives NaN.
     ``out``: a contiguous tensor like ``g`` for the result, which may be ``g`` itself where that is contiguous and otherwise lies

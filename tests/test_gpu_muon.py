@@ -350,3 +350,15 @@ def test_captured_calls_of_every_path(ops, t, m, n, batch):
         torch.cuda.synchronize()
         assert torch.equal(o, ops.orthogonalize(static)), k
         o.zero_()
+
+
+@pytest.mark.parametrize("m,n", [(8, 8), (16, 64), (64, 64), (64, 128), (128, 100), (13, 1000), (100, 1000), (333, 1501), (512, 512), (700, 1100), (1030, 2100)])
+def test_bf16_results_are_rounded_once(ops, m, n):
+    """A bf16 matrix is held in no fewer bits than a float32 one: its result is the float32 path's, rounded at the end.  With y the
+    unrounded result and |y - want| <= e (the float32 tests' bound), |bf16(y) - want| <= |bf16(y) - y| + e, and as the distance to
+    the nearest bf16 value changes by no more than its argument does, <= |bf16(want) - want| + 2 e."""
+    g = matrix(m, n, seed=m + 3 * n).bfloat16()
+    want = steps_of(g.double())
+    e = max(3 * rel(steps_of(g.float()), want), 2e-6)
+    off, once = rel(ops.orthogonalize(g.cuda()).cpu(), want), rel(want.bfloat16(), want)
+    assert off <= once + 2 * e, (off, once, e)
