@@ -6,8 +6,7 @@
 // Statistics, sums and products are fp32 whatever the tensors' type; the variance is taken around the mean of the row (a second
 // sweep over values that are already on the chip), never as a difference of moments.  Every sum has a fixed order: results do
 // not change from call to call.
-#include <type_traits>
-#include "itg_common.h"
+#include "layer_norm_rows.h"
 
 namespace {
 
@@ -27,49 +26,6 @@ __device__ __forceinline__ float act_slope_at(float u, int act, float slope) {
   if (act == ITG_ACT_TANH) { const float t = tanhf(u); return 1.f - t * t; }
   return 1.f;
 }
-
-// ---- rows held in registers.  A row of c values is cut into vectors of V (16 bytes; single values where c < V); TPR threads share a
-// row and a thread holds the R vectors tid, tid + TPR, ...  The last vector of a row that V does not divide either starts at c - V
-// and masks what it shares with its neighbour (both write the same values there), or, in rows with zero padding behind the
-// channels, lies where it belongs and masks the padding.  Vector loads and stores need the element's alignment only.
-struct LnV { int nv, off_last, lo_last, hi_last; };      // vectors per row; start of the last one and its valid elements [lo, hi)
-
-__host__ __device__ inline LnV ln_vectors(int c, int pad, int V) {
-  LnV v;
-  v.nv = (c + V - 1) / V;
-  const bool padded = pad > 0 && pad < V && (c + pad) % V == 0;
-  v.off_last = padded ? (v.nv - 1) * V : c - V;
-  v.lo_last = (v.nv - 1) * V - v.off_last;
-  v.hi_last = padded ? c - v.off_last : V;
-  return v;
-}
-
-template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[V]; };
-
-// V values as they lie in memory, in 32-bit words (a Pack of 16-bit values takes a register each)
-template <typename T, int V> struct Held {
-  static constexpr int N = (V * (int)sizeof(T) + 3) / 4;
-  uint32_t w[N];
-  __device__ __forceinline__ float at(int e) const {
-    if (sizeof(T) == 4) return __builtin_bit_cast(float, w[e]);
-    return (float)__builtin_bit_cast(T, (typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type)(w[e / 2] >> (16 * (e & 1))));
-  }
-  __device__ __forceinline__ void load(const T* q) {
-    struct __attribute__((packed, aligned(sizeof(T)))) Words { uint32_t w[N]; };
-    if (V * sizeof(T) % 4 == 0) {
-      const Words u = *reinterpret_cast<const Words*>(q);
-#pragma unroll
-      for (int i = 0; i < N; ++i) w[i] = u.w[i];
-    } else {
-      w[0] = *reinterpret_cast<const uint16_t*>(q);
-    }
-  }
-  // the compiler takes the values for changed: what is computed from them again is not carried over in registers instead
-  __device__ __forceinline__ void renew() {
-#pragma unroll
-    for (int i = 0; i < N; ++i) asm("" : "+v"(w[i]));
-  }
-};
 
 // The R vectors of a thread in row `q`.  A thread that has none reads the row's last one, and ln_take makes zeros of it: a load behind
 // a branch is waited for at the branch's end.
@@ -196,10 +152,7 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
   Held<T, V> mine[R];                   // the bits of the values it reads and writes
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int i = tid + r * TPR;
-    off[r] = i < lv.nv - 1 ? i * V : lv.off_last;
-    lo[r] = i < lv.nv - 1 ? 0 : lv.lo_last;
-    hi[r] = i < lv.nv - 1 ? V : i < lv.nv ? lv.hi_last : 0;
+    ln_place(lv, tid + r * TPR, V, off[r], lo[r], hi[r]);
     if (MASK) {
       ln_bits<T, V>(hi[r], mine[r]);
 #pragma unroll
@@ -279,18 +232,16 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
   Held<W, V> tw[R] = {}, tb[R] = {};
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int i = tid + r * TPR;
-    off[r] = i < lv.nv - 1 ? i * V : lv.off_last;
-    lo[r] = i < lv.nv - 1 ? 0 : lv.lo_last;
-    hi[r] = i < lv.nv - 1 ? V : i < lv.nv ? lv.hi_last : 0;
+    ln_place(lv, tid + r * TPR, V, off[r], lo[r], hi[r]);
     if (MASK) {
       ln_bits<T, V>(hi[r], mine[r]);
 #pragma unroll
       for (int e = 0; e < V; ++e) m[r][e] = e >= lo[r] && e < hi[r] ? 1.f : 0.f;
     }
     if (TIGHT) {
-      if (hi[r] > 0 && p.w) tw[r].load((const W*)p.w + off[r]);
-      if (ACT && hi[r] > 0 && p.b) tb[r].load((const W*)p.b + off[r]);
+      // (gamma and beta hold c values: a padded row's last vector ends behind them)
+      if (hi[r] > 0 && p.w) tw[r].load_first((const W*)p.w + off[r], MASK ? hi[r] : V);
+      if (ACT && hi[r] > 0 && p.b) tb[r].load_first((const W*)p.b + off[r], hi[r]);
     } else {
       ln_param<W, V, MASK>(p.w, off[r], hi[r], 1.f, w[r]);
       ln_param<W, V, MASK>(ACT ? p.b : nullptr, off[r], hi[r], 0.f, b[r]);

@@ -216,3 +216,65 @@ def test_training_operators_have_no_cpu_path():
                  lambda: ops.layer_norm(ops.GT(x.view(1, 1, 1, 1, 4, 8), 8))):
         with pytest.raises(ItgError):
             call()
+
+
+ROWS_PROGRAM = r"""
+#include "layer_norm_rows.h"
+#include <stdio.h>
+#include <string.h>
+#include <sys/mman.h>
+#include <unistd.h>
+// gamma ends where readable memory ends: a read behind its c values does not come back
+template <typename W> int run(char* end, int c, int pad, int threads, int per) {
+  W* gamma = (W*)end - c;
+  for (int i = 0; i < c; ++i) { uint32_t b = 0x3f80u + (uint32_t)(i % 97); memcpy(gamma + i, &b, sizeof(W)); }
+  const LnV lv = ln_vectors(c, pad, 8);
+  int seen = 0;
+  for (int i = 0; i < threads * per; ++i) {
+    int off, lo, hi;
+    ln_place(lv, i, 8, off, lo, hi);
+    if (off < 0 || off + 8 > c + pad || lo < 0 || hi > 8) return 1;
+    if (hi <= 0) continue;
+    Held<W, 8> k;
+    memset(&k, 0xff, sizeof(k));
+    k.load_first(gamma + off, hi);
+    W got[8], want[8];
+    memcpy(got, &k, sizeof(got));
+    memset(want, 0, sizeof(want));
+    memcpy(want, gamma + off, hi * sizeof(W));
+    if (memcmp(got, want, sizeof(got))) return 2;
+    for (int e = lo; e < hi; ++e) seen += off + e < c;
+  }
+  return seen == c ? 0 : 3;
+}
+int main() {
+  const size_t page = (size_t)sysconf(_SC_PAGESIZE), room = (16384 * 4 + page - 1) / page * page;
+  char* mem = (char*)mmap(0, room + page, PROT_READ | PROT_WRITE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0);
+  if (mem == (char*)MAP_FAILED || mprotect(mem + room, page, PROT_NONE)) return 9;
+  for (int c = 8193; c <= 16384; c += c < 8300 || c > 16300 ? 1 : 61)
+    for (int pad = 0; pad < 12; ++pad) {
+      if (c + pad > 16384 && pad) continue;
+      const int a = run<float>(mem + room, c, pad, 1024, 2), b = run<_Float16>(mem + room, c, pad, 1024, 2);
+      if (a || b) { printf("%d %d: %d %d\n", c, pad, a, b); return 1; }
+    }
+  return 0;
+}
+"""
+
+
+def test_layer_norm_parameters_are_read_to_their_last_value(tmp_path):
+    """long 16-bit rows with padding: the vector of gamma and beta that ends in the padding is read value by value.  The kernel's own
+    placement and load, compiled for the host, over a gamma behind whose last value no memory can be read."""
+    import shutil
+    import subprocess
+    import __graft_entry__ as g
+    if shutil.which(g.HIPCC) is None:
+        pytest.skip("hipcc not installed")
+    src, exe = tmp_path / "rows.hip", tmp_path / "rows"
+    src.write_text(ROWS_PROGRAM)
+    subprocess.check_call([g.HIPCC, "-x", "hip", "--cuda-host-only", "-O1", "-std=c++17", "-I", g.CSRC, "-I", os.path.join(ROOT, "include"), str(src),
+                           "-o", str(exe)])
+    assert subprocess.run([str(exe)]).returncode == 0
+    with open(os.path.join(g.CSRC, "layer_norm.hip")) as f:      # the kernels' only other whole-vector reads of gamma and beta: ln_param's, ln_at's
+        kernel = f.read()
+    assert kernel.count(".load_first((const W*)p.") == 2 and ".load((const W*)" not in kernel

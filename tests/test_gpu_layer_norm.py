@@ -486,3 +486,23 @@ def test_vectors_at_odd_addresses(ops, rows, c, t):
     assert shift(x).data_ptr() % 16 and torch.equal(y, y1)
     for p, q in zip(grads, g1):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("t,dt,tw,pdt", [(torch.bfloat16, 1, torch.float32, 0), (torch.bfloat16, 1, torch.bfloat16, 1), (torch.float16, 2, torch.float32, 0)])
+@pytest.mark.parametrize("act", [0, 1])
+def test_nothing_behind_the_parameters_counts(ops, t, dt, tw, pdt, act):
+    """rows of 16-bit values whose padding fills their last vector: NaN behind gamma's and beta's last value changes no bit"""
+    rows, c, pad = 600, 9001, 7
+    ld = c + pad
+    x, w, b, dy = make(rows, ld, t, tw, seed=6)
+    x[:, c:], dy[:, c:], w[c:], b[c:] = float("inf"), float("nan"), float("nan"), float("nan")
+    ws = torch.empty(ops._lib.fn("itg_layer_norm_bwd_workspace")(rows, c), device="cuda")
+    y, stat, dx = torch.empty_like(x), torch.empty(2 * rows, device="cuda"), torch.empty_like(x)
+    dw, db = torch.empty(c, device="cuda", dtype=tw), torch.empty(c, device="cuda", dtype=tw)
+    assert call("itg_layer_norm_fwd", x, ld, w, b, y, ld, stat, rows, c, pad, dt, pdt, 1e-5, act, 0.1) == 0
+    assert call("itg_layer_norm_bwd", x, ld, dy, ld, stat, w, b, dx, ld, dw, db, 0, rows, c, pad, dt, pdt, act, 0.1, ws, ws.numel()) == 0
+    xs, ps = x[:, :c].contiguous().requires_grad_(), [w[:c].clone().requires_grad_(), b[:c].clone().requires_grad_()]
+    ys = ops.layer_norm(xs, *ps, act=act, slope=0.1)
+    want = torch.autograd.grad(ys, [xs] + ps, dy[:, :c].contiguous())
+    assert torch.equal(y[:, :c], ys) and not y[:, c:].any()
+    assert torch.equal(dx[:, :c], want[0]) and not dx[:, c:].any() and torch.equal(dw, want[1]) and torch.equal(db, want[2])
