@@ -520,8 +520,6 @@ __global__ __launch_bounds__(1024) void ln_dw_reduce_kernel(const float* __restr
   }
 }
 
-constexpr int LN_CHUNKS = 1024;      // at most this many shares of dw | db
-inline int ln_chunks(int64_t rows) { return (int)(rows < LN_CHUNKS ? rows : LN_CHUNKS); }
 inline unsigned ln_grid(int64_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); }
 
 template <int V> inline int ln_kind(const LnP& p) { return p.act != ITG_ACT_NONE ? LN_ACT : p.c % V != 0 || p.pad != 0 ? LN_MASK : LN_PLAIN; }
@@ -540,14 +538,11 @@ int ln_fwd_run(const LnP& p, hipStream_t s) {
 }
 
 // Threads per row and vectors per thread: as few threads as hold the row at one vector each up to a wave; beyond, workgroups of
-// 128 .. 1024 threads at two vectors each.  Backward: up to two vectors in a wave (65536 x 1023 bf16 96 us, in two waves of one each
-// 120, where 1024 shares of dw | db are 8 waves a CU), then one of 8 or two of 4, as it keeps six values per channel it holds; at
-// two of 8 its row stays in 16 bits, see there.
+// 128 .. 1024 threads at two vectors each.  The backward pass's: ln_bwd_threads.
 template <typename T, typename W>
 int ln_fwd_t(const LnP& p, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  const int padded = p.pad > 0 && p.pad < V && (p.c + p.pad) % V == 0;
-  if (p.c < V && !padded) return p.c <= 4 ? ln_fwd_run<T, W, 1, 4, 1>(p, s) : ln_fwd_run<T, W, 1, 8, 1>(p, s);
+  if (p.c < V && !ln_padded(p.c, p.pad, V)) return p.c <= 4 ? ln_fwd_run<T, W, 1, 4, 1>(p, s) : ln_fwd_run<T, W, 1, 8, 1>(p, s);
   const int nv = (p.c + V - 1) / V;
   if (nv <= 4) return ln_fwd_run<T, W, V, 4, 1>(p, s);
   if (nv <= 8) return ln_fwd_run<T, W, V, 8, 1>(p, s);
@@ -564,18 +559,15 @@ int ln_fwd_t(const LnP& p, hipStream_t s) {
   return ITG_OK;
 }
 
-// workgroups of the backward pass over rows in registers: each leaves one share of dw | db
+// rows in registers; a workgroup leaves one share of dw | db
 template <typename T, typename W, int V, int TPR, int R>
-int ln_bwd_run(const LnP& p, int& chunks, hipStream_t s) {
-  constexpr int NT = TPR > 64 ? TPR : 256, GROUPS = NT / TPR;
-  const int64_t need = (p.rows + GROUPS - 1) / GROUPS, few = need / 4 > 256 ? need / 4 : 256;
-  // every CU has a workgroup before one gets fewer than four turns: a share costs a write and a read of 2 c floats
-  const int64_t most = 256 * (1024 / NT) < LN_CHUNKS ? (256 * (1024 / NT) < few ? 256 * (1024 / NT) : few) : (LN_CHUNKS < few ? LN_CHUNKS : few);
-  chunks = (int)(need < most ? need : most);
+int ln_bwd_run(const LnP& p, hipStream_t s) {
+  constexpr int NT = TPR > 64 ? TPR : 256;
+  const dim3 grid((unsigned)ln_bwd_groups(p.rows, TPR));
   const int kind = ln_kind<V>(p);
-  if (kind == LN_ACT) hipLaunchKernelGGL((ln_bwd_kernel<T, W, V, TPR, R, LN_ACT>), dim3(chunks), dim3(NT), 0, s, p);
-  else if (kind == LN_MASK) hipLaunchKernelGGL((ln_bwd_kernel<T, W, V, TPR, R, LN_MASK>), dim3(chunks), dim3(NT), 0, s, p);
-  else hipLaunchKernelGGL((ln_bwd_kernel<T, W, V, TPR, R, LN_PLAIN>), dim3(chunks), dim3(NT), 0, s, p);
+  if (kind == LN_ACT) hipLaunchKernelGGL((ln_bwd_kernel<T, W, V, TPR, R, LN_ACT>), grid, dim3(NT), 0, s, p);
+  else if (kind == LN_MASK) hipLaunchKernelGGL((ln_bwd_kernel<T, W, V, TPR, R, LN_MASK>), grid, dim3(NT), 0, s, p);
+  else hipLaunchKernelGGL((ln_bwd_kernel<T, W, V, TPR, R, LN_PLAIN>), grid, dim3(NT), 0, s, p);
   ITG_CHECK_LAUNCH();
   return ITG_OK;
 }
@@ -583,35 +575,24 @@ int ln_bwd_run(const LnP& p, int& chunks, hipStream_t s) {
 template <typename T, typename W>
 int ln_bwd_t(LnP p, void* dw, void* db, int acc, hipStream_t s) {
   constexpr int V = 16 / sizeof(T), K = V == 8 ? 1 : 2;      // K: vectors per thread of the workgroup sizes
-  const int nv = (p.c + V - 1) / V, padded = p.pad > 0 && p.pad < V && (p.c + p.pad) % V == 0;
+  const int nv = (p.c + V - 1) / V, threads = ln_bwd_threads(p.rows, p.c, p.pad, V), chunks = ln_bwd_shares(p.rows, p.c, p.pad, V);
   const bool shares = dw || db;
-  // A row in registers is read once, but every workgroup leaves a share of dw | db, 16 bytes a channel written and read, where the
-  // kernels for any length read the row three times and leave a share per 8 rows: those for few long rows (bf16, 8192 channels:
-  // 256 rows 24.4 us in registers, 16.0 swept; 768 rows 25.5, 30.5; 16384 channels: 512 rows 43, 33; 1536 rows 59, 81)
-  const bool few = p.c >= 8192 && p.rows * 16 < p.c;
-  int chunks = 0, rc = ITG_OK;
+  int rc = ITG_OK;
   if (!shares) p.part = nullptr;
-  if (p.c < V && !padded) rc = p.c <= 4 ? ln_bwd_run<T, W, 1, 4, 1>(p, chunks, s) : ln_bwd_run<T, W, 1, 8, 1>(p, chunks, s);
-  else if (nv <= 4) rc = ln_bwd_run<T, W, V, 4, 1>(p, chunks, s);
-  else if (nv <= 8) rc = ln_bwd_run<T, W, V, 8, 1>(p, chunks, s);
-  else if (nv <= 16) rc = ln_bwd_run<T, W, V, 16, 1>(p, chunks, s);
-  else if (nv <= 32) rc = ln_bwd_run<T, W, V, 32, 1>(p, chunks, s);
-  else if (nv <= 64) rc = ln_bwd_run<T, W, V, 64, 1>(p, chunks, s);
-  else if (nv <= 128) rc = ln_bwd_run<T, W, V, 64, 2>(p, chunks, s);
-  else if (K == 2 && nv <= 256) rc = ln_bwd_run<T, W, V, K == 2 ? 128 : 256, K>(p, chunks, s);
-  else if (nv <= 256 * K) rc = ln_bwd_run<T, W, V, 256, K>(p, chunks, s);
-  else if (nv <= 512 * K) rc = ln_bwd_run<T, W, V, 512, K>(p, chunks, s);
-  else if (nv <= 1024 * K && !few) rc = ln_bwd_run<T, W, V, 1024, K>(p, chunks, s);
-  else if (nv <= 2048 && !few) rc = ln_bwd_run<T, W, V, 1024, 2>(p, chunks, s);
+  if (p.c < V && !ln_padded(p.c, p.pad, V)) rc = threads == 4 ? ln_bwd_run<T, W, 1, 4, 1>(p, s) : ln_bwd_run<T, W, 1, 8, 1>(p, s);
+  else if (threads == 4) rc = ln_bwd_run<T, W, V, 4, 1>(p, s);
+  else if (threads == 8) rc = ln_bwd_run<T, W, V, 8, 1>(p, s);
+  else if (threads == 16) rc = ln_bwd_run<T, W, V, 16, 1>(p, s);
+  else if (threads == 32) rc = ln_bwd_run<T, W, V, 32, 1>(p, s);
+  else if (threads == 64) rc = nv <= 64 ? ln_bwd_run<T, W, V, 64, 1>(p, s) : ln_bwd_run<T, W, V, 64, 2>(p, s);
+  else if (K == 2 && threads == 128) rc = ln_bwd_run<T, W, V, K == 2 ? 128 : 256, K>(p, s);
+  else if (threads == 256) rc = ln_bwd_run<T, W, V, 256, K>(p, s);
+  else if (threads == 512) rc = ln_bwd_run<T, W, V, 512, K>(p, s);
+  else if (threads == 1024) rc = nv <= 1024 * K ? ln_bwd_run<T, W, V, 1024, K>(p, s) : ln_bwd_run<T, W, V, 1024, 2>(p, s);
   else {
     // (the shares read every row of dy and x, and dx may be written over either)
     if (shares) {
-      // about 2048 workgroups in all, and no share of fewer than 8 rows
-      const int cols = (nv + 255) / 256;
-      const int64_t want = 2048 / cols + 1, most = (p.rows + 7) / 8, k = want < most ? want : most;
-      const int64_t chunk = (p.rows + k - 1) / k;
-      chunks = (int)((p.rows + chunk - 1) / chunk);
-      hipLaunchKernelGGL((ln_dw_any_kernel<T, W, V>), dim3(cols, chunks), dim3(256), 0, s, p, chunk);
+      hipLaunchKernelGGL((ln_dw_any_kernel<T, W, V>), dim3((nv + 255) / 256, chunks), dim3(256), 0, s, p, ln_bwd_chunk(p.rows, p.c, V));
       ITG_CHECK_LAUNCH();
     }
     if (p.y) {
@@ -667,7 +648,7 @@ int itg_layer_norm_fwd(const void* x, int64_t ldx, const void* gamma, const void
 
 int64_t itg_layer_norm_bwd_workspace(int64_t rows, int c) {
   if (rows <= 0 || c <= 0 || c > ITG_LN_MAX_C) return ITG_ERR_ARG;
-  return (int64_t)ln_chunks(rows) * 2 * c;
+  return (int64_t)ln_bwd_most_shares(rows, c) * 2 * c;
 }
 
 int itg_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, const float* mean_rstd, const void* gamma,

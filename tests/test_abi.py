@@ -278,3 +278,18 @@ def test_layer_norm_parameters_are_read_to_their_last_value(tmp_path):
     with open(os.path.join(g.CSRC, "layer_norm.hip")) as f:      # the kernels' only other whole-vector reads of gamma and beta: ln_param's, ln_at's
         kernel = f.read()
     assert kernel.count(".load_first((const W*)p.") == 2 and ".load((const W*)" not in kernel
+
+
+def test_layer_norm_workspace_is_what_the_backward_pass_writes(lib):
+    """a share of dw | db per workgroup that makes one, not per row: with 1024 rows of 40000 / 2^20 / 2^24 channels 312 MiB, 8 GiB and
+    128 GiB would be asked for if every row could leave a share, while about 2048 * 256 vectors of channels are swept"""
+    size = lib.fn("itg_layer_norm_bwd_workspace")
+    for c in (16392, 40000, 1 << 20, 1 << 24):
+        for rows in (1, 7, 96, 1024, 5000, 1 << 20):
+            # shares: one per 8 rows, and no more than 2048 / ceil(vectors / 256) + 1, with vectors of 4 (fp32) or 8 values
+            most = max(min(-(-rows // 8), 2048 // -(-(-(-c // V)) // 256) + 1) for V in (4, 8))
+            assert 0 < size(rows, c) <= most * 2 * c, (rows, c)
+    assert size(1024, 1 << 24) * 4 <= 256 << 20 and size(1024, 40000) * 4 <= 64 << 20
+    for c, groups in ((9001, 256), (16384, 256), (4000, 512), (52, 1024), (3, 256)):      # rows in registers: workgroups of 1024, 512 and 256 threads, the last with 16 or 64 rows a turn and four turns at least
+        assert size(1 << 16, c) == groups * 2 * c, c
+    assert size(1, 52) == 2 * 52 and size(1 << 40, 1) > 0 and size(0, 8) == -1 and size(8, (1 << 24) + 1) == -1

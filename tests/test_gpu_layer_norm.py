@@ -506,3 +506,28 @@ def test_nothing_behind_the_parameters_counts(ops, t, dt, tw, pdt, act):
     want = torch.autograd.grad(ys, [xs] + ps, dy[:, :c].contiguous())
     assert torch.equal(y[:, :c], ys) and not y[:, c:].any()
     assert torch.equal(dx[:, :c], want[0]) and not dx[:, c:].any() and torch.equal(dw, want[1]) and torch.equal(db, want[2])
+
+
+@pytest.mark.parametrize("rows,c,pad", [(1, 1, 0), (9, 3, 1), (3000, 7, 1), (70, 52, 0), (2000, 1023, 1), (700, 2056, 0), (900, 5000, 0), (600, 9001, 7),
+                                        (300, 16384, 0), (40, 9001, 0), (1030, 16392, 0), (96, 40000, 0), (3, 70001, 0)])
+@pytest.mark.parametrize("t,dt", [(torch.float32, 0), (torch.bfloat16, 1)])
+def test_workspace_is_not_written_past_its_end(ops, rows, c, pad, t, dt):
+    """a workspace of the queried size and not a float more, in a buffer whose rest stays as it is; the results do not depend on it"""
+    ld = c + pad
+    x, w, b, dy = make(rows, ld, t, torch.float32, seed=rows)
+    w, b = w[:c].contiguous(), b[:c].contiguous()
+    n = ops._lib.fn("itg_layer_norm_bwd_workspace")(rows, c)
+    buf = torch.full((n + 4096,), 3.0, device="cuda")
+    y, stat, dx = torch.empty_like(x), torch.empty(2 * rows, device="cuda"), torch.empty_like(x)
+    dw, db = torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+    assert call("itg_layer_norm_fwd", x, ld, w, b, y, ld, stat, rows, c, pad, dt, 0, 1e-5, 0, 0.0) == 0
+    assert call("itg_layer_norm_bwd", x, ld, dy, ld, stat, w, b, dx, ld, dw, db, 0, rows, c, pad, dt, 0, 0, 0.0, buf, n) == 0
+    assert call("itg_layer_norm_bwd", x, ld, dy, ld, stat, w, b, dx, ld, dw, db, 0, rows, c, pad, dt, 0, 0, 0.0, buf, n - 1) == -4
+    assert torch.equal(buf[n:], torch.full((4096,), 3.0, device="cuda"))
+    other, more = [torch.empty_like(v) for v in (dx, dw, db)], torch.empty(4 * n + 4096, device="cuda")
+    assert call("itg_layer_norm_bwd", x, ld, dy, ld, stat, w, b, other[0], ld, other[1], other[2], 0, rows, c, pad, dt, 0, 0, 0.0, more, more.numel()) == 0
+    for p, q in zip((dx, dw, db), other):
+        assert torch.equal(p, q)
+    want, _ = oracle(x[:, :c].double(), w.double(), b.double(), dy[:, :c].double(), 1e-5, 0, 0.0, t, torch.float32)
+    near(dw, want[2], "dw")
+    near(db, want[3], "db")
