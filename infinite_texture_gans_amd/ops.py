@@ -10,6 +10,7 @@ import os
 import weakref
 
 import torch
+from torch.autograd import forward_ad as _fwd_ad
 
 from . import _lib
 from ._lib import Tensor as _T, ConvGeom as _G, PAD_ZERO, PAD_REPLICATE, ACT_NONE, ACT_LRELU, ACT_TANH  # noqa: F401
@@ -1269,7 +1270,7 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, slope=0.0, sink
     ``gamma`` / ``beta``: one value per channel, contiguous, float32 or x's type, both alike; None = 1 / 0.  Statistics and sums are
     fp32.  No running statistics: training and evaluation are the same function.  ``sinks`` = (gamma.grad, beta.grad) buffers
     the backward accumulates into.  The activation's derivative at 0 is that of its negative side.  A NaN or an infinity in a
-    row makes that row NaN.  No second derivatives.  A backward pass is captured into a graph only while no eager graph of the
+    row makes that row NaN.  No second derivatives, and none in forward mode (both refused).  A backward pass is captured into a graph only while no eager graph of the
     same leaves lives (torch's rule for every function of its tape)."""
     grid = isinstance(x, GT)
     t, c = (x.t, x.c) if grid else (x, x.shape[-1] if x.dim() else 0)
@@ -1290,6 +1291,8 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, slope=0.0, sink
     if sinks is not None and (gamma is None or beta is None or any(s is None or s.dtype != gamma.dtype or tuple(s.shape) != (c,)
                                                                    or not s.is_contiguous() or s.device != t.device for s in sinks)):
         raise _lib.ItgError("layer_norm: sinks are two contiguous buffers like gamma and beta")
+    if _fwd_ad._current_level >= 0 and any(v is not None and _fwd_ad.unpack_dual(v).tangent is not None for v in (t, gamma, beta)):
+        raise _lib.ItgError("layer_norm: no forward-mode derivatives")
     if torch.is_grad_enabled() and (t.requires_grad or (gamma is not None and gamma.requires_grad) or (beta is not None and beta.requires_grad)):
         y = _LayerNorm.apply(t, gamma, beta, (c, float(eps), int(act), float(slope), sinks))
     else:      # no tape: a quarter of the host's time for a call

@@ -531,3 +531,29 @@ def test_workspace_is_not_written_past_its_end(ops, rows, c, pad, t, dt):
     want, _ = oracle(x[:, :c].double(), w.double(), b.double(), dy[:, :c].double(), 1e-5, 0, 0.0, t, torch.float32)
     near(dw, want[2], "dw")
     near(db, want[3], "db")
+
+
+def test_forward_mode_derivatives_are_refused(ops):
+    """a tangent of x, gamma or beta would be lost on the way: with and without a tape, in no_grad, of a GT and through torch.func"""
+    import torch.autograd.forward_ad as fwd
+    from infinite_texture_gans_amd._lib import ItgError
+    x, w, b = torch.randn(4, 8, device="cuda"), torch.randn(8, device="cuda"), torch.randn(8, device="cuda")
+    plain = ops.layer_norm(x, w, b)
+    with fwd.dual_level():
+        for k in range(3):
+            args = [fwd.make_dual(v, torch.ones_like(v)) if i == k else v for i, v in enumerate((x, w, b))]
+            taped = [a.detach().requires_grad_() if i != k else a for i, a in enumerate(args)]
+            for call_args in (args, taped):
+                with pytest.raises(ItgError, match="forward"):
+                    ops.layer_norm(*call_args)
+                with torch.no_grad(), pytest.raises(ItgError, match="forward"):
+                    ops.layer_norm(*call_args)
+        grid = fwd.make_dual(x.view(1, 1, 1, 1, 4, 8), torch.ones(1, 1, 1, 1, 4, 8, device="cuda"))
+        with pytest.raises(ItgError, match="forward"):
+            ops.layer_norm(ops.GT(grid, 8), w, b)
+        assert torch.equal(ops.layer_norm(x, w, b), plain)                       # no tangent, nothing to lose
+        xs = x.clone().requires_grad_()
+        assert torch.equal(ops.layer_norm(xs, w, b), plain)
+    with pytest.raises(Exception):
+        torch.func.jvp(lambda v: ops.layer_norm(v, w, b), (x,), (torch.ones_like(x),))
+    assert torch.equal(ops.layer_norm(x, w, b), plain)
