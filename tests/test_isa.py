@@ -69,3 +69,18 @@ def test_strip_drop_sentinel_survives_any_row_offset():
     # the old form, for the record: wraps into range for a 3.2 GB tensor's upper rows
     out_bytes, ob = 3_200_000_000, 2_000_000_000
     assert (out_bytes + ob) % 2 ** 32 < out_bytes
+
+
+@pytest.mark.skipif(shutil.which(HIPCC) is None, reason="hipcc not installed")
+def test_strip_kernels_as_they_are_built(tmp_path):
+    """The checks above on the code that goes into the library: the build's own flags, under which no packed fp32 instruction is
+    formed (the flags of `_isa` leave them on)."""
+    import __graft_entry__ as g
+    src, out = os.path.join(CSRC, "conv_strip.hip"), os.path.join(str(tmp_path), "built.s")
+    flags = [f for f in g.FLAGS if f not in ("-fPIC", "-fvisibility=hidden")]
+    subprocess.run([g.HIPCC] + flags + ["--cuda-device-only", "-S", src, "-o", out], cwd=CSRC, check=True, stdout=subprocess.PIPE, stderr=subprocess.PIPE)
+    with open(out) as f:
+        lines = f.read().splitlines()
+    stores = [STORE.match(l) for l in lines if "buffer_store_dwordx4" in l]
+    assert len(stores) >= 24 and all(m is not None and m.group(4).rstrip(",") == "0" and "offen" in m.group(5) for m in stores)
+    assert not [l for l in lines if re.match(r"\s*v_pk_(add|mul|fma)_f32\b", l)]
