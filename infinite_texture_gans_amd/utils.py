@@ -85,13 +85,17 @@ _FLAGS = [
 ]
 
 
+# abbreviations that named one flag until --muon_* and --optimizer came
+_SHORT = {"map_dim": ("--m",), "outer_padding": ("--o",)}
+
+
 def prepare_parser():
     parser = argparse.ArgumentParser()
     for name, typ, default, hlp in _FLAGS:
         if typ == "flag":
             parser.add_argument("--" + name, action="store_true", default=default, help=hlp)
         else:
-            parser.add_argument("--" + name, type=typ, default=default, help=hlp)
+            parser.add_argument("--" + name, *_SHORT.get(name, ()), type=typ, default=default, help=hlp)
     parser.add_argument("--gpu_list", nargs="+", default=None, type=int, help="kept for CLI compatibility")
     return parser
 
