@@ -1768,10 +1768,13 @@ def _ns_coefficients(coefficients, steps):
     return (C.c_float * (3 * len(co)))(*[float(v) for c in co for v in c]), len(co)
 
 
+_NS_SIZES = "Newton-Schulz: matrices of 1 .. %d rows and columns, fewer than 2^22 of them, expected" % _lib.NS_MAX_DIM
+
+
 def _ns_workspace(jobs, n, dtype, device):
     need = _lib.fn("itg_newton_schulz_workspace")(jobs, n, dtype)
     if need < 0:
-        raise _lib.ItgError("Newton-Schulz: matrices of 1 .. %d rows and columns, fewer than 2^22 of them, expected" % _lib.NS_MAX_DIM)
+        raise _lib.ItgError(_NS_SIZES)
     return torch.empty(need, device=device, dtype=torch.uint8), need
 
 
@@ -1784,14 +1787,16 @@ def orthogonalize(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-12, out=None)
     step.  A matrix with a norm of ``eps`` or less has no direction and gives zeros; one with a NaN or an infinity gives NaN.
     ``out``: a contiguous tensor like ``g`` for the result, which may be ``g`` itself where that is contiguous and otherwise lies
     outside the memory that ``g`` spans."""
-    if not g.is_cuda or g.dtype not in _DTYPES:
-        raise _lib.ItgError("orthogonalize: a float32, bfloat16 or float16 tensor on the GPU expected, got %s on %s" % (g.dtype, g.device))
     if g.dim() < 2:
         raise _lib.ItgError("orthogonalize: matrices (..., rows, columns) expected, got shape %s" % (tuple(g.shape),))
+    rows, cols = g.shape[-2:]
+    if g.numel() and (rows > _lib.NS_MAX_DIM or cols > _lib.NS_MAX_DIM or g.numel() >= rows * cols << 31):      # (a job counts in 32 bits)
+        raise _lib.ItgError(_NS_SIZES)
+    if not g.is_cuda or g.dtype not in _DTYPES:
+        raise _lib.ItgError("orthogonalize: a float32, bfloat16 or float16 tensor on the GPU expected, got %s on %s" % (g.dtype, g.device))
     if not eps >= 0.0:
         raise _lib.ItgError("orthogonalize: negative eps %r" % (eps,))
     co, steps = _ns_coefficients(coefficients, steps)
-    rows, cols = g.shape[-2:]
     if out is not None and (out.shape != g.shape or out.dtype != g.dtype or out.device != g.device or not out.is_contiguous()
                             or (out.data_ptr() == g.data_ptr() and not g.is_contiguous())):
         raise _lib.ItgError("orthogonalize: out must be a contiguous tensor of g's shape, type and device")
@@ -1847,6 +1852,11 @@ class MuonPlan:
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise _lib.ItgError("MuonPlan: the parameters must live on the GPU: this build has no CPU path")
+        sizes = "MuonPlan: matrices of 1 .. %d rows and columns expected, got %s" % (_lib.NS_MAX_DIM, self.shapes)
+        if any(not 1 <= v <= _lib.NS_MAX_DIM for shape in self.shapes for v in shape):      # (a job counts in 32 bits)
+            raise _lib.ItgError(sizes)
+        if offset + sum(r * c for r, c in self.shapes) > 1 << 60:
+            raise _lib.ItgError("MuonPlan: the offset %d is out of range" % offset)
         jobs, at = [], int(offset)
         for r, c in self.shapes:
             jobs.append(_lib.NsJob(r, c, 1, 0, at, c, 0, at, c, 0))
@@ -1858,7 +1868,7 @@ class MuonPlan:
             arr = (_lib.NsJob * len(part))(*part)
             size = _lib.fn("itg_newton_schulz_workspace")(arr, len(part), _lib.DT_F32)
             if size < 0:
-                raise _lib.ItgError("MuonPlan: matrices of 1 .. %d rows and columns expected, got %s" % (_lib.NS_MAX_DIM, self.shapes))
+                raise _lib.ItgError(sizes)
             self.calls.append((arr, len(part)))
             need = max(need, size)
         self.workspace = torch.empty(need, device=self.device, dtype=torch.uint8)

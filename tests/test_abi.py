@@ -293,3 +293,21 @@ def test_layer_norm_workspace_is_what_the_backward_pass_writes(lib):
     for c, groups in ((9001, 256), (16384, 256), (4000, 512), (52, 1024), (3, 256)):      # rows in registers: workgroups of 1024, 512 and 256 threads, the last with 16 or 64 rows a turn and four turns at least
         assert size(1 << 16, c) == groups * 2 * c, c
     assert size(1, 52) == 2 * 52 and size(1 << 40, 1) > 0 and size(0, 8) == -1 and size(8, (1 << 24) + 1) == -1
+
+
+def test_matrix_sizes_past_32_bits_are_refused():
+    """The jobs count rows, columns and matrices in 32 bits: a size that does not fit would be cut to another one (2^32 + 4 rows to 4,
+    and the rest of the result left as it was).  The sizes are looked at before the device, so this runs without one: the tensors
+    are expanded from one value."""
+    import torch
+    from infinite_texture_gans_amd import ops
+    from infinite_texture_gans_amd._lib import ItgError
+    one = torch.zeros(1, 1, 1)
+    for shape in ((2 ** 32 + 3, 1, 1), (2 ** 31, 1, 1), (1, 2 ** 32 + 4, 3), (1, 3, 2 ** 32 + 4), (2 ** 20, 2 ** 12 + 1, 1, 1)):
+        with pytest.raises(ItgError, match="matrices"):
+            ops.orthogonalize(one.expand(*shape))
+    for shapes in ([(2 ** 32 + 4, 8)], [(8, 2 ** 32 + 4)], [(4, 8), (65537, 1)], [(-1, 4)]):
+        with pytest.raises(ItgError, match="rows and columns"):
+            ops.MuonPlan(shapes, "cuda")
+    with pytest.raises(ItgError, match="offset"):
+        ops.MuonPlan([(4, 8)], "cuda", offset=2 ** 61)
