@@ -1275,6 +1275,8 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, slope=0.0, sink
     grid = isinstance(x, GT)
     t, c = (x.t, x.c) if grid else (x, x.shape[-1] if x.dim() else 0)
     if grid:
+        if c > t.shape[-1] or t.shape[-1] - c > _lib.LN_MAX_C:
+            raise _lib.ItgError("layer_norm: %d channels of %d values a row (0 .. %d behind them are supported)" % (c, t.shape[-1], _lib.LN_MAX_C))
         _req_cuda(t, "layer_norm input")
     elif not t.is_cuda or t.dtype not in _DTYPES:
         raise _lib.ItgError("layer_norm: x must be a float32, bfloat16 or float16 tensor on the GPU, got %s on %s" % (t.dtype, t.device))

@@ -311,3 +311,16 @@ def test_matrix_sizes_past_32_bits_are_refused():
             ops.MuonPlan(shapes, "cuda")
     with pytest.raises(ItgError, match="offset"):
         ops.MuonPlan([(4, 8)], "cuda", offset=2 ** 61)
+
+
+def test_layer_norm_padding_past_32_bits_is_refused():
+    """the padding of a pixel is counted in 32 bits too; looked at before the device"""
+    import torch
+    from infinite_texture_gans_amd import ops
+    from infinite_texture_gans_amd._lib import ItgError
+    one = torch.zeros(1, 1, 1, 1, 1, 1)
+    for ld in (2 ** 32 + 8, 2 ** 24 + 9):
+        with pytest.raises(ItgError, match="values a row"):
+            ops.layer_norm(ops.GT(one.expand(1, 1, 1, 1, 1, ld), 8))
+    with pytest.raises(ItgError, match="channels"):
+        ops.layer_norm(ops.GT(one.expand(1, 1, 1, 1, 1, 8), 9))
