@@ -461,7 +461,7 @@ int64_t itg_newton_schulz_workspace(const itg_ns_job* jobs, int n, int dtype);
 int itg_newton_schulz(const itg_ns_job* jobs, int n, int dtype, const void* g, void* out, int steps, const float* coefficients,
                       float eps, void* workspace, int64_t workspace_bytes, void* stream);
 /* One optimiser step over fp32 matrices that live in flat buffers (job: count 1, contiguous, in_offset == out_offset, the same
- * offset in param, g, momentum and ema, which are four buffers; no two jobs overlap):
+ * offset in param, g, momentum and ema; no two jobs overlap, and no matrix of one buffer shares a value with one of another):
  *   momentum <- mu momentum + g;  U = nesterov ? g + mu momentum : momentum;  O = Newton-Schulz(U);
  *   param <- (1 - lr weight_decay) param - lr sqrt(max(1, rows / cols)) O;  ema <- ema_decay ema + (1 - ema_decay) param (ema may be NULL)
  * workspace as itg_newton_schulz with ITG_F32.                                                                               */

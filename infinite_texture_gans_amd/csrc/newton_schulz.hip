@@ -918,6 +918,28 @@ int ns_run(NsArgs& p, const NsPlan& pl, const float* abc, int steps, hipStream_t
   return ITG_OK;
 }
 
+// whether two matrices of different buffers share a value
+bool muon_overlap(const itg_ns_job* jobs, int n, const float* const (&buf)[4]) {
+  int64_t lo = jobs[0].out_offset, hi = lo;
+  auto size = [](const itg_ns_job& j) { return (int64_t)j.rows * j.cols; };
+  for (int i = 0; i < n; ++i) {
+    lo = jobs[i].out_offset < lo ? jobs[i].out_offset : lo;
+    hi = jobs[i].out_offset + size(jobs[i]) > hi ? jobs[i].out_offset + size(jobs[i]) : hi;
+  }
+  for (int a = 0; a < 4; ++a)
+    for (int b = 0; b < a; ++b) {
+      if (!buf[a] || !buf[b]) continue;
+      const int64_t apart = (int64_t)((uintptr_t)buf[a] - (uintptr_t)buf[b]);      // bytes from a value of b to a's
+      if (apart >= (hi - lo) * 4 || -apart >= (hi - lo) * 4) continue;
+      for (int i = 0; i < n; ++i)
+        for (int k = 0; k < n; ++k) {
+          const int64_t from = apart + (jobs[i].out_offset - jobs[k].out_offset) * 4;
+          if (from < size(jobs[k]) * 4 && -from < size(jobs[i]) * 4) return true;
+        }
+    }
+  return false;
+}
+
 }  // namespace
 
 extern "C" {
@@ -956,6 +978,8 @@ int itg_muon_step(const itg_ns_job* jobs, int n, float* param, const float* g, f
   NsArgs p; NsPlan pl;
   const int rc = ns_plan(jobs, n, true, p, pl);
   if (rc) return rc;
+  const float* const buf[4] = {param, g, momentum, ema};
+  if (muon_overlap(jobs, n, buf)) return ITG_ERR_ARG;
   if (!ns_coefficients_ok(coefficients, steps)) return ITG_ERR_ARG;
   if (!workspace || workspace_bytes < pl.bytes) return ITG_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return ITG_ERR_ALIGN;

@@ -1863,7 +1863,7 @@ class MuonPlan:
         for r, c in self.shapes:
             jobs.append(_lib.NsJob(r, c, 1, 0, at, c, 0, at, c, 0))
             at += r * c
-        self.end = at          # the buffers hold at least this many values
+        self.begin, self.end = int(offset), at          # the matrices' values; the buffers hold at least `end`
         self.calls, need = [], 0
         for i in range(0, len(jobs), _lib.NS_MAX_JOBS):
             part = jobs[i:i + _lib.NS_MAX_JOBS]
@@ -1887,8 +1887,9 @@ def muon_step(plan, p, g, momentum_buf, ema=None, lr=0.02, momentum=0.95, nester
         _req_cuda(t, "muon_step: " + name)
         if not t.is_contiguous() or t.numel() < plan.end or t.device != p.device:
             raise _lib.ItgError("muon_step: %s must be a contiguous buffer of at least %d values on one device" % (name, plan.end))
-    if len({t.data_ptr() for t in (p, g, momentum_buf, ema) if t is not None}) != (3 if ema is None else 4):
-        raise _lib.ItgError("muon_step: p, g, momentum_buf and ema must be buffers of their own")
+    at = sorted(t.data_ptr() for t in (p, g, momentum_buf, ema) if t is not None)
+    if any(b - a < 4 * (plan.end - plan.begin) for a, b in zip(at, at[1:])):
+        raise _lib.ItgError("muon_step: the matrices of p, g, momentum_buf and ema may not share values")
     if p.device != plan.workspace.device:
         raise _lib.ItgError("muon_step: the plan was made for %s, the parameters are on %s" % (plan.workspace.device, p.device))
     if not eps >= 0.0:

@@ -324,3 +324,29 @@ def test_layer_norm_padding_past_32_bits_is_refused():
             ops.layer_norm(ops.GT(one.expand(1, 1, 1, 1, 1, ld), 8))
     with pytest.raises(ItgError, match="channels"):
         ops.layer_norm(ops.GT(one.expand(1, 1, 1, 1, 1, 8), 9))
+
+
+def test_muon_buffers_that_share_values_are_refused(lib):
+    """param, gradient, momentum and EMA of a step are read and written by different workgroups: matrices of two of them that share a
+    value have no order.  Buffers that only interleave, their matrices beside each other, are fine (ws None: the check behind)."""
+    so = lib.load()
+    f, p = ctypes.c_float, ctypes.c_void_p
+    co = (f * 3)(3.4445, -4.7750, 2.0315)
+
+    def step(at, jobs=((0, 4, 8),)):
+        arr = (lib.NsJob * len(jobs))(*[lib.NsJob(r, c, 1, 0, o, c, 0, o, c, 0) for o, r, c in jobs])
+        return so.itg_muon_step(arr, len(jobs), *[p(4096 + 4 * a) if a is not None else None for a in at], f(0.1), f(0.9), 1, f(0.0), f(0.9), 1, co, f(0.0),
+                                None, 0, None)
+
+    assert step((0, 32, 64, 96)) == -4 and step((96, 64, 32, 0)) == -4 and step((0, 32, 64, None)) == -4
+    for other in range(1, 4):
+        for shift in (1, 31, -1, -31):
+            at = [1000, 2000, 3000, 4000]
+            for k in range(4):
+                if k != other:
+                    at[other] = at[k] + shift
+                    assert step(at) == -1, at
+            at[other] = 1000 * (other + 1)
+    # two matrices with room between them for the other buffers' matrices
+    two = ((0, 4, 8), (200, 4, 8))
+    assert step((0, 32, 64, 96), two) == -4 and step((0, 32, 64, 190), two) == -1 and step((0, 231, 400, 800), two) == -1 and step((0, 232, 400, 800), two) == -4

@@ -362,3 +362,28 @@ def test_bf16_results_are_rounded_once(ops, m, n):
     e = max(3 * rel(steps_of(g.float()), want), 2e-6)
     off, once = rel(ops.orthogonalize(g.cuda()).cpu(), want), rel(want.bfloat16(), want)
     assert off <= once + 2 * e, (off, once, e)
+
+
+def test_steps_on_overlapping_buffers_are_refused(ops):
+    """buffers that share values of the plan's matrices, also where the library takes a plan in several calls; slices side by side of
+    one allocation, and buffers that overlap outside the matrices, are steps like any other"""
+    from infinite_texture_gans_amd._lib import ItgError
+    for shapes, offset in (([(4, 8)], 5), ([(3, 5)] * 70, 0)):
+        n = sum(r * c for r, c in shapes)
+        plan = ops.MuonPlan(shapes, "cuda", offset=offset)
+        buf = torch.randn(12 * (n + 16), device="cuda") * 1e-3
+        size = offset + n
+        before = buf.clone()
+        for shift in (1, n - 1):
+            for a, b in ((0, 1), (0, 2), (0, 3), (1, 2), (1, 3), (2, 3)):
+                at = [k * 2 * (n + 16) for k in range(4)]
+                at[b] = at[a] + shift
+                with pytest.raises(ItgError):
+                    ops.muon_step(plan, *[buf[i:i + size] for i in at])
+        assert torch.equal(buf, before)
+        at = [0, n, 2 * n, 3 * n]                  # the values in front of a plan's matrices may be another buffer's matrices
+        got, alone = [buf[i:i + size] for i in at], [buf[i:i + size].clone() for i in at]
+        ops.muon_step(plan, *got, lr=0.1)
+        ops.muon_step(ops.MuonPlan(shapes, "cuda", offset=offset), *alone, lr=0.1)
+        for x, y in zip(got, alone):
+            assert torch.equal(x[offset:], y[offset:])
