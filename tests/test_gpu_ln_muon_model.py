@@ -240,3 +240,101 @@ def test_row_sharded_steps_equal_the_plain_ones(tmp_path):
                     assert float((got - v).abs().max()) <= 2 * 2e-4 * 2 + 1e-6, k
                 else:
                     assert rel_l2(got, v) < 2e-3, (k, rel_l2(got, v))
+
+
+# Gains, shifts and biases, whose Adam steps hide a gradient's size: the gradients themselves are compared (with 5e-3 where other
+# kernels run or sums have another order: fp32 rounding is 1e-5 there, and an activation within rounding of zero that takes the other
+# slope moves a gradient of these small nets by some 1e-3), and every value has to have moved by the step that its own gradient and
+# second moment give.  That step is computed in 64 bits; the kernel's is off by its fp32 operations (six roundings of it at most,
+# below 1e-6) and by the rounding of the value it is taken from.
+def vectors_moved(flat, before, v_before, opt, t, lr=2e-4, eps=1e-8):
+    n = flat.vectors
+    assert n > 0
+    b2 = float(torch.tensor(0.999, dtype=torch.float32))
+    g, v0, p0, p1 = (x[:n].cpu().double() for x in (flat.grad, v_before, before, flat.data))
+    v = b2 * v0 + (1 - b2) * g * g
+    step = -lr * g / (torch.sqrt(v) / (1 - b2 ** t) ** 0.5 + eps)
+    assert float(((p1 - p0) - step).abs().max()) <= 1e-5 * lr + 2 * 2.0 ** -24 * float(p0.abs().max())
+    assert float((v - opt.v.cpu().double()).abs().max()) <= 1e-6 * float(v.max())
+    # they have moved: in the first step every value whose gradient stands above eps by lr, later a value by sqrt(2) lr times the ratio
+    # of its gradients (which may be small for one of them)
+    assert float((g.abs() > 1e-6).double().mean()) > 0.9 and float((p1 - p0).abs().mean()) > 0.1 * lr
+
+
+def vector_gradients(net):
+    return {k: p.grad.cpu().clone() for k, p in net.named_parameters() if p.dim() < 2}
+
+
+def close_gradients(got, want):
+    assert set(got) == set(want)
+    live = 0
+    for k, g in want.items():
+        if float(g.abs().max()) < 1e-9:
+            assert float(got[k].abs().max()) < 1e-9, k
+            continue
+        live += 1
+        assert rel_l2(got[k], g) < 5e-3, (k, rel_l2(got[k], g))
+    assert live >= 0.9 * len(want)
+
+
+def test_vectors_of_a_replayed_step():
+    """the replay's gains, shifts and biases: the gradients of the same step launched eagerly, and Adam's step of them"""
+    from infinite_texture_gans_amd.engine import Trainer
+    nets = [build(BASE) for _ in range(2)]
+    trs = [Trainer(G, D, args_of("--smooth", "--optimizer", "muon"), cuda) for G, D in nets]
+    batches = [tuple(t.to(cuda) for t in inputs(BASE, s)) for s in range(3)]
+    for tr in trs:
+        tr.step(*batches[0])
+    trs[0].capture(*batches[0], warmup=0)
+    for t in (2, 3):
+        before = [[(f.data.clone(), o.v.clone()) for f, o in ((tr.flatG, tr.optG), (tr.flatD, tr.optD))] for tr in trs]
+        trs[0].step_graphed(*batches[t - 1])
+        trs[1].step(*batches[t - 1])
+        torch.cuda.synchronize()
+        for tr, was in zip(trs, before):
+            for flat, opt, (p0, v0) in ((tr.flatG, tr.optG, was[0]), (tr.flatD, tr.optD, was[1])):
+                vectors_moved(flat, p0, v0, opt, t)
+        if t == 2:                 # (later steps start from weights that differ by rounding, amplified)
+            for a, b in zip(*nets):
+                close_gradients(vector_gradients(a), vector_gradients(b))
+
+
+def _first_step(rank, world, port, out):
+    import os
+    import sys
+    sys.path.insert(0, os.path.dirname(__file__))
+    import torch.distributed as dist
+    from infinite_texture_gans_amd.engine import BandTrainer, Trainer
+    from infinite_texture_gans_amd.dist import BandComm
+    if world > 1:
+        os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+        dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        G, D = build(BASE)
+        args = args_of("--smooth", "--optimizer", "muon")
+        tr = BandTrainer(G, D, args, cuda, BandComm(rank, world)) if world else Trainer(G, D, args, cuda)
+        before = [f.data.clone() for f in (tr.flatG, tr.flatD)]
+        real, z = inputs(BASE, 0)
+        k = real.shape[0] // max(1, world)
+        tr.step(real[rank * k:(rank + 1) * k].to(cuda), z.to(cuda))
+        torch.cuda.synchronize()
+        for flat, opt, p0 in ((tr.flatG, tr.optG, before[0]), (tr.flatD, tr.optD, before[1])):
+            vectors_moved(flat, p0, torch.zeros_like(p0), opt, 1)
+        torch.save([vector_gradients(net) for net in (G, D)], "%s.%d.%d" % (out, world, rank))
+    finally:
+        if world > 1:
+            dist.destroy_process_group()
+
+
+def test_vectors_of_row_sharded_steps(tmp_path):
+    """the first step's gradients of gains, shifts and biases on one rank of patch rows and on two, against the plain step's"""
+    import torch.multiprocessing as mp
+    from test_gpu_model import free_port
+    out = str(tmp_path / "v")
+    _first_step(0, 0, 0, out)
+    _first_step(0, 1, 0, out)
+    mp.spawn(_first_step, args=(2, free_port(), out), nprocs=2, join=True)
+    plain = torch.load(out + ".0.0")
+    for name in (".1.0", ".2.0", ".2.1"):
+        for got, want in zip(torch.load(out + name), plain):
+            close_gradients(got, want)
