@@ -557,3 +557,28 @@ def test_forward_mode_derivatives_are_refused(ops):
     with pytest.raises(Exception):
         torch.func.jvp(lambda v: ops.layer_norm(v, w, b), (x,), (torch.ones_like(x),))
     assert torch.equal(ops.layer_norm(x, w, b), plain)
+
+
+@pytest.mark.parametrize("rows,c,t,groups", [((1 << 17) + 5, 2056, "bf16", 512), (1 << 17, 4096, "bf16", 512), (70001, 9001, "bf16", 256), (1 << 18, 416, "f32", 1024),
+                                             (100003, 52, "f32", 1024)])
+def test_long_column_sums(ops, rows, c, t, groups):
+    """Gradients of gamma and beta over many rows against 64-bit sums.  A channel's sum passes through the rows that one thread sees
+    (of `groups` workgroups, as the workspace says), the row groups and waves of its workgroup (9 additions at most), 16 shares of
+    a lane at most, and 6 steps of the last tree; each addition is off by half a step of a sum that the terms' sizes bound."""
+    assert ops._lib.fn("itg_layer_norm_bwd_workspace")(rows, c) == groups * 2 * c
+    t, depth = TYPES[t], -(-rows // groups) + 9 + 16 + 6
+    x, w, b, dy = make(rows, c, t, torch.float32, seed=c)
+    _, (_, dw, db) = run(ops, x, w, b, dy)
+    want, size, error = torch.zeros(2, c, device="cuda", dtype=torch.float64), torch.zeros(2, c, device="cuda", dtype=torch.float64), torch.zeros(c, device="cuda", dtype=torch.float64)
+    for k in range(0, rows, 1 << 12):
+        xs, du = x[k:k + (1 << 12)].double(), dy[k:k + (1 << 12)].double()
+        mean = xs.mean(1, keepdim=True)
+        r = 1 / torch.sqrt(((xs - mean) ** 2).mean(1, keepdim=True) + 1e-5)
+        xh, d = (xs - mean) * r, c / 64 + 16
+        dmean = (d + 1) * E * xs.abs().mean(1, keepdim=True)
+        exh = dmean * r + xh.abs() * ((d + 10) * E + (dmean * r) ** 2)
+        want += torch.stack([(du * xh).sum(0), du.sum(0)])
+        size += torch.stack([(du * xh).abs().sum(0), du.abs().sum(0)])
+        error += (du.abs() * exh).sum(0)
+    for got, k, more in ((dw, 0, error), (db, 1, 0.0)):
+        near(got, (want[k], depth * E * size[k] + more + E * want[k].abs() + 1e-30), "dw" if k == 0 else "db")
