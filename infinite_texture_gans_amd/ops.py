@@ -1230,7 +1230,7 @@ class _LayerNorm(torch.autograd.Function):
         c, eps, act, slope, sinks = how
         x, ldx = _rows(x)
         y, stat, dt, pdt = _ln_forward(x, ldx, gamma, beta, c, eps, act, slope, True)
-        ctx.meta = (stat.numel() // 2, c, x.shape[-1], ldx, dt, pdt, act, slope, sinks)
+        ctx.meta = (stat.numel() // 2, c, x.shape[-1], dt, pdt, act, slope, sinks)
         ctx.save_for_backward(x, gamma, beta, stat)
         return y
 
@@ -1240,8 +1240,9 @@ class _LayerNorm(torch.autograd.Function):
         if torch.is_grad_enabled():
             raise _lib.ItgError("layer_norm: no second derivatives (create_graph=True)")
         x, gamma, beta, stat = ctx.saved_tensors
-        rows, c, width, ldx, dt, pdt, act, slope, sinks = ctx.meta
+        rows, c, width, dt, pdt, act, slope, sinks = ctx.meta
         need_x, need_g, need_b, _ = ctx.needs_input_grad
+        x, ldx = _rows(x)      # hooks on saved tensors may have brought it back at other strides
         dy, ldy = _rows(dy)
         dx = _dense_like(x) if need_x else None
         acc, dg, db = 0, None, None

@@ -582,3 +582,31 @@ def test_long_column_sums(ops, rows, c, t, groups):
         error += (du.abs() * exh).sum(0)
     for got, k, more in ((dw, 0, error), (db, 1, 0.0)):
         near(got, (want[k], depth * E * size[k] + more + E * want[k].abs() + 1e-30), "dw" if k == 0 else "db")
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_saved_rows_that_come_back_at_another_stride(ops, t):
+    """hooks on saved tensors (offloading, copies) hand the backward pass a contiguous x where rows of a wider buffer were saved: the
+    rows are read at the stride that they have then"""
+    base = torch.randn(5, 300, 70, device="cuda").to(TYPES[t])
+    w, b = torch.randn(33, device="cuda"), torch.randn(33, device="cuda")
+    dy = torch.randn(5, 300, 33, device="cuda").to(TYPES[t])
+
+    def grads(x):
+        leaves = [x.detach().requires_grad_(), w.clone().requires_grad_(), b.clone().requires_grad_()]
+        return torch.autograd.grad(ops.layer_norm(*leaves, act=1, slope=0.1), leaves, dy)
+
+    def widened(v):      # the other way round: contiguous rows that come back inside wider ones
+        out = v.new_full(v.shape[:-1] + (v.shape[-1] + 7,), float("nan"))
+        out[..., 2:2 + v.shape[-1]] = v
+        return out[..., 2:2 + v.shape[-1]]
+    hooks = [lambda: torch.autograd.graph.save_on_cpu(), lambda: torch.autograd.graph.saved_tensors_hooks(lambda v: v.clone().contiguous(), lambda v: v),
+             lambda: torch.autograd.graph.saved_tensors_hooks(lambda v: v.clone(), lambda v: widened(v) if v.dim() == 3 else v),
+             lambda: torch.autograd.graph.saved_tensors_hooks(lambda v: v.clone(), lambda v: v.transpose(0, 1).contiguous().transpose(0, 1) if v.dim() == 3 else v)]
+    for x in (base[..., 1:34], base[..., 1:34].contiguous(), base.transpose(0, 1)[:5, :, :33].expand(5, 5, 33)[:, :1].expand(5, 300, 33)):
+        want = grads(x)
+        for hook in hooks:
+            with hook():
+                got = grads(x)
+            for p, q in zip(got, want):
+                assert torch.equal(p, q)
