@@ -1271,8 +1271,9 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, slope=0.0, sink
     ``gamma`` / ``beta``: one value per channel, contiguous, float32 or x's type, both alike; None = 1 / 0.  Statistics and sums are
     fp32.  No running statistics: training and evaluation are the same function.  ``sinks`` = (gamma.grad, beta.grad) buffers
     the backward accumulates into.  The activation's derivative at 0 is that of its negative side.  A NaN or an infinity in a
-    row makes that row NaN.  No second derivatives, and none in forward mode (both refused).  A backward pass is captured into a graph only while no eager graph of the
-    same leaves lives (torch's rule for every function of its tape)."""
+    row makes that row NaN.  No second derivatives, and none in forward mode (both refused).
+    A backward pass is captured into a graph only while no eager graph of the same leaves lives (torch's rule for every function of its
+    tape)."""
     grid = isinstance(x, GT)
     t, c = (x.t, x.c) if grid else (x, x.shape[-1] if x.dim() else 0)
     if grid:
@@ -1292,8 +1293,9 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, act=ACT_NONE, slope=0.0, sink
     if act not in (ACT_NONE, ACT_LRELU, ACT_TANH) or not eps >= 0.0:
         raise _lib.ItgError("layer_norm: unknown activation %r or negative eps %r" % (act, eps))
     if sinks is not None and (gamma is None or beta is None or any(s is None or s.dtype != gamma.dtype or tuple(s.shape) != (c,)
-                                                                   or not s.is_contiguous() or s.device != t.device for s in sinks)):
-        raise _lib.ItgError("layer_norm: sinks are two contiguous buffers like gamma and beta")
+                                                                   or not s.is_contiguous() or s.device != t.device for s in sinks)
+                              or abs(sinks[0].data_ptr() - sinks[1].data_ptr()) < c * gamma.element_size()):
+        raise _lib.ItgError("layer_norm: sinks are two contiguous buffers like gamma and beta, which share no value")
     if _fwd_ad._current_level >= 0 and any(v is not None and _fwd_ad.unpack_dual(v).tangent is not None for v in (t, gamma, beta)):
         raise _lib.ItgError("layer_norm: no forward-mode derivatives")
     if torch.is_grad_enabled() and (t.requires_grad or (gamma is not None and gamma.requires_grad) or (beta is not None and beta.requires_grad)):

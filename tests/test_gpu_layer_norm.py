@@ -610,3 +610,17 @@ def test_saved_rows_that_come_back_at_another_stride(ops, t):
                 got = grads(x)
             for p, q in zip(got, want):
                 assert torch.equal(p, q)
+
+
+def test_sinks_that_share_values_are_refused(ops):
+    """both would be written by different threads; slices side by side of one buffer are two sinks"""
+    from infinite_texture_gans_amd._lib import ItgError
+    x, w, b, dy = make(40, 26, torch.float32, torch.float32)
+    buf = torch.zeros(80, device="cuda")
+    for at in ((0, 0), (0, 25), (30, 5)):
+        with pytest.raises(ItgError, match="sinks"):
+            ops.layer_norm(x, w, b, sinks=tuple(buf[k:k + 26] for k in at))
+    w, b = w.requires_grad_(), b.requires_grad_()
+    want = torch.autograd.grad(ops.layer_norm(x, w, b), [w, b], dy)
+    ops.layer_norm(x.requires_grad_(), w, b, sinks=(buf[26:52], buf[:26])).backward(dy)
+    assert torch.equal(buf[26:52], want[0]) and torch.equal(buf[:26], want[1])
