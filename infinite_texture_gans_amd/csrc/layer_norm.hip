@@ -218,7 +218,9 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_fwd_kernel(LnP p) {
 // dx, and this workgroup's share of dw | db (`part`), which a thread sums over the rows it sees for the channels it holds.
 // At 16 channels in each of 1024 threads (rows of 8193 .. 16384 16-bit values) the row stays in its own 16 bits between the two
 // sweeps and gamma in its own type, and the next row is fetched behind the last sweep: fp32 copies and a row under way do not fit
-// the 128 registers that 1024 threads have (4096 x 12288 bf16: 88 us, swept three times by the kernels for any length 142).
+// the 128 registers that 1024 threads have.  Nor does this quite: 4 to 12 registers spill without masks, 14 to 47 with masks or an
+// activation (20 to 164 bytes of scratch a thread), some of them reloaded in the row loop (4096 x 12288 bf16: 88 us against 62 of the
+// bytes alone; swept three times by the kernels for any length 142).
 template <typename T, typename W, int V, int TPR, int R, int KIND>
 __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
   constexpr int NT = TPR > 64 ? TPR : 256, GROUPS = NT / TPR;
@@ -301,7 +303,7 @@ __global__ __launch_bounds__(TPR > 64 ? TPR : 256) void ln_bwd_kernel(LnP p) {
     // the next row is on its way while this one is reduced and written
     if (!TIGHT && row + step < p.rows) fetch(row + step);
     if (p.y) {
-      if (TIGHT) { s1 = row_sum<TPR>(s1, red[flip]); s2 = row_sum<TPR>(s2, red[flip + 1]); }      // (both at once spill there)
+      if (TIGHT) { s1 = row_sum<TPR>(s1, red[flip]); s2 = row_sum<TPR>(s2, red[flip + 1]); }      // (both at once spill more)
       else row_sum2<TPR>(s1, s2, red[flip]);
       const float m1 = s1 * inv, m2 = s2 * inv;
       T* dx = (T*)p.y + row * p.ldy;
